@@ -324,7 +324,7 @@ def _prepare_sparse(case, seed):
             "sel": torch.full((rows, hkv, case["budget"]), -1, device=DEV, dtype=torch.int32),
             "out": torch.zeros(rows, hq * d, device=DEV, dtype=torch.bfloat16), "host_lens": lens,
             # the serving engine's workspaces: page scores, split partials
-            "ws": torch.zeros(rows * hkv * (width + 64), device=DEV),
+            "ws": torch.zeros(rows * hkv * 2 * width, device=DEV),
             "part_o": torch.zeros(rows * hq * 32 * d, device=DEV), "part_lse": torch.zeros(rows * hq * 32, device=DEV)}
 
 
