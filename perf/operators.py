@@ -323,9 +323,8 @@ def _prepare_sparse(case, seed):
             "lens": lens_t, "start": lens_t - 1, "bt": bt, "kc": kc, "vc": vc, "bounds": bounds,
             "sel": torch.full((rows, hkv, case["budget"]), -1, device=DEV, dtype=torch.int32),
             "out": torch.zeros(rows, hq * d, device=DEV, dtype=torch.bfloat16), "host_lens": lens,
-            # the serving engine's workspaces: page scores, split partials
-            "ws": torch.zeros(rows * hkv * 2 * width, device=DEV),
-            "part_o": torch.zeros(rows * hq * 32 * d, device=DEV), "part_lse": torch.zeros(rows * hq * 32, device=DEV)}
+            # the serving engine's workspace: page scores
+            "ws": torch.zeros(rows * hkv * 2 * width, device=DEV)}
 
 
 # ---------------------------------------------------------------------------
@@ -394,9 +393,7 @@ def _run_sparse(s):
         ops = _kernels()
         ops.page_bounds(s["kc"], s["bounds"], s["bt"], s["start"], s["lens"], 1)
         ops.attn_select(s["qkv"], s["tok"], s["lens"], s["bt"], s["bounds"], s["sel"], first, last, hq, hkv, s["ws"])
-        splits = ops.sparse_splits(rows, hkv, budget)
-        ops.attn_decode_sparse(s["qkv"], s["out"], s["tok"], s["lens"], s["bt"], s["sel"], s["kc"], s["vc"], hq, hkv,
-                               splits, s["part_o"], s["part_lse"])
+        ops.attn_decode_sparse(s["qkv"], s["out"], s["tok"], s["lens"], s["bt"], s["sel"], s["kc"], s["vc"], hq, hkv)
         return {"bounds": s["bounds"], "sel": s["sel"], "out": s["out"]}
     kc, vc, bounds, group = s["kc"], s["vc"], s["bounds"], hq // hkv
     for r, length in enumerate(s["host_lens"]):
