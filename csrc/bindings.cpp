@@ -8,11 +8,14 @@
 #include <torch/extension.h>
 
 #include "kernels/attention.h"
+#include "kernels/attention_sparse.h"
 #include "kernels/elementwise.h"
 #include "kernels/gemm_bf16.h"
 #include "kernels/gemm_fp8.h"
+#include "kernels/lora.h"
 #include "kernels/moe.h"
 #include "kernels/moe_a2a.h"
+#include "kernels/qk_norm_rope.h"
 #include "kernels/sp_gather.h"
 #include "kernels/runtime.h"
 
@@ -655,6 +658,303 @@ void attn_prefill(const at::Tensor& q, at::Tensor& out, const at::Tensor& q_star
   lf::attn::prefill(a, kcache.data_ptr(), vcache.data_ptr(), stream());
 }
 
+// ---------------------------------------------------------------------------
+// Head norm + rotation + KV write, low-rank adapters, attention over selected pages.
+
+// A CUDA tensor of `t0`'s device with the given dtype and rank.
+void check_op(const at::Tensor& t, const at::Tensor& t0, const char* name, at::ScalarType dt, int64_t dim) {
+  LF_CHECK(t.is_cuda() && t.device() == t0.device(), std::string(name) + " must be a CUDA tensor on the operands' device");
+  LF_CHECK(t.scalar_type() == dt, std::string(name) + " must be " + std::string(c10::toString(dt)));
+  LF_CHECK(t.dim() == dim, std::string(name) + " must have " + std::to_string(dim) + " dimensions");
+}
+// Rows of unit inner stride, 16-byte aligned base and row stride (vector access).
+void check_rows16(const at::Tensor& t, const char* name) {
+  LF_CHECK(t.numel() == 0 || (t.stride(1) == 1 && t.stride(0) * t.element_size() % 16 == 0 &&
+                              reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.size(0) == 1 || t.stride(0) >= t.size(1))),
+           std::string(name) + " rows must be contiguous, 16-byte aligned and apart");
+}
+void check_dense16(const at::Tensor& t, const char* name) {
+  LF_CHECK(t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+           std::string(name) + " must be contiguous and 16-byte aligned");
+}
+void check_ints(const at::Tensor& t, const at::Tensor& t0, const char* name, int64_t count) {
+  check_op(t, t0, name, at::kInt, 1);
+  LF_CHECK(t.is_contiguous() && t.numel() >= count, std::string(name) + " must be contiguous with an entry per row");
+}
+void check_cache(const at::Tensor& t, const at::Tensor& t0, const char* name, int64_t Hkv) {
+  check_op(t, t0, name, at::kBFloat16, 4);
+  LF_CHECK(t.size(0) >= 1 && t.size(1) == Hkv, std::string(name) + " must be [pages, Hkv, page, D]");
+  check_dense16(t, name);
+}
+// The bytes two row-strided tensors can touch do not meet.
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  const char* a0 = static_cast<const char*>(a.data_ptr());
+  const char* b0 = static_cast<const char*>(b.data_ptr());
+  const int64_t an = ((a.size(0) - 1) * a.stride(0) + a.size(1)) * a.element_size();
+  const int64_t bn = ((b.size(0) - 1) * b.stride(0) + b.size(1)) * b.element_size();
+  return a0 + an <= b0 || b0 + bn <= a0;
+}
+bool same_rows(const at::Tensor& a, const at::Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && (a.stride(0) == b.stride(0) || a.size(0) <= 1);
+}
+
+void qk_norm_rope_kv_write(const at::Tensor& qkv, const at::Tensor& q_weight, const at::Tensor& k_weight, double eps,
+                           const at::Tensor& positions, const at::Tensor& slots, const at::Tensor& cos_sin,
+                           at::Tensor& q_out, at::Tensor& kcache, at::Tensor& vcache, int64_t Hq, int64_t Hkv,
+                           int64_t page) {
+  check_op(qkv, qkv, "qkv", at::kBFloat16, 2);
+  check_rows16(qkv, "qkv");
+  LF_CHECK(Hq >= 1 && Hkv >= 1, "qk_norm_rope: head counts");
+  check_cache(kcache, qkv, "kcache", Hkv);
+  check_cache(vcache, qkv, "vcache", Hkv);
+  LF_CHECK(kcache.sizes() == vcache.sizes(), "qk_norm_rope: K and V caches differ in shape");
+  const int64_t T = qkv.size(0), D = kcache.size(3);
+  LF_CHECK(lf::ew::qk_norm_rope_supported((int)D), "qk_norm_rope: head_dim must be 64, 128 or 256");
+  LF_CHECK(page >= 1 && page == kcache.size(2), "qk_norm_rope: page size");
+  LF_CHECK(qkv.size(1) == (Hq + 2 * Hkv) * D, "qk_norm_rope: qkv must hold (Hq + 2 Hkv) heads");
+  check_op(q_weight, qkv, "q_weight", at::kBFloat16, 1);
+  check_op(k_weight, qkv, "k_weight", at::kBFloat16, 1);
+  LF_CHECK(q_weight.numel() == D && k_weight.numel() == D, "qk_norm_rope: weights must be [D]");
+  check_dense16(q_weight, "q_weight");
+  check_dense16(k_weight, "k_weight");
+  LF_CHECK(eps >= 0, "qk_norm_rope: eps must not be negative");
+  check_ints(positions, qkv, "positions", T);
+  check_ints(slots, qkv, "slots", T);
+  check_op(cos_sin, qkv, "cos_sin", at::kFloat, 3);
+  LF_CHECK(cos_sin.size(0) >= 1 && cos_sin.size(1) == D / 2 && cos_sin.size(2) == 2,
+           "qk_norm_rope: cos_sin must be [max_pos, D / 2, 2]");
+  check_dense16(cos_sin, "cos_sin");
+  check_op(q_out, qkv, "q_out", at::kBFloat16, 2);
+  check_rows16(q_out, "q_out");
+  LF_CHECK(q_out.size(0) == T && q_out.size(1) == Hq * D, "qk_norm_rope: q_out must be [T, Hq * D]");
+  LF_CHECK(same_rows(qkv, q_out) || apart(qkv, q_out), "qk_norm_rope: q_out must be the Q columns of qkv or apart from it");
+  LF_CHECK(T < (1ll << 31), "qk_norm_rope: too many rows");
+  c10::cuda::CUDAGuard g(qkv.device());
+  lf::ew::QkNormRopeArgs a{};
+  a.qkv = qkv.data_ptr();
+  a.ld = qkv.stride(0);
+  a.q_out = q_out.data_ptr();
+  a.q_ld = q_out.stride(0);
+  a.q_weight = q_weight.data_ptr();
+  a.k_weight = k_weight.data_ptr();
+  a.positions = positions.data_ptr<int32_t>();
+  a.slots = slots.data_ptr<int32_t>();
+  a.cos_sin = cos_sin.data_ptr();
+  a.kcache = kcache.data_ptr();
+  a.vcache = vcache.data_ptr();
+  a.T = (int)T;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.D = (int)D;
+  a.page = (int)page;
+  a.max_pos = (int)std::min<int64_t>(cos_sin.size(0), INT32_MAX);
+  a.num_slots = kcache.size(0) * page;
+  a.eps = (float)eps;
+  lf::ew::qk_norm_rope_kv_write(a, stream());
+}
+
+void lora_add(const at::Tensor& x, const at::Tensor& lora_a, const at::Tensor& lora_b, const at::Tensor& scales,
+              const at::Tensor& ranks, const at::Tensor& rows, const at::Tensor& starts, const at::Tensor& base,
+              at::Tensor& out, const std::vector<int64_t>& slices) {
+  check_op(x, x, "x", at::kBFloat16, 2);
+  check_rows16(x, "x");
+  check_op(lora_a, x, "lora_a", at::kBFloat16, 3);
+  check_op(lora_b, x, "lora_b", at::kBFloat16, 3);
+  check_dense16(lora_a, "lora_a");
+  check_dense16(lora_b, "lora_b");
+  const int64_t T = x.size(0), K = x.size(1), pool = lora_a.size(0), N = lora_b.size(1), R = lora_b.size(2);
+  const int64_t S = (int64_t)slices.size();
+  LF_CHECK(pool >= 1 && lora_b.size(0) == pool, "lora_add: lora_a and lora_b must hold the same adapters");
+  LF_CHECK(R >= 8 && R <= lf::lora::kMaxRank && R % 8 == 0, "lora_add: rank of the pool must be a multiple of 8 up to 128");
+  LF_CHECK(K >= 8 && K % 8 == 0 && N >= 8 && N % 8 == 0, "lora_add: K and N must be multiples of 8");
+  LF_CHECK(S >= 1 && S <= lf::lora::kMaxSlices, "lora_add: 1 to 4 slices");
+  LF_CHECK(lora_a.size(1) == S * R && lora_a.size(2) == K, "lora_add: lora_a must be [pool, slices * R, K]");
+  const bool f32 = base.scalar_type() == at::kFloat;
+  check_op(base, x, "base", f32 ? at::kFloat : at::kBFloat16, 2);
+  check_op(out, x, "out", f32 ? at::kFloat : at::kBFloat16, 2);
+  check_rows16(base, "base");
+  check_rows16(out, "out");
+  LF_CHECK(base.size(0) == T && base.size(1) == N && out.size(0) == T && out.size(1) == N,
+           "lora_add: base and out must be [T, N]");
+  LF_CHECK(same_rows(base, out) || apart(base, out), "lora_add: out must be base itself or apart from it");
+  LF_CHECK(apart(x, out), "lora_add: out must not overlap x");
+  check_op(scales, x, "scales", at::kFloat, 1);
+  LF_CHECK(scales.is_contiguous() && scales.numel() == pool, "lora_add: a scale per adapter");
+  check_ints(ranks, x, "ranks", pool);
+  check_ints(rows, x, "rows", 0);
+  check_ints(starts, x, "starts", pool + 1);
+  LF_CHECK(starts.numel() == pool + 1, "lora_add: starts must hold pool + 1 offsets");
+  LF_CHECK(rows.numel() <= T, "lora_add: a row is listed at most once");
+  LF_CHECK(T < (1ll << 31) && pool < (1ll << 24) && K < (1ll << 31) && N < (1ll << 31), "lora_add: sizes");
+  c10::cuda::CUDAGuard g(x.device());
+  lf::lora::LoraArgs a{};
+  a.x = x.data_ptr();
+  a.ldx = x.stride(0);
+  a.a = lora_a.data_ptr();
+  a.b = lora_b.data_ptr();
+  a.scales = scales.data_ptr<float>();
+  a.ranks = ranks.data_ptr<int32_t>();
+  a.rows = rows.data_ptr<int32_t>();
+  a.starts = starts.data_ptr<int32_t>();
+  a.base = base.data_ptr();
+  a.ldb = base.stride(0);
+  a.out = out.data_ptr();
+  a.ldo = out.stride(0);
+  a.T = (int)T;
+  a.K = (int)K;
+  a.N = (int)N;
+  a.R = (int)R;
+  a.pool = (int)pool;
+  a.L = (int)rows.numel();
+  a.S = (int)S;
+  a.f32 = f32;
+  int64_t end = 0;
+  for (int64_t i = 0; i < S; ++i) {
+    LF_CHECK(slices[i] >= 8 && slices[i] % 8 == 0, "lora_add: slice widths must be positive multiples of 8");
+    end += slices[i];
+    LF_CHECK(end <= N, "lora_add: slices must add up to N");
+    a.col_end[i] = (int)end;
+  }
+  LF_CHECK(end == N, "lora_add: slices must add up to N");
+  lf::lora::lora_add(a, stream());
+}
+
+// Common checks of the sparse attention operators: rows, table, lengths.
+void check_paged_rows(const at::Tensor& seq_lens, const at::Tensor& block_table, const at::Tensor& t0) {
+  check_op(seq_lens, t0, "seq_lens", at::kInt, 1);
+  LF_CHECK(seq_lens.is_contiguous(), "seq_lens must be contiguous");
+  check_op(block_table, t0, "block_table", at::kInt, 2);
+  LF_CHECK(block_table.size(0) >= seq_lens.numel() && (block_table.size(1) <= 1 || block_table.stride(1) == 1),
+           "block_table must have a row per sequence and unit inner stride");
+  LF_CHECK(seq_lens.numel() <= 65535, "at most 65535 rows");
+  LF_CHECK(block_table.size(1) <= lf::attn::kSparseMaxPages, "block_table: at most 65536 pages a row");
+}
+
+void check_bounds(const at::Tensor& bounds, const at::Tensor& t0, int64_t pages, int64_t Hkv) {
+  check_op(bounds, t0, "bounds", at::kBFloat16, 4);
+  LF_CHECK(bounds.size(0) == pages && bounds.size(1) == Hkv && bounds.size(2) == 2 && bounds.size(3) == 128,
+           "bounds must be [pages, Hkv, 2, 128]");
+  check_dense16(bounds, "bounds");
+}
+
+void page_bounds(const at::Tensor& kcache, at::Tensor& bounds, const at::Tensor& block_table, const at::Tensor& start,
+                 const at::Tensor& seq_lens, int64_t max_new) {
+  check_op(kcache, kcache, "kcache", at::kBFloat16, 4);
+  check_cache(kcache, kcache, "kcache", kcache.size(1));
+  LF_CHECK(kcache.size(2) == 16 && kcache.size(3) == 128, "page_bounds: kcache must be [pages, Hkv, 16, 128]");
+  check_bounds(bounds, kcache, kcache.size(0), kcache.size(1));
+  check_paged_rows(seq_lens, block_table, kcache);
+  check_ints(start, kcache, "start", seq_lens.numel());
+  LF_CHECK(max_new >= 0 && max_new <= lf::attn::kSparseMaxPages * 16, "page_bounds: max_new");
+  LF_CHECK(kcache.size(0) < (1ll << 31), "page_bounds: pages");
+  c10::cuda::CUDAGuard g(kcache.device());
+  lf::attn::BoundsArgs a{};
+  a.kcache = reinterpret_cast<const __nv_bfloat16*>(kcache.data_ptr());
+  a.bounds = reinterpret_cast<__nv_bfloat16*>(bounds.data_ptr());
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.bt_stride = block_table.stride(0);
+  a.start = start.data_ptr<int32_t>();
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.rows = (int)seq_lens.numel();
+  a.Hkv = (int)kcache.size(1);
+  a.width = (int)block_table.size(1);
+  a.num_pages = (int)kcache.size(0);
+  a.max_new = (int)max_new;
+  lf::attn::page_bounds(a, stream());
+}
+
+void attn_select(const at::Tensor& q, const at::Tensor& tok_index, const at::Tensor& seq_lens,
+                 const at::Tensor& block_table, const at::Tensor& bounds, at::Tensor& sel, int64_t first, int64_t last,
+                 int64_t Hq, int64_t Hkv, at::Tensor& ws) {
+  check_op(q, q, "q", at::kBFloat16, 2);
+  check_rows16(q, "q");
+  LF_CHECK(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 16, "attn_select: GQA group of 1 to 16 heads");
+  LF_CHECK(q.size(1) >= Hq * 128, "attn_select: q must hold Hq heads of 128");
+  check_paged_rows(seq_lens, block_table, q);
+  const int64_t rows = seq_lens.numel(), width = block_table.size(1);
+  check_ints(tok_index, q, "tok_index", rows);
+  check_op(bounds, q, "bounds", at::kBFloat16, 4);
+  check_bounds(bounds, q, bounds.size(0), Hkv);
+  check_op(sel, q, "sel", at::kInt, 3);
+  LF_CHECK(sel.is_contiguous() && sel.size(0) == rows && sel.size(1) == Hkv, "attn_select: sel must be [rows, Hkv, budget]");
+  const int64_t budget = sel.size(2);
+  LF_CHECK(first >= 0 && last >= 0 && budget >= 1 && first + last <= budget && budget <= lf::attn::kSparseMaxPages,
+           "attn_select: the budget must hold the first and the last pages and one at least");
+  LF_CHECK(bounds.size(0) >= 1 && bounds.size(0) < (1ll << 31), "attn_select: pages");
+  check_op(ws, q, "ws", at::kFloat, 1);
+  LF_CHECK(ws.is_contiguous() && ws.numel() >= rows * Hkv * width * 2 && reinterpret_cast<uintptr_t>(ws.data_ptr()) % 8 == 0,
+           "attn_select: ws must hold 2 floats per row, KV head and page of the block table");
+  c10::cuda::CUDAGuard g(q.device());
+  lf::attn::SelectArgs a{};
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
+  a.q_ld = q.stride(0);
+  a.tok_index = tok_index.data_ptr<int32_t>();
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.bt_stride = block_table.stride(0);
+  a.bounds = reinterpret_cast<const __nv_bfloat16*>(bounds.data_ptr());
+  a.sel = sel.data_ptr<int32_t>();
+  a.ws = reinterpret_cast<float2*>(ws.data_ptr<float>());
+  a.rows = (int)rows;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.width = (int)width;
+  a.num_pages = (int)bounds.size(0);
+  a.tokens = (int)q.size(0);
+  a.budget = (int)budget;
+  a.first = (int)first;
+  a.last = (int)last;
+  lf::attn::select_pages(a, stream());
+}
+
+void attn_decode_sparse(const at::Tensor& q, at::Tensor& out, const at::Tensor& tok_index, const at::Tensor& seq_lens,
+                        const at::Tensor& block_table, const at::Tensor& sel, const at::Tensor& kcache,
+                        const at::Tensor& vcache, int64_t Hq, int64_t Hkv) {
+  check_op(q, q, "q", at::kBFloat16, 2);
+  check_rows16(q, "q");
+  check_op(out, q, "out", at::kBFloat16, 2);
+  check_rows16(out, "out");
+  LF_CHECK(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 16, "attn_decode_sparse: GQA group of 1 to 16 heads");
+  LF_CHECK(q.size(1) >= Hq * 128 && out.size(1) >= Hq * 128 && out.size(0) >= q.size(0),
+           "attn_decode_sparse: q and out must hold Hq heads of 128 for every token");
+  LF_CHECK(apart(q, out), "attn_decode_sparse: out must not overlap q");
+  check_cache(kcache, q, "kcache", Hkv);
+  check_cache(vcache, q, "vcache", Hkv);
+  LF_CHECK(kcache.size(2) == 16 && kcache.size(3) == 128 && vcache.sizes() == kcache.sizes(),
+           "attn_decode_sparse: caches must be [pages, Hkv, 16, 128]");
+  LF_CHECK(kcache.size(0) < (1ll << 31), "attn_decode_sparse: pages");
+  check_paged_rows(seq_lens, block_table, q);
+  const int64_t rows = seq_lens.numel();
+  check_ints(tok_index, q, "tok_index", rows);
+  check_op(sel, q, "sel", at::kInt, 3);
+  LF_CHECK(sel.is_contiguous() && sel.size(0) == rows && sel.size(1) == Hkv && sel.size(2) >= 1 &&
+               sel.size(2) <= lf::attn::kSparseMaxPages,
+           "attn_decode_sparse: sel must be [rows, Hkv, budget]");
+  c10::cuda::CUDAGuard g(q.device());
+  lf::attn::SparseArgs a{};
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
+  a.q_ld = q.stride(0);
+  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  a.out_ld = out.stride(0);
+  a.tok_index = tok_index.data_ptr<int32_t>();
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.bt_stride = block_table.stride(0);
+  a.sel = sel.data_ptr<int32_t>();
+  a.kcache = reinterpret_cast<const __nv_bfloat16*>(kcache.data_ptr());
+  a.vcache = reinterpret_cast<const __nv_bfloat16*>(vcache.data_ptr());
+  a.rows = (int)rows;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.width = (int)block_table.size(1);
+  a.num_pages = (int)kcache.size(0);
+  a.tokens = (int)q.size(0);
+  a.budget = (int)sel.size(2);
+  a.scale_log2 = (float)(1.4426950408889634 / std::sqrt(128.0));
+  lf::attn::decode_sparse(a, stream());
+}
+
 std::pair<int64_t, int64_t> read_error(bool clear) {
   auto st = lf::rt::read_error(stream(), clear);
   return {st.code, (int64_t)st.info};
@@ -721,6 +1021,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_prefill", &attn_prefill, py::arg("q"), py::arg("out"), py::arg("q_start"), py::arg("seq_lens"),
         py::arg("block_table"), py::arg("kcache"), py::arg("vcache"), py::arg("Hq"), py::arg("Hkv"),
         py::arg("max_q_len"), py::arg("progress") = 0);
+  m.def("qk_norm_rope_kv_write", &qk_norm_rope_kv_write);
+  m.def("lora_add", &lora_add);
+  m.def("page_bounds", &page_bounds);
+  m.def("attn_select", &attn_select);
+  m.def("attn_decode_sparse", &attn_decode_sparse);
   m.def("read_error", &read_error, py::arg("clear") = true);
   m.def("inject_error", &inject_error);
   m.def("set_wait_limit_ns", [](int64_t ns) {

@@ -1,0 +1,145 @@
+// RMS norm of every query and key head, split-half rotation and the paged
+// K / V write in one pass over the QKV projection's output.
+//
+//   y = x * rsqrt(mean_d(x^2) + eps) * w        (w: one [D] weight for Q, one for K)
+//   o[i]       = y[i] cos_i - y[i + D/2] sin_i
+//   o[i + D/2] = y[i + D/2] cos_i + y[i] sin_i   (i < D/2, angles of the token's position)
+//
+// V heads are copied.  All arithmetic is fp32 with one rounding to bf16 at the
+// store; the sum of squares of a head stays in registers.
+//
+// Bound by memory: every head is read once and written once.  D / 8 lanes own
+// one head, 16 bytes each, so the two elements of a rotation pair sit D / 16
+// lanes apart and meet by one shuffle, and the sum of squares is a shuffle
+// reduction over the same lanes: no shared memory and no barrier.  A CTA owns
+// one token; its lanes load the token's (cos, sin) row and the two weights
+// once and keep them while they walk the heads.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <stdexcept>
+
+#include "common.cuh"
+#include "qk_norm_rope.h"
+
+namespace lf {
+namespace ew {
+
+namespace {
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __bfloat1622float2(p[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                    pack_bf16x2(f[6], f[7]));
+}
+
+// Heads whose loads are in flight together per lane group.
+constexpr int kBatch = 4;
+
+template <int D, int NT>
+__global__ void __launch_bounds__(NT) qk_norm_rope_kernel(const QkNormRopeArgs a) {
+  constexpr int kLanes = D / 8;          // lanes of one head
+  constexpr int kGroups = NT / kLanes;   // heads a CTA works on at a time
+  pdl_trigger();
+  pdl_wait();
+  const int t = blockIdx.x;
+  const int group = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
+  const bool upper = l >= kLanes / 2;    // this lane holds elements of the second half
+  const int pair = (l % (kLanes / 2)) * 8;
+  const int heads = a.Hq + 2 * a.Hkv;
+  const uint4* row = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.qkv) + (int64_t)t * a.ld);
+
+  const int pos = a.positions[t];
+  const int slot = a.slots[t];
+  const bool pos_ok = pos >= 0 && pos < a.max_pos;
+  const bool slot_ok = slot >= 0 && (int64_t)slot < a.num_slots;
+  if (threadIdx.x == 0 && (!pos_ok || (slot >= 0 && !slot_ok))) set_error(kErrBadIndex, (unsigned long long)t);
+
+  float cs[8], sn[8];
+  {
+    // a position outside the table is recorded and not rotated
+    const float4* tab = reinterpret_cast<const float4*>(a.cos_sin) + ((int64_t)(pos_ok ? pos : 0) * (D / 2) + pair) / 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = pos_ok ? tab[i] : make_float4(1.f, 0.f, 1.f, 0.f);
+      cs[2 * i] = v.x;
+      sn[2 * i] = upper ? v.y : -v.y;
+      cs[2 * i + 1] = v.z;
+      sn[2 * i + 1] = upper ? v.w : -v.w;
+    }
+  }
+  const uint4 wq = reinterpret_cast<const uint4*>(a.q_weight)[l];
+  const uint4 wk = reinterpret_cast<const uint4*>(a.k_weight)[l];
+
+  const int64_t pg = slot_ok ? slot / a.page : 0;
+  const int off = slot_ok ? slot % a.page : 0;
+  uint4* qrow = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.q_out) + (int64_t)t * a.q_ld);
+
+  for (int h0 = group; h0 - group < heads; h0 += kBatch * kGroups) {   // uniform trip count over the CTA
+    uint4 v[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int h = h0 + b * kGroups;
+      v[b] = h < heads ? row[h * kLanes + l] : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int h = h0 + b * kGroups;
+      if (h - group >= heads) break;     // uniform: no lane group of this CTA has such a head
+      float x[8], w[8], o[8];
+      unpack8(v[b], x);
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+#pragma unroll
+      for (int m = kLanes / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+      const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+      unpack8(h < a.Hq ? wq : wk, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, x[i], kLanes / 2);
+        o[i] = x[i] * cs[i] + other * sn[i];
+      }
+      if (h < a.Hq) {
+        qrow[h * kLanes + l] = pack8(o);
+      } else if (h < heads && slot_ok) {
+        const bool is_k = h < a.Hq + a.Hkv;
+        const int kh = h - a.Hq - (is_k ? 0 : a.Hkv);
+        uint4* dst = reinterpret_cast<uint4*>(is_k ? a.kcache : a.vcache);
+        dst[((pg * a.Hkv + kh) * a.page + off) * kLanes + l] = is_k ? pack8(o) : v[b];
+      }
+    }
+  }
+}
+
+template <int D>
+void launch_d(const QkNormRopeArgs& a, cudaStream_t s) {
+  launch_k(qk_norm_rope_kernel<D, 128>, dim3(a.T), dim3(128), 0, s, 1, a);
+}
+
+}  // namespace
+
+bool qk_norm_rope_supported(int D) { return D == 64 || D == 128 || D == 256; }
+
+void qk_norm_rope_kv_write(const QkNormRopeArgs& a, cudaStream_t s) {
+  if (a.T <= 0) return;
+  if (a.D == 64) launch_d<64>(a, s);
+  else if (a.D == 128) launch_d<128>(a, s);
+  else if (a.D == 256) launch_d<256>(a, s);
+  else throw std::runtime_error("lunaflux qk_norm_rope: head_dim 64, 128 or 256");
+}
+
+}  // namespace ew
+}  // namespace lf

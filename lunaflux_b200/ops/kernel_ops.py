@@ -106,6 +106,77 @@ class KernelOps:
         self.launches += 1
         self.C.sample_keys(keys, rows, ranks, kc, params, out)
 
+    # ------------------------------------------- head norms, adapters, selected pages
+    def qk_norm_rope_kv_write(self, qkv, q_weight, k_weight, eps, positions, slots, cos_sin, q_out, kc, vc, Hq, Hkv,
+                              page):
+        """RMS norm of every query and key head (one [D] weight each), split-half
+        rotation and the paged K / V write in one pass; head_dim 64, 128 or 256.
+        Q goes to ``q_out`` ([T, Hq * D]; ``qkv[:, :Hq * D]`` for in place), K and
+        V to the cache at ``slots`` (-1: no write; a slot appears at most once).
+        A position outside the table or a slot outside the cache is recorded in
+        the error word."""
+        if qkv.shape[0] == 0:
+            return
+        self.launches += 1
+        self.C.qk_norm_rope_kv_write(qkv, q_weight, k_weight, eps, positions, slots, cos_sin, q_out, kc, vc, Hq, Hkv,
+                                     page)
+
+    def lora_add(self, x, lora_a, lora_b, scales, ranks, rows, starts, base, out, slices=None):
+        """Low-rank adapters of many requests beside a shared projection: for the
+        token rows listed in ``rows``, ``out = base + scale * B (A x)`` with the
+        row's adapter.
+
+        x [T, K]; lora_a [pool, S * R, K] and lora_b [pool, N, R] hold the
+        adapters padded to rank R (a multiple of 8 up to 128; what lies past
+        ``ranks[a]`` is not used); scales fp32 and ranks int32 [pool].  ``rows``
+        (int32) groups token rows by adapter, ``starts[a] .. starts[a + 1]``
+        being adapter a's; a row appears at most once, rows without an adapter
+        are not listed and left as they are.  base and out are [T, N], both bf16
+        or both fp32; out may be base.  ``slices`` are the column widths of a
+        stacked projection (e.g. Q, K, V), each with its own R rows of lora_a."""
+        if rows.numel() == 0:
+            return
+        self.launches += 1
+        self.C.lora_add(x, lora_a, lora_b, scales, ranks, rows, starts, base, out,
+                        [lora_b.shape[1]] if slices is None else list(slices))
+
+    def page_bounds(self, kc, bounds, bt, start, seq_lens, max_new):
+        """Smallest and largest key per dimension ([pages, Hkv, 2, D]) of the pages
+        that hold tokens start[r] .. seq_lens[r] of every row, over the row's
+        valid tokens.  ``max_new`` bounds seq_lens - start; call it after each
+        KV write, so that the bounds follow the cache."""
+        if seq_lens.numel() == 0 or max_new == 0:
+            return
+        self.launches += 1
+        self.C.page_bounds(kc, bounds, bt, start, seq_lens, max_new)
+
+    @staticmethod
+    def select_workspace(rows, Hkv, width):
+        """fp32 elements of ``attn_select``'s workspace for block tables of `width` pages."""
+        return 2 * rows * Hkv * width
+
+    def attn_select(self, q, tok, seq_lens, bt, bounds, sel, first, last, Hq, Hkv, ws):
+        """Pages every (row, KV head) attends to: sel [rows, Hkv, budget] int32,
+        logical pages in ascending order, then -1.  All pages where they fit the
+        budget; else the ``first`` first and ``last`` last ones and those of the
+        highest upper bound max_h sum_d max(q_hd lo_d, q_hd hi_d) over the
+        group's query heads, compared exactly, ties to the lowest page.  ``ws``:
+        ``select_workspace`` fp32 elements, used until the call's kernels end."""
+        if seq_lens.numel() == 0:
+            return
+        self.launches += 2 if bt.shape[1] > sel.shape[2] else 1
+        self.C.attn_select(q, tok, seq_lens, bt, bounds, sel, first, last, Hq, Hkv, ws)
+
+    def attn_decode_sparse(self, q, out, tok, seq_lens, bt, sel, kc, vc, Hq, Hkv):
+        """Decode attention over the pages of ``sel``: the first
+        min(pages of the row, budget) entries of every (row, KV head), each
+        page at most once.  A row of length 0 gives zeros; an entry outside the
+        row's pages is recorded in the error word and skipped."""
+        if seq_lens.numel() == 0:
+            return
+        self.launches += 1
+        self.C.attn_decode_sparse(q, out, tok, seq_lens, bt, sel, kc, vc, Hq, Hkv)
+
     # ---------------------------------------------------------------- MoE
     def moe_route(self, h, router, bias, topk, ids, weights):
         self.launches += 1

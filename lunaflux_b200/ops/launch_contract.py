@@ -221,6 +221,58 @@ CONTRACTS: Dict[str, Contract] = {c.op: c for c in (
               _r("GQA group of at most 16 heads", lambda d: d["Hq"] % d["Hkv"] == 0 and d["Hq"] // d["Hkv"] <= 16),
               _r("q / out hold Hq heads", lambda d: d["Nq"] >= d["Hq"] * 128 and d["No"] >= d["Hq"] * 128)),
              params=("Hq",)),
+    Contract("qk_norm_rope_kv_write", "qk_norm_rope_kv_write",
+             (Role("qkv", BF16, ("T", "N")), Role("q_weight", BF16, ("D",)), Role("k_weight", BF16, ("D",)),
+              Role("positions", I32, ("Tp",), rowmajor=False), Role("slots", I32, ("Ts",), rowmajor=False),
+              Role("cos_sin", F32, ("max_pos", "half", 2), rowmajor=False), Role("q_out", BF16, ("T", "Nq")),
+              Role("kcache", BF16, ("pages", "Hkv", "page", "D")), Role("vcache", BF16, ("pages", "Hkv", "page", "D"))),
+             (_r("qkv holds (Hq + 2 Hkv) heads", lambda d: d["N"] == (d["Hq"] + 2 * d["Hkv"]) * d["D"]),
+              _r("q_out holds Hq heads", lambda d: d["Nq"] == d["Hq"] * d["D"]),
+              _r("head_dim 64, 128 or 256, a table entry per pair", lambda d: d["D"] in (64, 128, 256) and d["half"] * 2 == d["D"]),
+              _r("positions / slots cover every row", lambda d: d["Tp"] >= d["T"] and d["Ts"] >= d["T"])),
+             params=("Hq", "Hkv", "page")),
+    Contract("lora_add", "lora_add",
+             (Role("x", BF16, ("T", "K")), Role("lora_a", BF16, ("pool", "SR", "K")),
+              Role("lora_b", BF16, ("pool", "N", "R")), Role("scales", F32, ("pool",), rowmajor=False),
+              Role("ranks", I32, ("pool",), rowmajor=False), Role("rows", I32, ("L",), rowmajor=False),
+              Role("starts", I32, ("P1",), rowmajor=False), Role("base", BF16 + F32, ("T", "N")),
+              Role("out", BF16 + F32, ("T", "N"))),
+             (_r("a pool rank of 8, 16, ..., 128", lambda d: d["R"] % 8 == 0 and 8 <= d["R"] <= 128),
+              _r("R rows of lora_a per slice", lambda d: d["SR"] == d["S"] * d["R"] and 1 <= d["S"] <= 4),
+              _r("slice widths multiples of 8 that add up to N", lambda d: d["Nsum"] == d["N"] and d["Wmod"] == 0),
+              _r("K % 8 == 0 and N % 8 == 0", lambda d: d["K"] % 8 == 0 and d["N"] % 8 == 0),
+              _r("an offset per adapter and the end", lambda d: d["P1"] == d["pool"] + 1),
+              _r("a row listed at most once", lambda d: d["L"] <= d["T"])),
+             params=("S", "Nsum", "Wmod")),
+    Contract("page_bounds", "page_bounds",
+             (Role("kcache", BF16, ("pages", "Hkv", 16, 128)), Role("bounds", BF16, ("pages", "Hkv", 2, 128)),
+              Role("block_table", I32, ("Rb", "W"), rowmajor=False), Role("start", I32, ("Rs",), rowmajor=False),
+              Role("seq_lens", I32, ("R",), rowmajor=False)),
+             (_r("starts and block-table rows per row", lambda d: d["Rs"] >= d["R"] and d["Rb"] >= d["R"]),
+              _r("max_new not negative", lambda d: d["max_new"] >= 0)),
+             params=("max_new",)),
+    Contract("attn_select", "attn_select",
+             (Role("q", BF16, ("Tq", "Nq")), Role("tok_index", I32, ("Rt",), rowmajor=False),
+              Role("seq_lens", I32, ("R",), rowmajor=False), Role("block_table", I32, ("Rb", "W"), rowmajor=False),
+              Role("bounds", BF16, ("pages", "Hkv", 2, 128)), Role("sel", I32, ("R", "Hkv", "budget"), rowmajor=False),
+              Role("ws", F32, ("ws",), rowmajor=False)),
+             (_r("token indices and block-table rows per row", lambda d: d["Rt"] >= d["R"] and d["Rb"] >= d["R"]),
+              _r("GQA group of at most 16 heads", lambda d: d["Hq"] % d["Hkv"] == 0 and d["Hq"] // d["Hkv"] <= 16),
+              _r("q holds Hq heads", lambda d: d["Nq"] >= d["Hq"] * 128),
+              _r("the budget holds the first and last pages", lambda d: d["first"] + d["last"] <= d["budget"]),
+              _r("2 floats of workspace per row, KV head and page", lambda d: d["ws"] >= 2 * d["R"] * d["Hkv"] * d["W"])),
+             params=("Hq", "Hkv", "first", "last")),
+    Contract("attn_decode_sparse", "attn_decode_sparse",
+             (Role("q", BF16, ("Tq", "Nq")), Role("out", BF16, ("To", "No")),
+              Role("tok_index", I32, ("Rt",), rowmajor=False), Role("seq_lens", I32, ("R",), rowmajor=False),
+              Role("block_table", I32, ("Rb", "W"), rowmajor=False),
+              Role("sel", I32, ("R", "Hkv", "budget"), rowmajor=False),
+              Role("kcache", BF16, ("pages", "Hkv", 16, 128)), Role("vcache", BF16, ("pages", "Hkv", 16, 128))),
+             (_r("token indices and block-table rows per row", lambda d: d["Rt"] >= d["R"] and d["Rb"] >= d["R"]),
+              _r("GQA group of at most 16 heads", lambda d: d["Hq"] % d["Hkv"] == 0 and d["Hq"] // d["Hkv"] <= 16),
+              _r("q / out hold Hq heads", lambda d: d["Nq"] >= d["Hq"] * 128 and d["No"] >= d["Hq"] * 128),
+              _r("an output row per token", lambda d: d["To"] >= d["Tq"])),
+             params=("Hq", "Hkv")),
     Contract("argmax", "argmax",
              (Role("logits", F32, ("R", "V")), Role("out", I32, ("Ro",), rowmajor=False)),
              (_r("a token per row", lambda d: d["Ro"] >= d["R"]),)),
@@ -369,6 +421,19 @@ def launch_checks():
             (C["attn_prefill"], (q, out, q_start, seq_lens, bt, kc, vc), {"Hq": Hq, "Hkv": Hkv}),
         "attn_decode": lambda q, out, tok, seq_lens, bt, kc, vc, Hq, Hkv, splits, part_o, part_lse, host=None:
             (C["attn_decode"], (q, out, tok, seq_lens, bt, kc, vc), {"Hq": Hq, "Hkv": Hkv}),
+        "qk_norm_rope_kv_write": lambda qkv, q_weight, k_weight, eps, positions, slots, cos_sin, q_out, kc, vc, Hq, Hkv, page:
+            (C["qk_norm_rope_kv_write"], (qkv, q_weight, k_weight, positions, slots, cos_sin, q_out, kc, vc),
+             {"Hq": Hq, "Hkv": Hkv, "page": page}),
+        "lora_add": lambda x, lora_a, lora_b, scales, ranks, rows, starts, base, out, slices=None:
+            (C["lora_add"], (x, lora_a, lora_b, scales, ranks, rows, starts, base, out),
+             {"S": len(slices or (0,)), "Nsum": sum(slices or (lora_b.shape[1],)),
+              "Wmod": max(w % 8 for w in (slices or (0,)))}),
+        "page_bounds": lambda kc, bounds, bt, start, seq_lens, max_new:
+            (C["page_bounds"], (kc, bounds, bt, start, seq_lens), {"max_new": max_new}),
+        "attn_select": lambda q, tok, seq_lens, bt, bounds, sel, first, last, Hq, Hkv, ws:
+            (C["attn_select"], (q, tok, seq_lens, bt, bounds, sel, ws), {"Hq": Hq, "Hkv": Hkv, "first": first, "last": last}),
+        "attn_decode_sparse": lambda q, out, tok, seq_lens, bt, sel, kc, vc, Hq, Hkv:
+            (C["attn_decode_sparse"], (q, out, tok, seq_lens, bt, sel, kc, vc), {"Hq": Hq, "Hkv": Hkv}),
         "argmax": lambda logits, out: (C["argmax"], (logits, out), {}),
         "sample": lambda logits, params, out: (C["sample"], (logits, params, out), {}),
         "gemm_grouped": lambda A, B, out, groups, num_groups, epi, align=128:

@@ -44,6 +44,15 @@ OPS: Tuple[OpEntry, ...] = (
             "csrc/kernels/attention.cu"),
     OpEntry("attn_decode", "attn_decode", ("bf16",), "cap 10: paged split-KV decode attention",
             "csrc/kernels/attention.cu"),
+    OpEntry("qk_norm_rope_kv_write", "qk_norm_rope_kv_write", ("bf16",),
+            "new: RMS norm of query and key heads with RoPE and the paged KV write", "csrc/kernels/qk_norm_rope.cu"),
+    OpEntry("lora_add", "lora_add", ("bf16", "bf16->fp32"),
+            "new: low-rank adapters of many requests beside a projection", "csrc/kernels/lora.cu"),
+    OpEntry("page_bounds", "page_bounds", ("bf16",), "new: key bounds of KV pages", "csrc/kernels/attention_sparse.cu"),
+    OpEntry("attn_select", "attn_select", ("bf16->int32",), "new: pages of the highest score bound per KV head",
+            "csrc/kernels/attention_sparse.cu"),
+    OpEntry("attn_decode_sparse", "attn_decode_sparse", ("bf16",), "new: decode attention over selected pages",
+            "csrc/kernels/attention_sparse.cu"),
     OpEntry("argmax", "argmax", ("fp32",), "sampling: greedy", "csrc/kernels/elementwise.cu"),
     OpEntry("argmax_keys", "argmax_keys", ("fp32",), "sampling: vocab-parallel greedy keys",
             "csrc/kernels/elementwise.cu"),

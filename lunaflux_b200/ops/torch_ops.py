@@ -249,6 +249,93 @@ class TorchOps:
         best = k.gather(0, kk.argmax(0)[None])[0]
         out[:rows] = (0xFFFFFFFF - (best & 0xFFFFFFFF)).to(torch.int32)
 
+    # ------------------------------------------- head norms, adapters, selected pages
+    def qk_norm_rope_kv_write(self, qkv, q_weight, k_weight, eps, positions, slots, cos_sin, q_out, kc, vc, Hq, Hkv,
+                              page):
+        T, D = qkv.shape[0], kc.shape[-1]
+        heads = qkv.view(T, Hq + 2 * Hkv, D)
+        cs = cos_sin[positions[:T].long()]
+        c, s = cs[..., 0][:, None, :], cs[..., 1][:, None, :]
+
+        def turn(x, w):
+            xf = x.float()
+            y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+            y1, y2 = y[..., : D // 2], y[..., D // 2:]
+            return torch.cat([y1 * c - y2 * s, y2 * c + y1 * s], -1).to(x.dtype)
+
+        k = turn(heads[:, Hq:Hq + Hkv], k_weight)
+        q_out.copy_(turn(heads[:, :Hq], q_weight).reshape(T, Hq * D))
+        sl = slots[:T].long()
+        ok = sl >= 0
+        pg, off = (sl // page)[ok], (sl % page)[ok]
+        kc[pg, :, off] = k[ok]
+        vc[pg, :, off] = heads[ok, Hq + Hkv:]
+
+    def lora_add(self, x, lora_a, lora_b, scales, ranks, rows, starts, base, out, slices=None):
+        slices = [lora_b.shape[1]] if slices is None else list(slices)
+        R = lora_b.shape[2]
+        at = starts.tolist()
+        for a, rank in enumerate(ranks.tolist()):
+            t = rows[at[a]:at[a + 1]].long()
+            if t.numel() == 0:
+                continue
+            h = x[t].float()
+            col = 0
+            for i, n in enumerate(slices):
+                low = h @ lora_a[a, i * R:i * R + rank].float().t()
+                up = low @ lora_b[a, col:col + n, :rank].float().t()
+                out[t, col:col + n] = (base[t, col:col + n].float() + scales[a] * up).to(out.dtype)
+                col += n
+
+    def page_bounds(self, kc, bounds, bt, start, seq_lens, max_new):
+        P = kc.shape[2]
+        for r, (s, n) in enumerate(zip(start.tolist(), seq_lens.tolist())):
+            for p in range(s // P, -(-n // P)):
+                if s < n:
+                    keys = kc[int(bt[r, p]), :, : min(P, n - p * P)]
+                    bounds[int(bt[r, p])] = torch.stack([keys.amin(1), keys.amax(1)], 1)
+
+    @staticmethod
+    def select_workspace(rows, Hkv, width):
+        return 0
+
+    def attn_select(self, q, tok, seq_lens, bt, bounds, sel, first, last, Hq, Hkv, ws=None):
+        D, G, budget, P = bounds.shape[-1], Hq // Hkv, sel.shape[2], 16
+        sel.fill_(-1)
+        for r, n in enumerate(seq_lens.tolist()):
+            pages = -(-n // P)
+            if pages <= budget:
+                sel[r, :, :pages] = torch.arange(pages, dtype=torch.int32, device=sel.device)
+                continue
+            b = bounds[bt[r, :pages].long()].transpose(0, 1).double()        # [Hkv, pages, 2, D]
+            qh = q[int(tok[r]), : Hq * D].view(Hkv, G, D).double()
+            score = qh.clamp(max=0) @ b[:, :, 0].transpose(1, 2) + qh.clamp(min=0) @ b[:, :, 1].transpose(1, 2)
+            score = torch.where(torch.isfinite(score), score, math.inf).amax(1)
+            score = score[:, first:pages - last]
+            order = torch.sort(score, dim=-1, descending=True, stable=True).indices + first
+            forced = torch.cat([torch.arange(first), torch.arange(pages - last, pages)]).to(order.device)
+            best = torch.cat([forced.expand(Hkv, -1), order[:, : budget - first - last]], 1)
+            sel[r] = best.sort(-1).values.to(torch.int32)
+
+    def attn_decode_sparse(self, q, out, tok, seq_lens, bt, sel, kc, vc, Hq, Hkv):
+        D, P, G = kc.shape[-1], kc.shape[2], Hq // Hkv
+        head = torch.arange(Hkv, device=q.device)[:, None]
+        for r, n in enumerate(seq_lens.tolist()):
+            t = int(tok[r])
+            count = min(-(-n // P), sel.shape[2])
+            if count == 0:
+                out[t, : Hq * D] = 0
+                continue
+            s = sel[r, :, :count].long()
+            phys = bt[r].long()[s]
+            K = kc[phys, head].reshape(Hkv, -1, D).float()
+            V = vc[phys, head].reshape(Hkv, -1, D).float()
+            at = (s[..., None] * P + torch.arange(P, device=q.device)).reshape(Hkv, 1, -1)
+            V = V.masked_fill(at.transpose(1, 2) >= n, 0.0)
+            sc = (q[t, : Hq * D].view(Hkv, G, D).float() @ K.transpose(1, 2)) / math.sqrt(D)
+            p = sc.masked_fill(at >= n, float("-inf")).softmax(-1)
+            out[t, : Hq * D] = (p @ V).reshape(Hq * D).to(out.dtype)
+
     # ---------------------------------------------------------------- MoE
     def moe_route(self, h, router, bias, topk, ids, weights):
         logits = h.float() @ router.float().t()
