@@ -6,19 +6,26 @@
 // for the rows t listed in `rows`, grouped by adapter (`starts` is the CSR
 // offset of every adapter of the pool).  Slices are the column ranges of a
 // stacked projection (Q, K, V), each with its own A.  Sums are fp32, h is handed
-// on as two bf16 parts (three for fp32 outputs), an error of at most 2^-16 (2^-24) of h,
-// and the output is rounded once.
+// on as two bf16 parts (three for fp32 outputs), an error of at most 2^-16
+// (2^-24) of h, and the output is rounded once.
 //
 // A cluster of eight CTAs owns a tile of up to TM rows of one adapter: every
-// CTA multiplies an eighth of K, the partial h (TM x S R fp32) are added
-// through distributed shared memory in rank order, and every CTA expands an
-// eighth of the columns.  So the whole operator is one launch without a
-// workspace, x and the weights are read by one CTA each, and a result does not
-// depend on the other rows of the call.
+// CTA multiplies an eighth of K, the partial h are added through distributed
+// shared memory in rank order, and every CTA expands an eighth of the columns.
+// So the whole operator is one launch without a workspace, x and the weights
+// are read by one CTA each, and a row's result depends neither on the other
+// rows nor on the order of arrival.  Only the adapter's rank is read, of A and
+// of B: inside a tile, h has S * ceil8(rank) columns ("compact" below).
+//
+// Two kernels.  The small one (TM = 16, weights straight from global memory into
+// the MMA operands) is for decode, where reading the weights bounds the call;
+// the large one (TM = 32 or 64, x, A and B staged in shared memory) is for
+// prefill, where x, base and out do, and the weights come from L2 once per tile.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <stdexcept>
 
 #include "common.cuh"
@@ -32,7 +39,7 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kCluster = 8;
 constexpr int kWarps = 8;
-constexpr int TM = 16;                   // rows of a tile
+constexpr int kThreads = kWarps * 32;
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -42,53 +49,73 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;   // 0 bytes read: the 16 bytes become zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t x;
   asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(x));
   return x;
 }
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   uint32_t addr;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return addr;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
+__device__ __forceinline__ void st_cluster2(uint32_t addr, uint2 v) {
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
+}
 
-// Splits v into PARTS bf16 values that add up to it.
+// The four values as PARTS bf16 values each that add up to them.
 template <int PARTS>
-__device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 (&p)[PARTS]) {
+__device__ __forceinline__ void split4(float4 v, uint2 (&p)[PARTS]) {
 #pragma unroll
   for (int i = 0; i < PARTS; ++i) {
-    p[i] = __float2bfloat16(v);
-    v -= __bfloat162float(p[i]);
+    p[i].x = pack_bf16x2(v.x, v.y);
+    p[i].y = pack_bf16x2(v.z, v.w);
+    const float2 a = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&p[i].x));
+    const float2 b = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&p[i].y));
+    v.x -= a.x, v.y -= a.y, v.z -= b.x, v.w -= b.y;
   }
 }
 
-template <bool F32>
-__global__ void __launch_bounds__(kWarps * 32) lora_kernel(const LoraArgs a) {
-  constexpr int kParts = F32 ? 3 : 2;
-  extern __shared__ __align__(16) uint8_t raw[];
-  __shared__ int tile_info[3];            // adapter, first entry of rows, valid rows
-  __shared__ int tile_rows[TM];
-  pdl_trigger();
-  pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, c = lane & 3;
-  const uint32_t rank_cta = cluster_rank();
-  const int tile = blockIdx.x / kCluster;
-  const int SR = a.S * a.R;
-  const int SRp = (SR + 15) / 16 * 16;    // whole 16-row tiles of A
-  float* part = reinterpret_cast<float*>(raw);              // [SRp][TM] this CTA's partial h
-  float* red = part + SRp * TM;                             // [kWarps][16][TM]
-  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(red + kWarps * 16 * TM);   // [kParts][TM][SRp + 8]
-  const int hld = SRp + 8;
-
-  // the tile's adapter: a scan over the tiles of every adapter of the pool
-  if (warp == 0) {
+// Finds the tile's adapter by a scan over the tiles of every adapter of the pool
+// (warp 0) and its token rows.  Every CTA of the cluster finds the same.
+struct Tile {
+  int adapter;   // -1: past the last tile
+  int rank;
+  float scale;
+};
+template <int TM>
+__device__ __forceinline__ Tile find_tile(const LoraArgs& a, int tile, int* info, int* tile_rows) {
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
     int before = 0, found = -1, first = 0, valid = 0;
     bool bad = false;
     for (int b0 = 0; b0 < a.pool && found < 0; b0 += 32) {
@@ -103,8 +130,7 @@ __global__ void __launch_bounds__(kWarps * 32) lora_kernel(const LoraArgs a) {
         const int v = __shfl_up_sync(kFull, incl, o);
         if (lane >= o) incl += v;
       }
-      const bool mine = before + incl > tile && before + incl - tiles <= tile;
-      const uint32_t m = __ballot_sync(kFull, mine);
+      const uint32_t m = __ballot_sync(kFull, before + incl > tile && before + incl - tiles <= tile);
       if (m) {
         const int src = __ffs(m) - 1;
         const int j = tile - (before + incl - tiles);
@@ -115,168 +141,605 @@ __global__ void __launch_bounds__(kWarps * 32) lora_kernel(const LoraArgs a) {
       before += __shfl_sync(kFull, incl, 31);
     }
     if (__any_sync(kFull, bad) && lane == 0) set_error(kErrBadIndex, 0);
-    if (lane == 0) tile_info[0] = found, tile_info[1] = first, tile_info[2] = valid;
-    if (lane < TM) {
+    if (lane == 0) info[0] = found;
+#pragma unroll
+    for (int i = lane; i < TM; i += 32) {
       int row = -1;
-      if (found >= 0 && lane < valid) {
-        row = a.rows[first + lane];
+      if (found >= 0 && i < valid) {
+        row = a.rows[first + i];
         if (row < 0 || row >= a.T) {
-          set_error(kErrBadIndex, (unsigned long long)(first + lane));
+          set_error(kErrBadIndex, (unsigned long long)(first + i));
           row = -1;
         }
       }
-      tile_rows[lane] = row;
+      tile_rows[i] = row;
     }
   }
   __syncthreads();
-  const int ad = tile_info[0];
-  if (ad < 0) return;                     // past the last tile: the whole cluster leaves
-  int rank = a.ranks[ad];
-  if (rank < 0 || rank > a.R) {
-    if (tid == 0) set_error(kErrBadIndex, (unsigned long long)ad);
-    rank = 0;
+  Tile t{info[0], 0, 0.f};
+  if (t.adapter < 0) return t;
+  t.rank = a.ranks[t.adapter];
+  t.scale = a.scales[t.adapter];
+  if (t.rank < 0 || t.rank > a.R) {
+    if (threadIdx.x == 0) set_error(kErrBadIndex, (unsigned long long)t.adapter);
+    t.rank = 0;
   }
-  const float scale = a.scales[ad];
+  return t;
+}
 
-  // shrink: h^T = A x^T over this CTA's eighth of K, the warps splitting it further
-  const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) + (int64_t)ad * SR * a.K;
-  const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
-  const int r0 = tile_rows[g], r1 = tile_rows[g + 8];
-  const __nv_bfloat16* x0 = r0 >= 0 ? x + (int64_t)r0 * a.ldx : nullptr;
-  const __nv_bfloat16* x1 = r1 >= 0 ? x + (int64_t)r1 * a.ldx : nullptr;
-  const int kblocks = (a.K + 31) / 32;
-  const int per_cta = (kblocks + kCluster - 1) / kCluster;
-  const int kb0 = (int)rank_cta * per_cta, kb1 = min(kblocks, kb0 + per_cta);
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  for (int mt = 0; mt < SRp / 16; ++mt) {
-    // rows of A past the adapter's rank in their slice count as zero and are not read
-    const int j0 = mt * 16 + g, j1 = j0 + 8;
-    const bool on0 = j0 < SR && j0 % a.R < rank, on1 = j1 < SR && j1 % a.R < rank;
-    const __nv_bfloat16* A0 = A + (int64_t)j0 * a.K;
-    const __nv_bfloat16* A1 = A + (int64_t)j1 * a.K;
-    float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    for (int kb = kb0 + warp; kb < kb1; kb += kWarps) {
-      const int k = kb * 32 + c * 8;
-      const bool in = k < a.K;            // K is a multiple of 8
-      const uint4 va = in && on0 ? *reinterpret_cast<const uint4*>(A0 + k) : zero;
-      const uint4 vb = in && on1 ? *reinterpret_cast<const uint4*>(A1 + k) : zero;
-      const uint4 v0 = in && x0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
-      const uint4 v1 = in && x1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
-      mma_bf16(acc[0], va.x, vb.x, va.y, vb.y, v0.x, v0.y);
-      mma_bf16(acc[0], va.z, vb.z, va.w, vb.w, v0.z, v0.w);
-      mma_bf16(acc[1], va.x, vb.x, va.y, vb.y, v1.x, v1.y);
-      mma_bf16(acc[1], va.z, vb.z, va.w, vb.w, v1.z, v1.w);
-    }
-    float* rw = red + warp * 16 * TM;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      rw[g * TM + t * 8 + 2 * c] = acc[t][0];
-      rw[g * TM + t * 8 + 2 * c + 1] = acc[t][1];
-      rw[(g + 8) * TM + t * 8 + 2 * c] = acc[t][2];
-      rw[(g + 8) * TM + t * 8 + 2 * c + 1] = acc[t][3];
-    }
-    __syncthreads();
-    {
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) s += red[w * 16 * TM + tid];   // 256 threads = 16 x TM
-      part[mt * 16 * TM + tid] = s;
-    }
-    __syncthreads();
+// Eight consecutive output columns of one row: base + scale * d, rounded once.
+template <bool F32>
+struct BaseCols {
+  uint4 v[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
+    const uint4* p = F32 ? reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(base) + at)
+                         : reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + at);
+    v[0] = p[0];
+    if (F32) v[F32 ? 1 : 0] = p[1];
   }
-  cluster_sync_all();
-  for (int i = tid; i < SRp * TM; i += kWarps * 32) {
-    float v = 0.f;
-    for (int q = 0; q < kCluster; ++q) v += ld_cluster(part + i, q);
-    __nv_bfloat16 p[kParts];
-    split_bf16<kParts>(v, p);
-    const int j = i / TM, row = i % TM;
+  __device__ __forceinline__ void store(void* out, int64_t at, const float (&d)[8], float scale) const {
+    if (F32) {
+      float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
+      const float* b = reinterpret_cast<const float*>(v);
+      p[0] = make_float4(b[0] + scale * d[0], b[1] + scale * d[1], b[2] + scale * d[2], b[3] + scale * d[3]);
+      p[1] = make_float4(b[4] + scale * d[4], b[5] + scale * d[5], b[6] + scale * d[6], b[7] + scale * d[7]);
+    } else {
+      const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(v);
+      uint32_t o[4];
 #pragma unroll
-    for (int q = 0; q < kParts; ++q) hs[(q * TM + row) * hld + j] = p[q];
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __bfloat1622float2(b[i]);
+        o[i] = pack_bf16x2(f.x + scale * d[2 * i], f.y + scale * d[2 * i + 1]);
+      }
+      *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(out) + at) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
   }
-  cluster_sync_all();                     // all partials are read, and hs is complete
+};
 
-  // expand: groups of 32 columns of one slice, dealt over the cluster's warps
-  const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b) + (int64_t)ad * a.N * a.R;
-  const int rows_[2] = {r0, r1};
-  int group = 0, begin = 0;
+// The idx-th block of W columns that does not cross a slice; false past the last.
+template <int W>
+__device__ __forceinline__ bool column_block(const LoraArgs& a, int idx, int& slice, int& c0, int& end) {
+  int begin = 0;
   for (int s = 0; s < a.S; ++s) {
-    const int end = a.col_end[s];
-    for (int c0 = begin; c0 < end; c0 += 32, ++group) {
-      if (group % (kCluster * kWarps) != (int)rank_cta * kWarps + warp) continue;
+    end = a.col_end[s];
+    const int n = (end - begin + W - 1) / W;
+    if (idx < n) {
+      slice = s;
+      c0 = begin + idx * W;
+      return true;
+    }
+    idx -= n;
+    begin = end;
+  }
+  return false;
+}
+
+// ===========================================================================
+// Small tiles: 16 rows.  Shrink h^T = A x^T: 16 compact columns of h are the
+// rows of m16n8k16, the tile's rows its columns; lane (g, c) = (lane / 4,
+// lane % 4) loads 16 bytes at k = 32 kb + 8 c of A rows g, g + 8 and of token
+// rows g, g + 8: two k-steps whose order of k is the same on both sides.  The
+// warps split K further; MT column tiles and U blocks of k are in flight at a
+// time.  Expand: 32 output columns per warp, column n of tile t being column
+// 8 (n / 2) + 2 t + n % 2, so that a lane ends with eight consecutive columns
+// of two rows; B and base of the first columns are fetched before the cluster
+// barrier, since they do not depend on h.
+// ===========================================================================
+constexpr int kSmallRows = 16;
+
+template <bool F32, int MT, int U, int KS>
+__global__ void __launch_bounds__(kThreads) lora_small_kernel(const LoraArgs a, int cols_max) {
+  constexpr int TM = kSmallRows;
+  constexpr int kParts = F32 ? 3 : 2;
+  constexpr int NG = F32 ? (KS == 1 ? 2 : 1) : 4 / KS;     // column groups in flight
+  extern __shared__ __align__(128) uint8_t raw[];
+  __shared__ int info[1];
+  __shared__ int tile_rows[TM];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const int cta = (int)cluster_rank();
+  const Tile tl = find_tile<TM>(a, blockIdx.x / kCluster, info, tile_rows);
+  if (tl.adapter < 0) return;             // the whole cluster
+  const int rank = tl.rank;
+  const int rp = (rank + 7) / 8 * 8;
+  const int cols = a.S * rp;              // compact columns of h
+  const int mtiles = (cols + 15) / 16;
+  float* part = reinterpret_cast<float*>(raw);                     // [cols_max][TM]
+  float* red = part + cols_max * TM;                               // [kWarps][MT * 16][TM]
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(red + kWarps * MT * 16 * TM);   // [kParts][TM][hld]
+  const int hld = cols_max + 24;          // reads of a 16-wide step may pass the last column
+
+  const int r0 = tile_rows[g], r1 = tile_rows[g + 8];
+  {
+    const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) + (int64_t)tl.adapter * a.S * a.R * a.K;
+    const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
+    const __nv_bfloat16* x0 = x + (int64_t)(r0 >= 0 ? r0 : 0) * a.ldx;
+    const __nv_bfloat16* x1 = x + (int64_t)(r1 >= 0 ? r1 : 0) * a.ldx;
+    const int kblocks = (a.K + 31) / 32;
+    const int per_cta = (kblocks + kCluster - 1) / kCluster;
+    const int kb0 = cta * per_cta, kb1 = min(kblocks, kb0 + per_cta);
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    for (int m0 = 0; m0 < mtiles; m0 += MT) {
+      const __nv_bfloat16* ap[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int j = (m0 + m) * 16 + u * 8 + g;
+          const int s = rp ? j / rp : 0, i = j - s * rp;
+          ap[m][u] = j < cols && i < rank ? A + (int64_t)(s * a.R + i) * a.K : nullptr;
+        }
+      float acc[MT][2][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.f;
+      for (int kb = kb0 + warp; kb < kb1; kb += kWarps * U) {
+        uint4 vx[U][2], va[U][MT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int b = kb + u * kWarps;
+          const int k = b * 32 + c * 8;
+          const bool in = b < kb1 && k < a.K;       // K is a multiple of 8
+          vx[u][0] = in && r0 >= 0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
+          vx[u][1] = in && r1 >= 0 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            va[u][m][0] = in && ap[m][0] ? *reinterpret_cast<const uint4*>(ap[m][0] + k) : zero;
+            va[u][m][1] = in && ap[m][1] ? *reinterpret_cast<const uint4*>(ap[m][1] + k) : zero;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const uint4 p = va[u][m][0], q = va[u][m][1], v = vx[u][t];
+              mma_bf16(acc[m][t], p.x, q.x, p.y, q.y, v.x, v.y);
+              mma_bf16(acc[m][t], p.z, q.z, p.w, q.w, v.z, v.w);
+            }
+      }
+      float* rw = red + warp * MT * 16 * TM;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          *reinterpret_cast<float2*>(rw + (m * 16 + g) * TM + t * 8 + 2 * c) = make_float2(acc[m][t][0], acc[m][t][1]);
+          *reinterpret_cast<float2*>(rw + (m * 16 + g + 8) * TM + t * 8 + 2 * c) = make_float2(acc[m][t][2], acc[m][t][3]);
+        }
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m0 + m >= mtiles) break;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) s += red[(w * MT + m) * 16 * TM + tid];   // 256 threads = 16 x TM
+        part[(m0 + m) * 16 * TM + tid] = s;
+      }
+      __syncthreads();
+    }
+  }
+
+  // B and base of this warp's next NG groups of 32 columns, the first 16 KS of their k
+  const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b) + (int64_t)tl.adapter * a.N * a.R;
+  uint2 bv[NG][KS][4];
+  BaseCols<F32> bs[NG][2];
+  int gs[NG], gc[NG], ge[NG];
+  auto load_b = [&](int i, int kb) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int k = kb + ks * 16 + 4 * c;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int col = gc[i] + (g >> 1) * 8 + 2 * t + (g & 1);
+        uint2 v = make_uint2(0u, 0u);
+        if (gs[i] >= 0 && col < ge[i] && k < rank) {
+          v = *reinterpret_cast<const uint2*>(B + (int64_t)col * a.R + k);
+          if (k + 1 >= rank) v.x &= 0xffffu;       // past the rank nothing counts, not even a NaN
+          if (k + 2 >= rank) v.y = 0u;
+          else if (k + 3 >= rank) v.y &= 0xffffu;
+        }
+        bv[i][ks][t] = v;
+      }
+    }
+  };
+  auto load_groups = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      gs[i] = -1;
+      gc[i] = ge[i] = 0;
+      if (!column_block<32>(a, first + i * kCluster * kWarps, gs[i], gc[i], ge[i])) gs[i] = -1;
+      load_b(i, 0);
+      const int col = gc[i] + 8 * c;
+      if (gs[i] >= 0 && col < ge[i]) {
+        if (r0 >= 0) bs[i][0].load(a.base, (int64_t)r0 * a.ldb + col);
+        if (r1 >= 0) bs[i][1].load(a.base, (int64_t)r1 * a.ldb + col);
+      }
+    }
+  };
+  int group = cta * kWarps + warp;
+  load_groups(group);
+  cluster_arrive();
+  cluster_wait();
+  for (int i = tid; i < mtiles * 16 * TM / 4; i += kThreads) {     // four rows of one column
+    float4 v[kCluster];
+#pragma unroll
+    for (int q = 0; q < kCluster; ++q) v[q] = ld_cluster4(cluster_addr(part + i * 4, q));
+#pragma unroll
+    for (int q = 1; q < kCluster; ++q) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
+    uint2 p[kParts];
+    split4<kParts>(v[0], p);
+    const int j = i / (TM / 4), row = i % (TM / 4) * 4;
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+      const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&p[q]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) hs[(q * TM + row + r) * hld + j] = e[r];
+    }
+  }
+  cluster_arrive();                       // this CTA has read the others' partials
+  __syncthreads();
+
+  while (gs[0] >= 0) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      if (gs[i] < 0) break;
       float acc[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-      for (int kb = 0; kb < rank; kb += 16) {
-        const int k = kb + 4 * c;
-        uint2 hv[kParts][2];
+      for (int kb = 0; kb < rank; kb += 16 * KS) {
+        if (kb > 0) load_b(i, kb);
 #pragma unroll
-        for (int q = 0; q < kParts; ++q) {
-          // k past R (R a multiple of 8, not of 16) would be the next slice's h
-          hv[q][0] = k < a.R ? *reinterpret_cast<const uint2*>(hs + (q * TM + g) * hld + s * a.R + k) : make_uint2(0u, 0u);
-          hv[q][1] = k < a.R ? *reinterpret_cast<const uint2*>(hs + (q * TM + g + 8) * hld + s * a.R + k) : make_uint2(0u, 0u);
-        }
+        for (int ks = 0; ks < KS; ++ks) {
+          const int k = kb + ks * 16 + 4 * c;
+          if (kb + ks * 16 >= rank) break;
+          const __nv_bfloat16* h = hs + g * hld + gs[i] * rp + k;
+          const bool in = k < rp;         // beyond it lies the next slice's h
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          // column n = g of tile t is column 8 (g / 2) + 2 t + g % 2 of the group:
-          // a lane then ends up with eight consecutive columns
-          const int col = c0 + (g >> 1) * 8 + 2 * t + (g & 1);
-          uint2 bv = make_uint2(0u, 0u);
-          if (col < end && k < rank) {
-            bv = *reinterpret_cast<const uint2*>(B + (int64_t)col * a.R + k);
-            if (k + 1 >= rank) bv.x &= 0xffffu;
-            if (k + 2 >= rank) bv.y = 0u;
-            else if (k + 3 >= rank) bv.y &= 0xffffu;
+          for (int q = 0; q < kParts; ++q) {
+            const uint2 h0 = in ? *reinterpret_cast<const uint2*>(h + q * TM * hld) : make_uint2(0u, 0u);
+            const uint2 h1 = in ? *reinterpret_cast<const uint2*>(h + (q * TM + 8) * hld) : make_uint2(0u, 0u);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) mma_bf16(acc[t], h0.x, h1.x, h0.y, h1.y, bv[i][ks][t].x, bv[i][ks][t].y);
           }
-#pragma unroll
-          for (int q = 0; q < kParts; ++q) mma_bf16(acc[t], hv[q][0].x, hv[q][1].x, hv[q][0].y, hv[q][1].y, bv.x, bv.y);
         }
       }
-      const int col = c0 + 8 * c;
-      if (col >= end) continue;
+      const int col = gc[i] + 8 * c;
+      if (col < ge[i]) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (rows_[u] < 0) continue;
-        float d[8];
+        for (int u = 0; u < 2; ++u) {
+          const int row = u ? r1 : r0;
+          if (row < 0) continue;
+          float d[8];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) d[2 * t] = scale * acc[t][2 * u], d[2 * t + 1] = scale * acc[t][2 * u + 1];
-        if (F32) {
-          const float4* bp = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.base) + (int64_t)rows_[u] * a.ldb + col);
-          float4* op = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + (int64_t)rows_[u] * a.ldo + col);
-          const float4 b0 = bp[0], b1 = bp[1];
-          op[0] = make_float4(b0.x + d[0], b0.y + d[1], b0.z + d[2], b0.w + d[3]);
-          op[1] = make_float4(b1.x + d[4], b1.y + d[5], b1.z + d[6], b1.w + d[7]);
-        } else {
-          const uint4 bv = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.base) + (int64_t)rows_[u] * a.ldb + col);
-          const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(&bv);
-          uint32_t o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(b2[i]);
-            o[i] = pack_bf16x2(f.x + d[2 * i], f.y + d[2 * i + 1]);
-          }
-          *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (int64_t)rows_[u] * a.ldo + col) = make_uint4(o[0], o[1], o[2], o[3]);
+          for (int t = 0; t < 4; ++t) d[2 * t] = acc[t][2 * u], d[2 * t + 1] = acc[t][2 * u + 1];
+          bs[i][u].store(a.out, (int64_t)row * a.ldo + col, d, tl.scale);
         }
       }
     }
-    begin = end;
+    if (NG > 1 && gs[NG - 1] < 0) break;
+    group += NG * kCluster * kWarps;
+    load_groups(group);
   }
+  cluster_wait();                         // no CTA leaves while another reads its partial h
+}
+
+// ===========================================================================
+// Large tiles: TM = 64 rows (32 where S * R > 256, so that the partial h and its
+// parts fit).  Shrink h = x A^T over chunks of 64 k in a three-stage cp.async
+// ring; a warp owns 32 rows and a share of the compact columns.  The partial h
+// are reduced in slices: CTA q adds rows [q TM / 8, ...) of all eight CTAs, splits
+// them into bf16 parts and stores those into every CTA's shared memory, a sixth
+// of the traffic of every CTA reading everything.  Expand: a warp owns 16 rows,
+// the row groups of a column group share its 64 columns of B (two stages).
+// Shared-memory rows are 128 bytes with the 16-byte pieces xor-ed by row % 8.
+// ===========================================================================
+constexpr int kStages = 3;
+constexpr int kLargeRows = 768;         // listed rows from which the large tiles are used
+
+template <int TM>
+__host__ __device__ constexpr int large_groups() { return kWarps / (TM / 16); }   // column groups of the expansion
+
+struct LargeSmem {
+  size_t hs, total;     // [stages | partial h | B stages] below hs
+};
+template <int TM>
+__host__ __device__ inline LargeSmem large_smem(int cols_max, int R, int parts) {
+  const size_t stages = (size_t)kStages * 128 * (TM + cols_max);
+  const size_t part = (size_t)TM * (cols_max + 4) * 4;
+  const size_t b = (size_t)large_groups<TM>() * 2 * 64 * ((R + 63) / 64 * 128);
+  size_t low = part > b ? part : b;
+  const size_t hs = (size_t)parts * TM * ((cols_max + 15) / 16 * 16 + 24) * 2;
+  if (low + hs < stages) low = stages - hs;
+  low = (low + 127) / 128 * 128;
+  return {low, low + hs};
+}
+
+template <bool F32, int TM, int NTW>
+__global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(const LoraArgs a, int cols_max, int smem_hs) {
+  constexpr int kParts = F32 ? 3 : 2;
+  constexpr int WR = TM / 32;             // row groups of the shrink
+  constexpr int WQ = kWarps / WR;         // column shares
+  constexpr int NCG = large_groups<TM>();
+  extern __shared__ __align__(128) uint8_t raw[];
+  __shared__ int info[1];
+  __shared__ int tile_rows[TM];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const int cta = (int)cluster_rank();
+  const Tile tl = find_tile<TM>(a, blockIdx.x / kCluster, info, tile_rows);
+  if (tl.adapter < 0) return;
+  const int rank = tl.rank;
+  const int rp = (rank + 7) / 8 * 8;
+  const int cols = a.S * rp;
+  const int ntiles = cols / 8;
+  const int hld = (cols_max + 15) / 16 * 16 + 24;       // hld / 8 is odd: ldmatrix rows hit all banks
+  const int pld = cols_max + 4;
+  float* part = reinterpret_cast<float*>(raw);
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(raw + smem_hs);
+  const uint32_t raw_u = smem_u32(raw);
+
+  // ---- shrink
+  {
+    const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) + (int64_t)tl.adapter * a.S * a.R * a.K;
+    const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
+    const int chunks = (a.K + 63) / 64;
+    const int per_cta = (chunks + kCluster - 1) / kCluster;
+    const int ch0 = cta * per_cta, n = min(chunks, ch0 + per_cta) - ch0;
+    const int stage_bytes = 128 * (TM + cols);
+    auto load_stage = [&](int i) {
+      if (i < n) {
+        const uint32_t st = raw_u + (i % kStages) * stage_bytes;
+        const int kbase = (ch0 + i) * 64;
+        for (int p = tid; p < (TM + cols) * 8; p += kThreads) {
+          const int r = p >> 3, k = kbase + (p & 7) * 8;
+          const __nv_bfloat16* src = x;
+          bool on = k < a.K;
+          if (r < TM) {
+            const int row = tile_rows[r];
+            on = on && row >= 0;
+            if (on) src = x + (int64_t)row * a.ldx + k;
+          } else {
+            const int j = r - TM, s = j / rp, q = j - s * rp;
+            on = on && q < rank;
+            if (on) src = A + (int64_t)(s * a.R + q) * a.K + k;
+          }
+          cp_async16(st + r * 128 + (((p & 7) ^ (r & 7)) << 4), src, on);
+        }
+      }
+      cp_async_commit();
+    };
+    const int wr = warp % WR, wq = warp / WR;
+    const int per = (ntiles + 2 * WQ - 1) / (2 * WQ) * 2;       // even: ldmatrix brings tiles in pairs
+    const int t0 = wq * per, tn = min(ntiles, t0 + per) - t0;   // may be <= 0
+    float acc[2][NTW][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int t = 0; t < NTW; ++t) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.f;
+    for (int i = 0; i < kStages - 1; ++i) load_stage(i);
+    for (int i = 0; i < n; ++i) {
+      cp_async_wait<kStages - 2>();
+      __syncthreads();
+      load_stage(i + kStages - 1);
+      const uint32_t st = raw_u + (i % kStages) * stage_bytes;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        uint32_t xa[2][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const int r = wr * 32 + m * 16 + (lane & 15);
+          ldsm_x4(st + r * 128 + (((ks * 2 + (lane >> 4)) ^ (r & 7)) << 4), xa[m]);
+        }
+#pragma unroll
+        for (int t = 0; t < NTW; t += 2) {
+          if (t >= tn) break;
+          // an odd last tile's partner lies past the compact columns: the row is clamped, the result unused
+          const int r = TM + min((t0 + t + (lane >> 4)) * 8 + (lane & 7), cols - 1);
+          uint32_t b[4];
+          ldsm_x4(st + r * 128 + (((ks * 2 + (lane >> 3 & 1)) ^ (r & 7)) << 4), b);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            mma_bf16(acc[m][t], xa[m][0], xa[m][1], xa[m][2], xa[m][3], b[0], b[1]);
+            mma_bf16(acc[m][t + 1], xa[m][0], xa[m][1], xa[m][2], xa[m][3], b[2], b[3]);
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+    __syncthreads();                      // the ring's memory becomes the partial h
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int t = 0; t < NTW; ++t) {
+        if (t >= tn) break;
+        float* p = part + (wr * 32 + m * 16 + g) * pld + (t0 + t) * 8 + 2 * c;
+        *reinterpret_cast<float2*>(p) = make_float2(acc[m][t][0], acc[m][t][1]);
+        *reinterpret_cast<float2*>(p + 8 * pld) = make_float2(acc[m][t][2], acc[m][t][3]);
+      }
+  }
+  cluster_arrive();
+  cluster_wait();
+  {
+    constexpr int kOwn = TM / kCluster;   // rows this CTA adds up
+    const int quads = cols / 4;
+    for (int i = tid; i < kOwn * quads; i += kThreads) {
+      const int row = cta * kOwn + i / quads, j = i % quads * 4;
+      float4 v[kCluster];
+#pragma unroll
+      for (int q = 0; q < kCluster; ++q) v[q] = ld_cluster4(cluster_addr(part + row * pld + j, q));
+#pragma unroll
+      for (int q = 1; q < kCluster; ++q) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
+      uint2 p[kParts];
+      split4<kParts>(v[0], p);
+#pragma unroll
+      for (int q = 0; q < kCluster; ++q)
+#pragma unroll
+        for (int s = 0; s < kParts; ++s) st_cluster2(cluster_addr(hs + (s * TM + row) * hld + j, q), p[s]);
+    }
+  }
+  cluster_arrive();                       // all parts of h are in place, all partials read
+  cluster_wait();
+
+  // ---- expand
+  const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b) + (int64_t)tl.adapter * a.N * a.R;
+  constexpr int RG = TM / 16;             // warps of a column group
+  const int rg = warp % RG, cg = warp / RG;
+  const int gtid = rg * 32 + lane;        // thread of the column group
+  const int kpieces = (rp + 15) / 16 * 2; // 16-byte pieces of a row, whole 16-wide steps
+  const uint32_t bbuf = raw_u + cg * 2 * 64 * ((a.R + 63) / 64 * 128);
+  const int bstage = 64 * ((a.R + 63) / 64 * 128);
+  const int row0 = tile_rows[rg * 16 + g], row1 = tile_rows[rg * 16 + g + 8];
+  auto load_b = [&](int block, int st) {
+    int s, c0, end;
+    if (column_block<64>(a, block, s, c0, end)) {
+      for (int p = gtid; p < 64 * kpieces; p += RG * 32) {
+        // column q * 8 + 2 t + e of a 32-column half is stored as row t * 8 + 2 q + e
+        const int col = p / kpieces, k = p % kpieces * 8;
+        const int lc = col & 31;
+        const int r = (col & 32) + (lc >> 1 & 3) * 8 + (lc >> 3) * 2 + (lc & 1);
+        const bool on = c0 + col < end && k < rank;
+        cp_async16(bbuf + st * bstage + (k >> 6) * 8192 + r * 128 + (((k >> 3 & 7) ^ (r & 7)) << 4),
+                   on ? B + (int64_t)(c0 + col) * a.R + k : B, on);
+      }
+    }
+    cp_async_commit();
+  };
+  constexpr int kStep = kCluster * NCG;
+  int block = cta * NCG + cg;
+  load_b(block, 0);
+  int slice, c0, end;
+  for (int it = 0; column_block<64>(a, block, slice, c0, end); ++it, block += kStep) {
+    load_b(block + kStep, (it + 1) & 1);
+    BaseCols<F32> bs[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int col = c0 + h * 32 + 8 * c;
+      if (col < end) {
+        if (row0 >= 0) bs[h][0].load(a.base, (int64_t)row0 * a.ldb + col);
+        if (row1 >= 0) bs[h][1].load(a.base, (int64_t)row1 * a.ldb + col);
+      }
+    }
+    cp_async_wait<1>();
+    bar_sync(1 + cg, RG * 32);
+    float acc[8][4];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+    const uint32_t bst = bbuf + (it & 1) * bstage;
+    for (int k = 0; k < rp; k += 16) {
+      uint32_t h[kParts][4];
+#pragma unroll
+      for (int q = 0; q < kParts; ++q)
+        ldsm_x4(smem_u32(hs + (q * TM + rg * 16 + (lane & 15)) * hld + slice * rp + k + (lane >> 4) * 8), h[q]);
+      // a last step of eight: the upper half of h belongs to the next slice
+      if (k + 8 >= rp) {
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) h[q][2] = h[q][3] = 0u;
+      }
+#pragma unroll
+      for (int t = 0; t < 8; t += 2) {
+        const int r = (t + (lane >> 4)) * 8 + (lane & 7);
+        uint32_t b[4];
+        ldsm_x4(bst + (k >> 6) * 8192 + r * 128 + (((((k & 63) >> 3) + (lane >> 3 & 1)) ^ (r & 7)) << 4), b);
+        if (k + 16 > rank) {              // past the rank nothing counts, not even a NaN
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int kk = k + (e & 1) * 8 + 2 * c;
+            if (kk >= rank) b[e] = 0u;
+            else if (kk + 1 >= rank) b[e] &= 0xffffu;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+          mma_bf16(acc[t], h[q][0], h[q][1], h[q][2], h[q][3], b[0], b[1]);
+          mma_bf16(acc[t + 1], h[q][0], h[q][1], h[q][2], h[q][3], b[2], b[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int col = c0 + h * 32 + 8 * c;
+      if (col >= end) continue;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = u ? row1 : row0;
+        if (row < 0) continue;
+        float d[8];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) d[2 * t] = acc[h * 4 + t][2 * u], d[2 * t + 1] = acc[h * 4 + t][2 * u + 1];
+        bs[h][u].store(a.out, (int64_t)row * a.ldo + col, d, tl.scale);
+      }
+    }
+    bar_sync(1 + cg, RG * 32);            // the stage is free for the block after the next
+  }
+  cp_async_wait<0>();
+}
+
+void raise_smem(const void* k, size_t smem) {
+  if (smem <= 48 * 1024) return;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) launch_failed(e);
+}
+
+template <bool F32, int MT, int U, int KS>
+void launch_small(const LoraArgs& a, cudaStream_t s) {
+  const int cols = (a.S * a.R + 15) / 16 * 16;
+  const int parts = F32 ? 3 : 2;
+  const size_t smem = sizeof(float) * kSmallRows * (cols + kWarps * MT * 16) + (size_t)2 * parts * kSmallRows * (cols + 24);
+  auto k = lora_small_kernel<F32, MT, U, KS>;
+  raise_smem(reinterpret_cast<const void*>(k), smem);
+  const int tiles = a.L / kSmallRows + std::min(a.L, a.pool);   // at least the sum of ceil(rows / 16) over the adapters
+  launch_k(k, dim3((unsigned)tiles * kCluster), dim3(kThreads), smem, s, (unsigned)kCluster, a, cols);
+}
+
+template <bool F32>
+void small(const LoraArgs& a, cudaStream_t s) {
+  const bool one = a.S * a.R <= 16;
+  if (a.R <= 16) {
+    if (one) launch_small<F32, 1, 4, 1>(a, s);
+    else launch_small<F32, 4, 1, 1>(a, s);
+  } else {
+    launch_small<F32, 4, 1, 4>(a, s);
+  }
+}
+
+template <bool F32, int TM, int NTW>
+void launch_large(const LoraArgs& a, cudaStream_t s) {
+  const int cols = (a.S * a.R + 15) / 16 * 16;
+  const LargeSmem sm = large_smem<TM>(cols, a.R, F32 ? 3 : 2);
+  auto k = lora_large_kernel<F32, TM, NTW>;
+  raise_smem(reinterpret_cast<const void*>(k), sm.total);
+  const int tiles = a.L / TM + std::min(a.L, a.pool);
+  launch_k(k, dim3((unsigned)tiles * kCluster), dim3(kThreads), sm.total, s, (unsigned)kCluster, a, cols, (int)sm.hs);
+}
+
+// Four fp32 slices of rank 128 leave no room for a large tile's parts of h.
+bool large_fits(const LoraArgs& a) {
+  const int cols = (a.S * a.R + 15) / 16 * 16;
+  return cols <= 256 || large_smem<32>(cols, a.R, a.f32 ? 3 : 2).total <= 226 * 1024;
+}
+
+template <bool F32>
+void large(const LoraArgs& a, cudaStream_t s) {
+  const int cols = a.S * a.R;
+  if (cols <= 64) launch_large<F32, 64, 2>(a, s);
+  else if (cols <= 192) launch_large<F32, 64, 6>(a, s);
+  else if (cols <= 256) launch_large<F32, 64, 8>(a, s);
+  else launch_large<F32, 32, 8>(a, s);
 }
 
 }  // namespace
 
 void lora_add(const LoraArgs& a, cudaStream_t s) {
   if (a.L <= 0 || a.N <= 0 || a.pool <= 0) return;
-  const int SRp = (a.S * a.R + 15) / 16 * 16;
-  const int parts = a.f32 ? 3 : 2;
-  const size_t smem = sizeof(float) * (SRp * TM + kWarps * 16 * TM) + (size_t)2 * parts * TM * (SRp + 8);
-  const int tiles = a.L / TM + (a.L < a.pool ? a.L : a.pool);   // sum of ceil(rows / TM) over the adapters
-  auto k = a.f32 ? lora_kernel<true> : lora_kernel<false>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) launch_failed(e);
-  }
-  launch_k(k, dim3((unsigned)tiles * kCluster), dim3(kWarps * 32), smem, s, (unsigned)kCluster, a);
+  const bool big = a.L >= kLargeRows && large_fits(a);
+  if (a.f32) big ? large<true>(a, s) : small<true>(a, s);
+  else big ? large<false>(a, s) : small<false>(a, s);
 }
 
 }  // namespace lora

@@ -217,6 +217,14 @@ LORA_SHAPES = [
     (300, 136, (64, 64, 64, 72), 40, [100, 100, 100], [40, 33, 8]),
     (1200, 512, (256, 64, 64), 16, [700, 3, 400], None),
     (700, 1024, (1032,), 64, [64, 65, 63, 128, 1, 300], [64, 32, 16, 8, 64, 64]),
+    # enough rows for the large tiles
+    (900, 200, (48, 8, 16), 8, [1, 800, 0, 65], [8, 3, 8, 1]),
+    (800, 1000, (136, 72), 24, [400, 400], [24, 13]),
+    (1000, 520, (256, 64, 64), 64, [64, 65, 63, 0, 700, 100], [64, 32, 9, 8, 41, 0]),
+    (1000, 136, (72,), 128, [990], [77]),
+    (1000, 264, (128, 64), 128, [500, 500], [128, 100]),
+    (800, 328, (64, 8, 72, 64), 128, [31, 33, 736], [128, 50, 121]),
+    (770, 8, (8,), 40, [769], [33]),
 ]
 
 
