@@ -37,7 +37,7 @@ namespace lora {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kCluster = 8;
+constexpr int kCluster = 8;               // largest cluster
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 
@@ -54,6 +54,14 @@ __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;   // 0 bytes read: the 16 bytes become zero
@@ -105,66 +113,60 @@ __device__ __forceinline__ void split4(float4 v, uint2 (&p)[PARTS]) {
   }
 }
 
-// Finds the tile's adapter by a scan over the tiles of every adapter of the pool
-// (warp 0) and its token rows.  Every CTA of the cluster finds the same.
+// The tile's adapter, by a scan over the tiles of every adapter of the pool.
+// Called by whole warps; every warp and CTA that asks finds the same.  The
+// ranks and scales are fetched with the offsets, one round trip for all.
 struct Tile {
-  int adapter;   // -1: past the last tile
+  int adapter;       // -1: past the last tile
+  int first, valid;  // its entries of `rows`
   int rank;
   float scale;
 };
 template <int TM>
-__device__ __forceinline__ Tile find_tile(const LoraArgs& a, int tile, int* info, int* tile_rows) {
+__device__ __forceinline__ Tile find_tile(const LoraArgs& a, int tile) {
   const int lane = threadIdx.x & 31;
-  if (threadIdx.x < 32) {
-    int before = 0, found = -1, first = 0, valid = 0;
-    bool bad = false;
-    for (int b0 = 0; b0 < a.pool && found < 0; b0 += 32) {
-      const int ad = b0 + lane;
-      int s0 = 0, s1 = 0;
-      if (ad < a.pool) s0 = a.starts[ad], s1 = a.starts[ad + 1];
-      if (s0 < 0 || s1 < s0 || s1 > a.L) bad = true, s0 = s1 = 0;
-      const int tiles = (s1 - s0 + TM - 1) / TM;
-      int incl = tiles;
+  Tile t{-1, 0, 0, 0, 0.f};
+  int before = 0;
+  bool bad = false;
+  for (int b0 = 0; b0 < a.pool && t.adapter < 0; b0 += 32) {
+    const int ad = b0 + lane;
+    int s0 = 0, s1 = 0, rank = 0;
+    float scale = 0.f;
+    if (ad < a.pool) s0 = a.starts[ad], s1 = a.starts[ad + 1], rank = a.ranks[ad], scale = a.scales[ad];
+    if (s0 < 0 || s1 < s0 || s1 > a.L) bad = true, s0 = s1 = 0;
+    const int tiles = (s1 - s0 + TM - 1) / TM;
+    int incl = tiles;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(kFull, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const uint32_t m = __ballot_sync(kFull, before + incl > tile && before + incl - tiles <= tile);
-      if (m) {
-        const int src = __ffs(m) - 1;
-        const int j = tile - (before + incl - tiles);
-        found = b0 + src;
-        first = __shfl_sync(kFull, s0 + j * TM, src);
-        valid = __shfl_sync(kFull, min(TM, s1 - s0 - j * TM), src);
-      }
-      before += __shfl_sync(kFull, incl, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kFull, incl, o);
+      if (lane >= o) incl += v;
     }
-    if (__any_sync(kFull, bad) && lane == 0) set_error(kErrBadIndex, 0);
-    if (lane == 0) info[0] = found;
-#pragma unroll
-    for (int i = lane; i < TM; i += 32) {
-      int row = -1;
-      if (found >= 0 && i < valid) {
-        row = a.rows[first + i];
-        if (row < 0 || row >= a.T) {
-          set_error(kErrBadIndex, (unsigned long long)(first + i));
-          row = -1;
-        }
-      }
-      tile_rows[i] = row;
+    const uint32_t m = __ballot_sync(kFull, before + incl > tile && before + incl - tiles <= tile);
+    if (m) {
+      const int src = __ffs(m) - 1;
+      const int j = (tile - (before + incl - tiles)) * TM;
+      t.adapter = b0 + src;
+      t.first = __shfl_sync(kFull, s0 + j, src);
+      t.valid = __shfl_sync(kFull, min(TM, s1 - s0 - j), src);
+      t.rank = __shfl_sync(kFull, rank, src);
+      t.scale = __shfl_sync(kFull, scale, src);
     }
+    before += __shfl_sync(kFull, incl, 31);
   }
-  __syncthreads();
-  Tile t{info[0], 0, 0.f};
-  if (t.adapter < 0) return t;
-  t.rank = a.ranks[t.adapter];
-  t.scale = a.scales[t.adapter];
+  if (__any_sync(kFull, bad) && lane == 0) set_error(kErrBadIndex, 0);
   if (t.rank < 0 || t.rank > a.R) {
-    if (threadIdx.x == 0) set_error(kErrBadIndex, (unsigned long long)t.adapter);
+    if (lane == 0) set_error(kErrBadIndex, (unsigned long long)t.adapter);
     t.rank = 0;
   }
   return t;
+}
+// Token row i of the tile, -1 where it has none.
+__device__ __forceinline__ int tile_row(const LoraArgs& a, const Tile& t, int i) {
+  if (i >= t.valid) return -1;
+  const int row = a.rows[t.first + i];
+  if (row >= 0 && row < a.T) return row;
+  set_error(kErrBadIndex, (unsigned long long)(t.first + i));
+  return -1;
 }
 
 // Eight consecutive output columns of one row: base + scale * d, rounded once.
@@ -217,91 +219,128 @@ __device__ __forceinline__ bool column_block(const LoraArgs& a, int idx, int& sl
 // ===========================================================================
 // Small tiles: 16 rows.  Shrink h^T = A x^T: 16 compact columns of h are the
 // rows of m16n8k16, the tile's rows its columns; lane (g, c) = (lane / 4,
-// lane % 4) loads 16 bytes at k = 32 kb + 8 c of A rows g, g + 8 and of token
+// lane % 4) needs 16 bytes at k = 32 kb + 8 c of A rows g, g + 8 and of token
 // rows g, g + 8: two k-steps whose order of k is the same on both sides.  The
-// warps split K further; MT column tiles and U blocks of k are in flight at a
-// time.  Expand: 32 output columns per warp, column n of tile t being column
-// 8 (n / 2) + 2 t + n % 2, so that a lane ends with eight consecutive columns
-// of two rows; B and base of the first columns are fetched before the cluster
+// warps split K further.  Every lane copies its own pieces into its own slots
+// of a ring in shared memory (cp.async) and reads only those back: a deep
+// pipeline without registers and without a barrier.  Expand: 32 output columns
+// per warp, column n of tile t being column 8 (n / 2) + 2 t + n % 2, so that a
+// lane ends with eight consecutive columns of two rows; B and base of the next
+// columns are always under way, the first ones from before the cluster
 // barrier, since they do not depend on h.
 // ===========================================================================
 constexpr int kSmallRows = 16;
 
-template <bool F32, int MT, int U, int KS>
-__global__ void __launch_bounds__(kThreads) lora_small_kernel(const LoraArgs a, int cols_max) {
+template <int MT>
+constexpr int small_stages() { return MT >= 4 ? 2 : MT == 3 ? 3 : 4; }
+template <int MT>
+constexpr int small_ring() { return small_stages<MT>() * (2 * MT + 2) * kThreads * 16; }
+
+// 8 (WIDE) or 4 consecutive k of one column of B.
+template <bool WIDE>
+struct BPiece;
+template <>
+struct BPiece<true> {
+  uint4 v;
+};
+template <>
+struct BPiece<false> {
+  uint2 v;
+};
+
+// WIDE: R is a multiple of 32, a lane reads 8 consecutive k of a column (two
+// k-steps); else 4 (one k-step).
+template <bool F32, int MT, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs a, int cols_max, int cl) {
   constexpr int TM = kSmallRows;
   constexpr int kParts = F32 ? 3 : 2;
-  constexpr int NG = F32 ? (KS == 1 ? 2 : 1) : 4 / KS;     // column groups in flight
+  constexpr int ST = small_stages<MT>();
+  constexpr int KB = WIDE ? 32 : 16;      // k of one item of the expansion
   extern __shared__ __align__(128) uint8_t raw[];
-  __shared__ int info[1];
-  __shared__ int tile_rows[TM];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int cta = (int)cluster_rank();
-  const Tile tl = find_tile<TM>(a, blockIdx.x / kCluster, info, tile_rows);
+  const Tile tl = find_tile<TM>(a, blockIdx.x / cl);
   if (tl.adapter < 0) return;             // the whole cluster
+  const int my_row = lane < TM ? tile_row(a, tl, lane) : -1;
   const int rank = tl.rank;
   const int rp = (rank + 7) / 8 * 8;
   const int cols = a.S * rp;              // compact columns of h
   const int mtiles = (cols + 15) / 16;
-  float* part = reinterpret_cast<float*>(raw);                     // [cols_max][TM]
-  float* red = part + cols_max * TM;                               // [kWarps][MT * 16][TM]
-  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(red + kWarps * MT * 16 * TM);   // [kParts][TM][hld]
-  const int hld = cols_max + 24;          // reads of a 16-wide step may pass the last column
+  float* red = reinterpret_cast<float*>(raw);                      // [kWarps][MT * 16][TM], over the ring
+  float* part = reinterpret_cast<float*>(raw + small_ring<MT>());  // [cols_max][TM]
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(part + cols_max * TM);   // [kParts][TM][hld]
+  const int hld = cols_max + 40;          // a 32-wide item may pass the last column
 
-  const int r0 = tile_rows[g], r1 = tile_rows[g + 8];
+  int r0 = -1, r1 = -1;
   {
     const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) + (int64_t)tl.adapter * a.S * a.R * a.K;
     const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
-    const __nv_bfloat16* x0 = x + (int64_t)(r0 >= 0 ? r0 : 0) * a.ldx;
-    const __nv_bfloat16* x1 = x + (int64_t)(r1 >= 0 ? r1 : 0) * a.ldx;
     const int kblocks = (a.K + 31) / 32;
-    const int per_cta = (kblocks + kCluster - 1) / kCluster;
+    const int per_cta = (kblocks + cl - 1) / cl;
     const int kb0 = cta * per_cta, kb1 = min(kblocks, kb0 + per_cta);
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    const int n = kb1 > kb0 + warp ? (kb1 - kb0 - warp + kWarps - 1) / kWarps : 0;   // this warp's blocks
+    const uint32_t ring = smem_u32(raw) + tid * 16;
+    auto slot = [&](int it, int i) { return ring + (uint32_t)(it % ST * (2 * MT + 2) + i) * (kThreads * 16); };
+    auto k_of = [&](int it) { return (kb0 + warp + it * kWarps) * 32 + c * 8; };
     for (int m0 = 0; m0 < mtiles; m0 += MT) {
-      const __nv_bfloat16* ap[MT][2];
+      int64_t ap[MT][2];                  // offsets of the A rows, -1 for a row that does not exist
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int j = (m0 + m) * 16 + u * 8 + g;
-          const int s = rp ? j / rp : 0, i = j - s * rp;
-          ap[m][u] = j < cols && i < rank ? A + (int64_t)(s * a.R + i) * a.K : nullptr;
+          const int s = j / rp, i = j - s * rp;
+          ap[m][u] = j < cols && i < rank ? (int64_t)(s * a.R + i) * a.K : -1;
         }
+      auto issue_a = [&](int it) {
+        if (it >= n) return;
+        const int k = k_of(it);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const bool on = k < a.K && ap[m][u] >= 0;   // K is a multiple of 8
+            cp_async16(slot(it, 2 * m + u), A + (on ? ap[m][u] + k : 0), on);
+          }
+      };
+      auto issue_x = [&](int it) {
+        if (it < n) {
+          const int k = k_of(it);
+          const bool on0 = k < a.K && r0 >= 0, on1 = k < a.K && r1 >= 0;
+          cp_async16(slot(it, 2 * MT), x + (on0 ? (int64_t)r0 * a.ldx + k : 0), on0);
+          cp_async16(slot(it, 2 * MT + 1), x + (on1 ? (int64_t)r1 * a.ldx + k : 0), on1);
+        }
+        cp_async_commit();
+      };
+#pragma unroll
+      for (int it = 0; it < ST; ++it) issue_a(it);      // before the token rows have arrived
+      r0 = __shfl_sync(kFull, my_row, g), r1 = __shfl_sync(kFull, my_row, g + 8);
+#pragma unroll
+      for (int it = 0; it < ST; ++it) issue_x(it);
       float acc[MT][2][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int t = 0; t < 2; ++t) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.f;
-      for (int kb = kb0 + warp; kb < kb1; kb += kWarps * U) {
-        uint4 vx[U][2], va[U][MT][2];
+      for (int it = 0; it < n; ++it) {
+        cp_async_wait<ST - 1>();
+        const uint4 v0 = lds16(slot(it, 2 * MT)), v1 = lds16(slot(it, 2 * MT + 1));
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int b = kb + u * kWarps;
-          const int k = b * 32 + c * 8;
-          const bool in = b < kb1 && k < a.K;       // K is a multiple of 8
-          vx[u][0] = in && r0 >= 0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
-          vx[u][1] = in && r1 >= 0 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            va[u][m][0] = in && ap[m][0] ? *reinterpret_cast<const uint4*>(ap[m][0] + k) : zero;
-            va[u][m][1] = in && ap[m][1] ? *reinterpret_cast<const uint4*>(ap[m][1] + k) : zero;
-          }
+        for (int m = 0; m < MT; ++m) {
+          const uint4 p = lds16(slot(it, 2 * m)), q = lds16(slot(it, 2 * m + 1));
+          mma_bf16(acc[m][0], p.x, q.x, p.y, q.y, v0.x, v0.y);
+          mma_bf16(acc[m][0], p.z, q.z, p.w, q.w, v0.z, v0.w);
+          mma_bf16(acc[m][1], p.x, q.x, p.y, q.y, v1.x, v1.y);
+          mma_bf16(acc[m][1], p.z, q.z, p.w, q.w, v1.z, v1.w);
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              const uint4 p = va[u][m][0], q = va[u][m][1], v = vx[u][t];
-              mma_bf16(acc[m][t], p.x, q.x, p.y, q.y, v.x, v.y);
-              mma_bf16(acc[m][t], p.z, q.z, p.w, q.w, v.z, v.w);
-            }
+        issue_a(it + ST);
+        issue_x(it + ST);
       }
+      cp_async_wait<0>();
+      __syncthreads();                    // the ring's memory becomes the warps' sums
       float* rw = red + warp * MT * 16 * TM;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -321,55 +360,55 @@ __global__ void __launch_bounds__(kThreads) lora_small_kernel(const LoraArgs a, 
       }
       __syncthreads();
     }
+    r0 = __shfl_sync(kFull, my_row, g), r1 = __shfl_sync(kFull, my_row, g + 8);
   }
 
-  // B and base of this warp's next NG groups of 32 columns, the first 16 KS of their k
+  // An item is KB values of k of a group of 32 columns; the warp's items run over
+  // its groups and, inside, over k.  One item is computed while the next is fetched.
   const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b) + (int64_t)tl.adapter * a.N * a.R;
-  uint2 bv[NG][KS][4];
-  BaseCols<F32> bs[NG][2];
-  int gs[NG], gc[NG], ge[NG];
-  auto load_b = [&](int i, int kb) {
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int k = kb + ks * 16 + 4 * c;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int col = gc[i] + (g >> 1) * 8 + 2 * t + (g & 1);
-        uint2 v = make_uint2(0u, 0u);
-        if (gs[i] >= 0 && col < ge[i] && k < rank) {
-          v = *reinterpret_cast<const uint2*>(B + (int64_t)col * a.R + k);
-          if (k + 1 >= rank) v.x &= 0xffffu;       // past the rank nothing counts, not even a NaN
-          if (k + 2 >= rank) v.y = 0u;
-          else if (k + 3 >= rank) v.y &= 0xffffu;
-        }
-        bv[i][ks][t] = v;
-      }
-    }
-  };
-  auto load_groups = [&](int first) {
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      gs[i] = -1;
-      gc[i] = ge[i] = 0;
-      if (!column_block<32>(a, first + i * kCluster * kWarps, gs[i], gc[i], ge[i])) gs[i] = -1;
-      load_b(i, 0);
-      const int col = gc[i] + 8 * c;
-      if (gs[i] >= 0 && col < ge[i]) {
-        if (r0 >= 0) bs[i][0].load(a.base, (int64_t)r0 * a.ldb + col);
-        if (r1 >= 0) bs[i][1].load(a.base, (int64_t)r1 * a.ldb + col);
-      }
-    }
+  struct Group {
+    int slice, c0, end, kb;
   };
   int group = cta * kWarps + warp;
-  load_groups(group);
+  auto open_group = [&](Group& q) {
+    q.kb = 0;
+    if (!column_block<32>(a, group, q.slice, q.c0, q.end)) q.slice = -1;
+    group += cl * kWarps;
+  };
+  auto next_item = [&](Group& q) {
+    q.kb += KB;
+    if (q.kb >= rank) open_group(q);
+  };
+  BPiece<WIDE> bn[4];
+  BaseCols<F32> base_n[2];
+  auto fetch = [&](const Group& q) {
+    if (q.slice < 0) return;
+    const int k = q.kb + KB / 4 * c;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int col = q.c0 + (g >> 1) * 8 + 2 * t + (g & 1);
+      bn[t] = BPiece<WIDE>{};
+      if (col < q.end && k < rank) bn[t] = *reinterpret_cast<const BPiece<WIDE>*>(B + (int64_t)col * a.R + k);
+    }
+    const int col = q.c0 + 8 * c;
+    if (q.kb == 0 && col < q.end) {
+      if (r0 >= 0) base_n[0].load(a.base, (int64_t)r0 * a.ldb + col);
+      if (r1 >= 0) base_n[1].load(a.base, (int64_t)r1 * a.ldb + col);
+    }
+  };
+  Group cur, nxt;
+  open_group(cur);
+  fetch(cur);
   cluster_arrive();
   cluster_wait();
   for (int i = tid; i < mtiles * 16 * TM / 4; i += kThreads) {     // four rows of one column
     float4 v[kCluster];
 #pragma unroll
-    for (int q = 0; q < kCluster; ++q) v[q] = ld_cluster4(cluster_addr(part + i * 4, q));
+    for (int q = 0; q < kCluster; ++q)
+      if (q < cl) v[q] = ld_cluster4(cluster_addr(part + i * 4, q));
 #pragma unroll
-    for (int q = 1; q < kCluster; ++q) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
+    for (int q = 1; q < kCluster; ++q)
+      if (q < cl) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
     uint2 p[kParts];
     split4<kParts>(v[0], p);
     const int j = i / (TM / 4), row = i % (TM / 4) * 4;
@@ -383,46 +422,63 @@ __global__ void __launch_bounds__(kThreads) lora_small_kernel(const LoraArgs a, 
   cluster_arrive();                       // this CTA has read the others' partials
   __syncthreads();
 
-  while (gs[0] >= 0) {
+  float acc[4][4];
+  BaseCols<F32> bs[2];
+  while (cur.slice >= 0) {
+    BPiece<WIDE> b[4];
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      if (gs[i] < 0) break;
-      float acc[4][4];
+    for (int t = 0; t < 4; ++t) b[t] = bn[t];
+    if (cur.kb == 0) {
+      bs[0] = base_n[0], bs[1] = base_n[1];
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-      for (int kb = 0; kb < rank; kb += 16 * KS) {
-        if (kb > 0) load_b(i, kb);
+    }
+    nxt = cur;
+    next_item(nxt);
+    fetch(nxt);
+    const int k = cur.kb + KB / 4 * c;
+    if (cur.kb + KB > rank) {             // past the rank nothing counts, not even a NaN
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int k = kb + ks * 16 + 4 * c;
-          if (kb + ks * 16 >= rank) break;
-          const __nv_bfloat16* h = hs + g * hld + gs[i] * rp + k;
-          const bool in = k < rp;         // beyond it lies the next slice's h
+      for (int t = 0; t < 4; ++t) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&b[t]);
 #pragma unroll
-          for (int q = 0; q < kParts; ++q) {
-            const uint2 h0 = in ? *reinterpret_cast<const uint2*>(h + q * TM * hld) : make_uint2(0u, 0u);
-            const uint2 h1 = in ? *reinterpret_cast<const uint2*>(h + (q * TM + 8) * hld) : make_uint2(0u, 0u);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) mma_bf16(acc[t], h0.x, h1.x, h0.y, h1.y, bv[i][ks][t].x, bv[i][ks][t].y);
-          }
-        }
-      }
-      const int col = gc[i] + 8 * c;
-      if (col < ge[i]) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int row = u ? r1 : r0;
-          if (row < 0) continue;
-          float d[8];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) d[2 * t] = acc[t][2 * u], d[2 * t + 1] = acc[t][2 * u + 1];
-          bs[i][u].store(a.out, (int64_t)row * a.ldo + col, d, tl.scale);
+        for (int i = 0; i < KB / 8; ++i) {
+          if (k + 2 * i >= rank) w[i] = 0u;
+          else if (k + 2 * i + 1 >= rank) w[i] &= 0xffffu;
         }
       }
     }
-    if (NG > 1 && gs[NG - 1] < 0) break;
-    group += NG * kCluster * kWarps;
-    load_groups(group);
+    const __nv_bfloat16* h = hs + g * hld + cur.slice * rp + k;
+    const bool in = k < rp;               // beyond it lies the next slice's h
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+      BPiece<WIDE> h0{}, h1{};
+      if (in) {
+        h0 = *reinterpret_cast<const BPiece<WIDE>*>(h + q * TM * hld);
+        h1 = *reinterpret_cast<const BPiece<WIDE>*>(h + (q * TM + 8) * hld);
+      }
+      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&h0);
+      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&h1);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&b[t]);
+#pragma unroll
+        for (int i = 0; i < KB / 16; ++i) mma_bf16(acc[t], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], w[2 * i], w[2 * i + 1]);
+      }
+    }
+    const int col = cur.c0 + 8 * c;
+    if (cur.kb + KB >= rank && col < cur.end) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = u ? r1 : r0;
+        if (row < 0) continue;
+        float d[8];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) d[2 * t] = acc[t][2 * u], d[2 * t + 1] = acc[t][2 * u + 1];
+        bs[u].store(a.out, (int64_t)row * a.ldo + col, d, tl.scale);
+      }
+    }
+    cur = nxt;
   }
   cluster_wait();                         // no CTA leaves while another reads its partial h
 }
@@ -431,13 +487,14 @@ __global__ void __launch_bounds__(kThreads) lora_small_kernel(const LoraArgs a, 
 // Large tiles: TM = 64 rows (32 where S * R > 256, so that the partial h and its
 // parts fit).  Shrink h = x A^T over chunks of 64 k in a three-stage cp.async
 // ring; a warp owns 32 rows and a share of the compact columns.  The partial h
-// are reduced in slices: CTA q adds rows [q TM / 8, ...) of all eight CTAs, splits
-// them into bf16 parts and stores those into every CTA's shared memory, a sixth
+// are reduced in slices: CTA q of CL adds rows [q TM / CL, ...) of all CTAs, splits
+// them into bf16 parts and stores those into every CTA's shared memory, a fraction
 // of the traffic of every CTA reading everything.  Expand: a warp owns 16 rows,
 // the row groups of a column group share its 64 columns of B (two stages).
 // Shared-memory rows are 128 bytes with the 16-byte pieces xor-ed by row % 8.
 // ===========================================================================
 constexpr int kStages = 3;
+constexpr int kLargeCols = kMaxSlices * kMaxRank;
 constexpr int kLargeRows = 768;         // listed rows from which the large tiles are used
 
 template <int TM>
@@ -458,21 +515,21 @@ __host__ __device__ inline LargeSmem large_smem(int cols_max, int R, int parts) 
   return {low, low + hs};
 }
 
-template <bool F32, int TM, int NTW>
+template <bool F32, int TM, int NTW, int CL>
 __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(const LoraArgs a, int cols_max, int smem_hs) {
   constexpr int kParts = F32 ? 3 : 2;
   constexpr int WR = TM / 32;             // row groups of the shrink
   constexpr int WQ = kWarps / WR;         // column shares
   constexpr int NCG = large_groups<TM>();
   extern __shared__ __align__(128) uint8_t raw[];
-  __shared__ int info[1];
   __shared__ int tile_rows[TM];
+  __shared__ const __nv_bfloat16* row_src[TM + kLargeCols];   // first element of every staged row, null for a zero row
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int cta = (int)cluster_rank();
-  const Tile tl = find_tile<TM>(a, blockIdx.x / kCluster, info, tile_rows);
+  const Tile tl = find_tile<TM>(a, blockIdx.x / CL);
   if (tl.adapter < 0) return;
   const int rank = tl.rank;
   const int rp = (rank + 7) / 8 * 8;
@@ -489,27 +546,34 @@ __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(
     const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) + (int64_t)tl.adapter * a.S * a.R * a.K;
     const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
     const int chunks = (a.K + 63) / 64;
-    const int per_cta = (chunks + kCluster - 1) / kCluster;
+    const int per_cta = (chunks + CL - 1) / CL;
     const int ch0 = cta * per_cta, n = min(chunks, ch0 + per_cta) - ch0;
     const int stage_bytes = 128 * (TM + cols);
+    for (int r = tid; r < TM + cols; r += kThreads) {
+      const __nv_bfloat16* src = nullptr;
+      if (r < TM) {
+        const int row = tile_row(a, tl, r);
+        tile_rows[r] = row;
+        if (row >= 0) src = x + (int64_t)row * a.ldx;
+      } else {
+        const int j = r - TM, s = j / rp, q = j - s * rp;
+        if (q < rank) src = A + (int64_t)(s * a.R + q) * a.K;
+      }
+      row_src[r] = src;
+    }
+    __syncthreads();
+    // thread t copies piece t % 8 of rows t / 8, t / 8 + 32, ...
+    const int piece = tid & 7, rfirst = tid >> 3;
+    const uint32_t dst0 = raw_u + rfirst * 128 + ((piece ^ (rfirst & 7)) << 4);
     auto load_stage = [&](int i) {
       if (i < n) {
-        const uint32_t st = raw_u + (i % kStages) * stage_bytes;
-        const int kbase = (ch0 + i) * 64;
-        for (int p = tid; p < (TM + cols) * 8; p += kThreads) {
-          const int r = p >> 3, k = kbase + (p & 7) * 8;
-          const __nv_bfloat16* src = x;
-          bool on = k < a.K;
-          if (r < TM) {
-            const int row = tile_rows[r];
-            on = on && row >= 0;
-            if (on) src = x + (int64_t)row * a.ldx + k;
-          } else {
-            const int j = r - TM, s = j / rp, q = j - s * rp;
-            on = on && q < rank;
-            if (on) src = A + (int64_t)(s * a.R + q) * a.K + k;
-          }
-          cp_async16(st + r * 128 + (((p & 7) ^ (r & 7)) << 4), src, on);
+        const uint32_t dst = dst0 + (i % kStages) * stage_bytes;
+        const int k = (ch0 + i) * 64 + piece * 8;
+        const bool in = k < a.K;
+        for (int r = rfirst, o = 0; r < TM + cols; r += 32, o += 32 * 128) {
+          const __nv_bfloat16* src = row_src[r];
+          const bool on = in && src != nullptr;
+          cp_async16(dst + o, on ? src + k : x, on);
         }
       }
       cp_async_commit();
@@ -566,21 +630,27 @@ __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(
   cluster_arrive();
   cluster_wait();
   {
-    constexpr int kOwn = TM / kCluster;   // rows this CTA adds up
+    constexpr int kOwn = TM / CL;         // rows this CTA adds up
+    uint32_t part_at[CL], hs_at[CL];
+#pragma unroll
+    for (int q = 0; q < CL; ++q) {
+      part_at[q] = cluster_addr(part + cta * kOwn * pld, q);
+      hs_at[q] = cluster_addr(hs + cta * kOwn * hld, q);
+    }
     const int quads = cols / 4;
     for (int i = tid; i < kOwn * quads; i += kThreads) {
-      const int row = cta * kOwn + i / quads, j = i % quads * 4;
-      float4 v[kCluster];
+      const int row = i / quads, j = (i - row * quads) * 4;
+      float4 v[CL];
 #pragma unroll
-      for (int q = 0; q < kCluster; ++q) v[q] = ld_cluster4(cluster_addr(part + row * pld + j, q));
+      for (int q = 0; q < CL; ++q) v[q] = ld_cluster4(part_at[q] + (row * pld + j) * 4);
 #pragma unroll
-      for (int q = 1; q < kCluster; ++q) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
+      for (int q = 1; q < CL; ++q) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
       uint2 p[kParts];
       split4<kParts>(v[0], p);
 #pragma unroll
-      for (int q = 0; q < kCluster; ++q)
+      for (int q = 0; q < CL; ++q)
 #pragma unroll
-        for (int s = 0; s < kParts; ++s) st_cluster2(cluster_addr(hs + (s * TM + row) * hld + j, q), p[s]);
+        for (int s = 0; s < kParts; ++s) st_cluster2(hs_at[q] + ((s * TM + row) * hld + j) * 2, p[s]);
     }
   }
   cluster_arrive();                       // all parts of h are in place, all partials read
@@ -591,26 +661,33 @@ __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(
   constexpr int RG = TM / 16;             // warps of a column group
   const int rg = warp % RG, cg = warp / RG;
   const int gtid = rg * 32 + lane;        // thread of the column group
-  const int kpieces = (rp + 15) / 16 * 2; // 16-byte pieces of a row, whole 16-wide steps
   const uint32_t bbuf = raw_u + cg * 2 * 64 * ((a.R + 63) / 64 * 128);
   const int bstage = 64 * ((a.R + 63) / 64 * 128);
   const int row0 = tile_rows[rg * 16 + g], row1 = tile_rows[rg * 16 + g + 8];
+  // thread t of the group copies piece t % 8 of columns t / 8, t / 8 + RG * 4, ...
+  const int bpiece = gtid & 7, bfirst = gtid >> 3;
+  const int kp16 = (rp + 15) / 16 * 16;   // whole 16-wide steps; what lies past the rank is zero
   auto load_b = [&](int block, int st) {
     int s, c0, end;
     if (column_block<64>(a, block, s, c0, end)) {
-      for (int p = gtid; p < 64 * kpieces; p += RG * 32) {
+#pragma unroll
+      for (int col = bfirst; col < 64; col += RG * 4) {
         // column q * 8 + 2 t + e of a 32-column half is stored as row t * 8 + 2 q + e
-        const int col = p / kpieces, k = p % kpieces * 8;
         const int lc = col & 31;
         const int r = (col & 32) + (lc >> 1 & 3) * 8 + (lc >> 3) * 2 + (lc & 1);
-        const bool on = c0 + col < end && k < rank;
-        cp_async16(bbuf + st * bstage + (k >> 6) * 8192 + r * 128 + (((k >> 3 & 7) ^ (r & 7)) << 4),
-                   on ? B + (int64_t)(c0 + col) * a.R + k : B, on);
+        const uint32_t dst = bbuf + st * bstage + r * 128 + ((bpiece ^ (r & 7)) << 4);
+        const __nv_bfloat16* src = B + (int64_t)(c0 + col) * a.R;
+        const bool in = c0 + col < end;
+        for (int kb = 0; kb < kp16; kb += 64) {
+          const int k = kb + bpiece * 8;
+          const bool on = in && k < rank;
+          if (k < kp16) cp_async16(dst + kb * 128, on ? src + k : B, on);
+        }
       }
     }
     cp_async_commit();
   };
-  constexpr int kStep = kCluster * NCG;
+  constexpr int kStep = CL * NCG;
   int block = cta * NCG + cg;
   load_b(block, 0);
   int slice, c0, end;
@@ -686,36 +763,56 @@ void raise_smem(const void* k, size_t smem) {
   if (e != cudaSuccess) launch_failed(e);
 }
 
-template <bool F32, int MT, int U, int KS>
+int cta_slots() {   // two CTAs per SM
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return 2 * n;
+}
+
+template <bool F32, int MT, bool WIDE>
 void launch_small(const LoraArgs& a, cudaStream_t s) {
   const int cols = (a.S * a.R + 15) / 16 * 16;
   const int parts = F32 ? 3 : 2;
-  const size_t smem = sizeof(float) * kSmallRows * (cols + kWarps * MT * 16) + (size_t)2 * parts * kSmallRows * (cols + 24);
-  auto k = lora_small_kernel<F32, MT, U, KS>;
+  const size_t smem = small_ring<MT>() + sizeof(float) * kSmallRows * cols + (size_t)2 * parts * kSmallRows * (cols + 40);
+  auto k = lora_small_kernel<F32, MT, WIDE>;
   raise_smem(reinterpret_cast<const void*>(k), smem);
   const int tiles = a.L / kSmallRows + std::min(a.L, a.pool);   // at least the sum of ceil(rows / 16) over the adapters
-  launch_k(k, dim3((unsigned)tiles * kCluster), dim3(kThreads), smem, s, (unsigned)kCluster, a, cols);
+  // Fewer CTAs per tile where they would not all run at once, as long as a CTA's
+  // share of the weights stays small.
+  const int64_t bytes = 2 * (int64_t)a.R * ((int64_t)a.S * a.K + a.N);
+  int cl = kCluster;
+  while (cl > 1 && (int64_t)tiles * cl > cta_slots() && bytes / cl < 128 * 1024) cl /= 2;
+  launch_k(k, dim3((unsigned)(tiles * cl)), dim3(kThreads), smem, s, (unsigned)cl, a, cols, cl);
 }
 
 template <bool F32>
 void small(const LoraArgs& a, cudaStream_t s) {
-  const bool one = a.S * a.R <= 16;
-  if (a.R <= 16) {
-    if (one) launch_small<F32, 1, 4, 1>(a, s);
-    else launch_small<F32, 4, 1, 1>(a, s);
+  const int cols = a.S * a.R;
+  if (a.R % 32 == 0) {
+    if (cols <= 32) launch_small<F32, 2, true>(a, s);
+    else launch_small<F32, 4, true>(a, s);
   } else {
-    launch_small<F32, 4, 1, 4>(a, s);
+    if (cols <= 16) launch_small<F32, 1, false>(a, s);
+    else if (cols <= 48) launch_small<F32, 3, false>(a, s);
+    else launch_small<F32, 4, false>(a, s);
   }
+}
+
+template <bool F32, int TM, int NTW, int CL>
+void launch_large_cl(const LoraArgs& a, int tiles, cudaStream_t s) {
+  const int cols = (a.S * a.R + 15) / 16 * 16;
+  const LargeSmem sm = large_smem<TM>(cols, a.R, F32 ? 3 : 2);
+  auto k = lora_large_kernel<F32, TM, NTW, CL>;
+  raise_smem(reinterpret_cast<const void*>(k), sm.total);
+  launch_k(k, dim3((unsigned)tiles * CL), dim3(kThreads), sm.total, s, (unsigned)CL, a, cols, (int)sm.hs);
 }
 
 template <bool F32, int TM, int NTW>
 void launch_large(const LoraArgs& a, cudaStream_t s) {
-  const int cols = (a.S * a.R + 15) / 16 * 16;
-  const LargeSmem sm = large_smem<TM>(cols, a.R, F32 ? 3 : 2);
-  auto k = lora_large_kernel<F32, TM, NTW>;
-  raise_smem(reinterpret_cast<const void*>(k), sm.total);
   const int tiles = a.L / TM + std::min(a.L, a.pool);
-  launch_k(k, dim3((unsigned)tiles * kCluster), dim3(kThreads), sm.total, s, (unsigned)kCluster, a, cols, (int)sm.hs);
+  if ((int64_t)tiles * kCluster <= cta_slots()) launch_large_cl<F32, TM, NTW, kCluster>(a, tiles, s);
+  else launch_large_cl<F32, TM, NTW, 4>(a, tiles, s);
 }
 
 // Four fp32 slices of rank 128 leave no room for a large tile's parts of h.
