@@ -814,7 +814,7 @@ void lora_add(const at::Tensor& x, const at::Tensor& lora_a, const at::Tensor& l
     LF_CHECK(slices[i] >= 8 && slices[i] % 8 == 0, "lora_add: slice widths must be positive multiples of 8");
     end += slices[i];
     LF_CHECK(end <= N, "lora_add: slices must add up to N");
-    a.col_end[i] = (int)end;
+    a.col_begin[i + 1] = (int)end;
   }
   LF_CHECK(end == N, "lora_add: slices must add up to N");
   lf::lora::lora_add(a, stream());

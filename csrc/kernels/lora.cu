@@ -67,6 +67,10 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool o
   const int n = on ? 16 : 0;   // 0 bytes read: the 16 bytes become zero
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 8 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -173,15 +177,13 @@ __device__ __forceinline__ int tile_row(const LoraArgs& a, const Tile& t, int i)
 template <bool F32>
 struct BaseCols {
   uint4 v[F32 ? 2 : 1];
-  __device__ __forceinline__ void load(const void* base, int64_t at) {
-    const uint4* p = F32 ? reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(base) + at)
-                         : reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + at);
-    v[0] = p[0];
-    if (F32) v[F32 ? 1 : 0] = p[1];
+  __device__ __forceinline__ void load(const void* at) {
+#pragma unroll
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) v[i] = reinterpret_cast<const uint4*>(at)[i];
   }
-  __device__ __forceinline__ void store(void* out, int64_t at, const float (&d)[8], float scale) const {
+  __device__ __forceinline__ void store(void* at, const float (&d)[8], float scale) const {
     if (F32) {
-      float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
+      float4* p = reinterpret_cast<float4*>(at);
       const float* b = reinterpret_cast<const float*>(v);
       p[0] = make_float4(b[0] + scale * d[0], b[1] + scale * d[1], b[2] + scale * d[2], b[3] + scale * d[3]);
       p[1] = make_float4(b[4] + scale * d[4], b[5] + scale * d[5], b[6] + scale * d[6], b[7] + scale * d[7]);
@@ -193,27 +195,24 @@ struct BaseCols {
         const float2 f = __bfloat1622float2(b[i]);
         o[i] = pack_bf16x2(f.x + scale * d[2 * i], f.y + scale * d[2 * i + 1]);
       }
-      *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(out) + at) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 };
 
-// The idx-th block of W columns that does not cross a slice; false past the last.
+// The idx-th block of W (32 or 64) columns that does not cross a slice: its
+// slice (-1 past the last block), first column and the slice's end.
+struct Block {
+  int slice, c0, end;
+};
 template <int W>
-__device__ __forceinline__ bool column_block(const LoraArgs& a, int idx, int& slice, int& c0, int& end) {
-  int begin = 0;
-  for (int s = 0; s < a.S; ++s) {
-    end = a.col_end[s];
-    const int n = (end - begin + W - 1) / W;
-    if (idx < n) {
-      slice = s;
-      c0 = begin + idx * W;
-      return true;
-    }
-    idx -= n;
-    begin = end;
-  }
-  return false;
+__device__ __forceinline__ Block column_block(const LoraArgs& a, int idx) {
+  const int* first = W == 32 ? a.block32 : a.block64;
+  if (idx >= first[kMaxSlices]) return Block{-1, 0, 0};
+  int s = 0;
+#pragma unroll
+  for (int i = 1; i < kMaxSlices; ++i) s += idx >= first[i];   // absent slices begin past the last block
+  return Block{s, a.col_begin[s] + (idx - first[s]) * W, a.col_begin[s + 1]};
 }
 
 // ===========================================================================
@@ -226,27 +225,27 @@ __device__ __forceinline__ bool column_block(const LoraArgs& a, int idx, int& sl
 // pipeline without registers and without a barrier.  Expand: 32 output columns
 // per warp, column n of tile t being column 8 (n / 2) + 2 t + n % 2, so that a
 // lane ends with eight consecutive columns of two rows; B and base of the next
-// columns are always under way, the first ones from before the cluster
-// barrier, since they do not depend on h.
+// columns come through the same ring, the first ones from before the reduction
+// of h, on which they do not depend.
 // ===========================================================================
 constexpr int kSmallRows = 16;
 
 template <int MT>
 constexpr int small_stages() { return MT >= 4 ? 2 : MT == 3 ? 3 : 4; }
-template <int MT>
-constexpr int small_ring() { return small_stages<MT>() * (2 * MT + 2) * kThreads * 16; }
-
-// 8 (WIDE) or 4 consecutive k of one column of B.
-template <bool WIDE>
-struct BPiece;
-template <>
-struct BPiece<true> {
-  uint4 v;
-};
-template <>
-struct BPiece<false> {
-  uint2 v;
-};
+// The ring in units of 16 bytes per lane.  The warps' sums take its first 2 MT
+// units between the two phases; the expansion's items use the others.
+template <bool F32, bool WIDE>
+constexpr int item_units() { return (WIDE ? 4 : 2) + (F32 ? 4 : 2); }   // four pieces of B, two of base
+template <bool F32, int MT, bool WIDE>
+constexpr int small_units() {
+  const int k = small_stages<MT>() * (2 * MT + 2), least = 2 * MT + 2 * item_units<F32, WIDE>();
+  return k > least ? k : least;
+}
+template <bool F32, int MT, bool WIDE>
+constexpr int small_items() {   // items under way
+  const int n = (small_units<F32, MT, WIDE>() - 2 * MT) / item_units<F32, WIDE>();
+  return n < 4 ? n : 4;
+}
 
 // WIDE: R is a multiple of 32, a lane reads 8 consecutive k of a column (two
 // k-steps); else 4 (one k-step).
@@ -256,6 +255,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
   constexpr int kParts = F32 ? 3 : 2;
   constexpr int ST = small_stages<MT>();
   constexpr int KB = WIDE ? 32 : 16;      // k of one item of the expansion
+  constexpr int kUnit = kThreads * 16;    // a ring unit of all lanes
+  constexpr int IU = item_units<F32, WIDE>(), NI = small_items<F32, MT, WIDE>();
   extern __shared__ __align__(128) uint8_t raw[];
   pdl_trigger();
   pdl_wait();
@@ -266,81 +267,156 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
   if (tl.adapter < 0) return;             // the whole cluster
   const int my_row = lane < TM ? tile_row(a, tl, lane) : -1;
   const int rank = tl.rank;
-  const int rp = (rank + 7) / 8 * 8;
-  const int cols = a.S * rp;              // compact columns of h
-  const int mtiles = (cols + 15) / 16;
+  const int rb = (rank + 7) / 8;          // 8-row blocks of A per slice
+  const int rp = rb * 8;
+  const int mtiles = (a.S * rb + 1) / 2;
   float* red = reinterpret_cast<float*>(raw);                      // [kWarps][MT * 16][TM], over the ring
-  float* part = reinterpret_cast<float*>(raw + small_ring<MT>());  // [cols_max][TM]
-  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(part + cols_max * TM);   // [kParts][TM][hld]
+  float* part = reinterpret_cast<float*>(raw + small_units<F32, MT, WIDE>() * kUnit);   // [cols_max][TM]
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(part + cols_max * TM);           // [kParts][TM][hld]
   const int hld = cols_max + 40;          // a 32-wide item may pass the last column
+  const uint32_t ring = smem_u32(raw) + tid * 16;
 
+  // The expansion's items: KB values of k of a group of 32 columns; the warp's
+  // items run over its groups and, inside, over k.
+  const int lcol = (g >> 1) * 8 + (g & 1);                         // this lane's first column of B in a group
+  const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b) + (int64_t)tl.adapter * a.N * a.R;
+  const int gstep = cl * kWarps;
+  struct Item {
+    int group, kb;
+    Block at;
+  };
+  auto next_item = [&](Item& q) {
+    q.kb += KB;
+    if (q.kb >= rank) {
+      q.kb = 0;
+      q.group += gstep;
+      q.at = column_block<32>(a, q.group);
+    }
+  };
+  const char *base0 = nullptr, *base1 = nullptr;                   // this lane's columns of base, null without a row
+  auto issue_item = [&](const Item& q, uint32_t slot) {
+    if (q.at.slice >= 0) {
+      const bool kin = q.kb + KB / 4 * c < rank;
+      const int left = q.at.end - q.at.c0 - lcol;                  // columns from this lane's first to the slice's end
+      const __nv_bfloat16* b = B + (int64_t)(q.at.c0 + lcol) * a.R + q.kb + KB / 4 * c;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const bool on = kin && 2 * t < left;
+        const __nv_bfloat16* src = on ? b + 2 * t * a.R : B;
+        if (WIDE) cp_async16(slot + t * kUnit, src, on);
+        else cp_async8(slot + (t >> 1) * kUnit + (t & 1) * 8, src, on);
+      }
+      if (q.kb == 0 && q.at.c0 + 8 * c < q.at.end) {
+        const uint32_t ab = slot + (WIDE ? 4 : 2) * kUnit;
+        const int64_t off = (int64_t)q.at.c0 * (F32 ? 4 : 2);
+        if (base0 != nullptr) {
+          cp_async16(ab, base0 + off, true);
+          if (F32) cp_async16(ab + kUnit, base0 + off + 16, true);
+        }
+        if (base1 != nullptr) {
+          cp_async16(ab + (F32 ? 2 : 1) * kUnit, base1 + off, true);
+          if (F32) cp_async16(ab + 3 * kUnit, base1 + off + 16, true);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+  Item cur{cta * kWarps + warp, 0, column_block<32>(a, cta * kWarps + warp)};
+  Item ahead = cur;
+  const uint32_t items = ring + 2 * MT * kUnit;
   int r0 = -1, r1 = -1;
-  {
+  auto start_items = [&]() {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      issue_item(ahead, items + i * IU * kUnit);
+      if (ahead.at.slice >= 0) next_item(ahead);
+    }
+  };
+  auto take_rows = [&]() {
+    r0 = __shfl_sync(kFull, my_row, g), r1 = __shfl_sync(kFull, my_row, g + 8);
+    const int es = F32 ? 4 : 2;
+    if (r0 >= 0) base0 = reinterpret_cast<const char*>(a.base) + ((int64_t)r0 * a.ldb + 8 * c) * es;
+    if (r1 >= 0) base1 = reinterpret_cast<const char*>(a.base) + ((int64_t)r1 * a.ldb + 8 * c) * es;
+  };
+
+  if (mtiles == 0) {                      // rank 0: out = base
+    take_rows();
+    start_items();
+  } else {
     const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) + (int64_t)tl.adapter * a.S * a.R * a.K;
     const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
     const int kblocks = (a.K + 31) / 32;
     const int per_cta = (kblocks + cl - 1) / cl;
-    const int kb0 = cta * per_cta, kb1 = min(kblocks, kb0 + per_cta);
-    const int n = kb1 > kb0 + warp ? (kb1 - kb0 - warp + kWarps - 1) / kWarps : 0;   // this warp's blocks
-    const uint32_t ring = smem_u32(raw) + tid * 16;
-    auto slot = [&](int it, int i) { return ring + (uint32_t)(it % ST * (2 * MT + 2) + i) * (kThreads * 16); };
-    auto k_of = [&](int it) { return (kb0 + warp + it * kWarps) * 32 + c * 8; };
+    const int kb0 = cta * per_cta + warp, kb1 = min(kblocks, (cta + 1) * per_cta);
+    const int n = kb1 > kb0 ? (kb1 - kb0 + kWarps - 1) / kWarps : 0;   // this warp's blocks
+    const int k0 = kb0 * 32 + c * 8;
+    const __nv_bfloat16 *x0 = nullptr, *x1 = nullptr;
+    int s = 0, ib = 0;                    // slice and 8-row block of the next rows of A
     for (int m0 = 0; m0 < mtiles; m0 += MT) {
-      int64_t ap[MT][2];                  // offsets of the A rows, -1 for a row that does not exist
+      const __nv_bfloat16* pa[MT][2];     // this lane's rows of A at its first k, null for none
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int j = (m0 + m) * 16 + u * 8 + g;
-          const int s = j / rp, i = j - s * rp;
-          ap[m][u] = j < cols && i < rank ? (int64_t)(s * a.R + i) * a.K : -1;
+          pa[m][u] = s < a.S && ib * 8 + g < rank ? A + (int64_t)(s * a.R + ib * 8 + g) * a.K + k0 : nullptr;
+          if (++ib == rb) ib = 0, ++s;
         }
-      auto issue_a = [&](int it) {
+      auto issue_a = [&](int it, uint32_t slot) {
         if (it >= n) return;
-        const int k = k_of(it);
+        const int dk = it * (kWarps * 32);
+        const bool in = k0 + dk < a.K;    // K is a multiple of 8
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const bool on = k < a.K && ap[m][u] >= 0;   // K is a multiple of 8
-            cp_async16(slot(it, 2 * m + u), A + (on ? ap[m][u] + k : 0), on);
+            const bool on = in && pa[m][u] != nullptr;
+            cp_async16(slot + (2 * m + u) * kUnit, on ? pa[m][u] + dk : A, on);
           }
       };
-      auto issue_x = [&](int it) {
+      auto issue_x = [&](int it, uint32_t slot) {
         if (it < n) {
-          const int k = k_of(it);
-          const bool on0 = k < a.K && r0 >= 0, on1 = k < a.K && r1 >= 0;
-          cp_async16(slot(it, 2 * MT), x + (on0 ? (int64_t)r0 * a.ldx + k : 0), on0);
-          cp_async16(slot(it, 2 * MT + 1), x + (on1 ? (int64_t)r1 * a.ldx + k : 0), on1);
+          const int dk = it * (kWarps * 32);
+          const bool in = k0 + dk < a.K;
+          const bool on0 = in && x0 != nullptr, on1 = in && x1 != nullptr;
+          cp_async16(slot + 2 * MT * kUnit, on0 ? x0 + dk : x, on0);
+          cp_async16(slot + (2 * MT + 1) * kUnit, on1 ? x1 + dk : x, on1);
         }
         cp_async_commit();
       };
+      constexpr int kSlot = (2 * MT + 2) * kUnit;
 #pragma unroll
-      for (int it = 0; it < ST; ++it) issue_a(it);      // before the token rows have arrived
-      r0 = __shfl_sync(kFull, my_row, g), r1 = __shfl_sync(kFull, my_row, g + 8);
+      for (int it = 0; it < ST; ++it) issue_a(it, ring + it * kSlot);   // before the token rows have arrived
+      if (m0 == 0) {
+        take_rows();
+        if (r0 >= 0) x0 = x + (int64_t)r0 * a.ldx + k0;
+        if (r1 >= 0) x1 = x + (int64_t)r1 * a.ldx + k0;
+      }
 #pragma unroll
-      for (int it = 0; it < ST; ++it) issue_x(it);
+      for (int it = 0; it < ST; ++it) issue_x(it, ring + it * kSlot);
       float acc[MT][2][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int t = 0; t < 2; ++t) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.f;
+      uint32_t slot = ring;
       for (int it = 0; it < n; ++it) {
         cp_async_wait<ST - 1>();
-        const uint4 v0 = lds16(slot(it, 2 * MT)), v1 = lds16(slot(it, 2 * MT + 1));
+        const uint4 v0 = lds16(slot + 2 * MT * kUnit), v1 = lds16(slot + (2 * MT + 1) * kUnit);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          const uint4 p = lds16(slot(it, 2 * m)), q = lds16(slot(it, 2 * m + 1));
+          const uint4 p = lds16(slot + 2 * m * kUnit), q = lds16(slot + (2 * m + 1) * kUnit);
           mma_bf16(acc[m][0], p.x, q.x, p.y, q.y, v0.x, v0.y);
           mma_bf16(acc[m][0], p.z, q.z, p.w, q.w, v0.z, v0.w);
           mma_bf16(acc[m][1], p.x, q.x, p.y, q.y, v1.x, v1.y);
           mma_bf16(acc[m][1], p.z, q.z, p.w, q.w, v1.z, v1.w);
         }
-        issue_a(it + ST);
-        issue_x(it + ST);
+        issue_a(it + ST, slot);
+        issue_x(it + ST, slot);
+        slot = slot == ring + (ST - 1) * kSlot ? ring : slot + kSlot;
       }
       cp_async_wait<0>();
-      __syncthreads();                    // the ring's memory becomes the warps' sums
+      if (m0 + MT >= mtiles) start_items();   // the last pass over K: this lane's slots are free
+      __syncthreads();                    // the ring's first units become the warps' sums
       float* rw = red + warp * MT * 16 * TM;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -353,52 +429,15 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         if (m0 + m >= mtiles) break;
-        float s = 0.f;
+        float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) s += red[(w * MT + m) * 16 * TM + tid];   // 256 threads = 16 x TM
-        part[(m0 + m) * 16 * TM + tid] = s;
+        for (int w = 0; w < kWarps; ++w) v += red[(w * MT + m) * 16 * TM + tid];   // 256 threads = 16 x TM
+        part[(m0 + m) * 16 * TM + tid] = v;
       }
-      __syncthreads();
+      if (m0 + MT < mtiles) __syncthreads();
     }
-    r0 = __shfl_sync(kFull, my_row, g), r1 = __shfl_sync(kFull, my_row, g + 8);
   }
 
-  // An item is KB values of k of a group of 32 columns; the warp's items run over
-  // its groups and, inside, over k.  One item is computed while the next is fetched.
-  const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b) + (int64_t)tl.adapter * a.N * a.R;
-  struct Group {
-    int slice, c0, end, kb;
-  };
-  int group = cta * kWarps + warp;
-  auto open_group = [&](Group& q) {
-    q.kb = 0;
-    if (!column_block<32>(a, group, q.slice, q.c0, q.end)) q.slice = -1;
-    group += cl * kWarps;
-  };
-  auto next_item = [&](Group& q) {
-    q.kb += KB;
-    if (q.kb >= rank) open_group(q);
-  };
-  BPiece<WIDE> bn[4];
-  BaseCols<F32> base_n[2];
-  auto fetch = [&](const Group& q) {
-    if (q.slice < 0) return;
-    const int k = q.kb + KB / 4 * c;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int col = q.c0 + (g >> 1) * 8 + 2 * t + (g & 1);
-      bn[t] = BPiece<WIDE>{};
-      if (col < q.end && k < rank) bn[t] = *reinterpret_cast<const BPiece<WIDE>*>(B + (int64_t)col * a.R + k);
-    }
-    const int col = q.c0 + 8 * c;
-    if (q.kb == 0 && col < q.end) {
-      if (r0 >= 0) base_n[0].load(a.base, (int64_t)r0 * a.ldb + col);
-      if (r1 >= 0) base_n[1].load(a.base, (int64_t)r1 * a.ldb + col);
-    }
-  };
-  Group cur, nxt;
-  open_group(cur);
-  fetch(cur);
   cluster_arrive();
   cluster_wait();
   for (int i = tid; i < mtiles * 16 * TM / 4; i += kThreads) {     // four rows of one column
@@ -422,63 +461,77 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
   cluster_arrive();                       // this CTA has read the others' partials
   __syncthreads();
 
+  const int es = F32 ? 4 : 2;
+  char* out0 = reinterpret_cast<char*>(a.out) + ((int64_t)r0 * a.ldo + 8 * c) * es;   // used where the row exists
+  char* out1 = reinterpret_cast<char*>(a.out) + ((int64_t)r1 * a.ldo + 8 * c) * es;
   float acc[4][4];
   BaseCols<F32> bs[2];
-  while (cur.slice >= 0) {
-    BPiece<WIDE> b[4];
+  uint32_t slot = items;
+  while (cur.at.slice >= 0) {
+    cp_async_wait<NI - 1>();
+    uint32_t b[4][KB / 8];
+    if (WIDE) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) b[t] = bn[t];
+      for (int t = 0; t < 4; ++t) *reinterpret_cast<uint4*>(b[t]) = lds16(slot + t * kUnit);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint4 v = lds16(slot + t * kUnit);
+        b[2 * t][0] = v.x, b[2 * t][1] = v.y, b[2 * t + 1][0] = v.z, b[2 * t + 1][1] = v.w;
+      }
+    }
     if (cur.kb == 0) {
-      bs[0] = base_n[0], bs[1] = base_n[1];
+      const uint32_t ab = slot + (WIDE ? 4 : 2) * kUnit;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < (F32 ? 2 : 1); ++v) bs[u].v[v] = lds16(ab + (u * (F32 ? 2 : 1) + v) * kUnit);
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
     }
-    nxt = cur;
-    next_item(nxt);
-    fetch(nxt);
     const int k = cur.kb + KB / 4 * c;
     if (cur.kb + KB > rank) {             // past the rank nothing counts, not even a NaN
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(&b[t]);
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < KB / 8; ++i) {
-          if (k + 2 * i >= rank) w[i] = 0u;
-          else if (k + 2 * i + 1 >= rank) w[i] &= 0xffffu;
+        for (int x = 0; x < KB / 8; ++x) {
+          if (k + 2 * x >= rank) b[t][x] = 0u;
+          else if (k + 2 * x + 1 >= rank) b[t][x] &= 0xffffu;
         }
-      }
     }
-    const __nv_bfloat16* h = hs + g * hld + cur.slice * rp + k;
+    const __nv_bfloat16* h = hs + g * hld + cur.at.slice * rp + k;
     const bool in = k < rp;               // beyond it lies the next slice's h
 #pragma unroll
     for (int q = 0; q < kParts; ++q) {
-      BPiece<WIDE> h0{}, h1{};
-      if (in) {
-        h0 = *reinterpret_cast<const BPiece<WIDE>*>(h + q * TM * hld);
-        h1 = *reinterpret_cast<const BPiece<WIDE>*>(h + (q * TM + 8) * hld);
+      uint32_t w0[KB / 8], w1[KB / 8];
+#pragma unroll
+      for (int x = 0; x < KB / 8; ++x) {
+        w0[x] = in ? reinterpret_cast<const uint32_t*>(h + q * TM * hld)[x] : 0u;
+        w1[x] = in ? reinterpret_cast<const uint32_t*>(h + (q * TM + 8) * hld)[x] : 0u;
       }
-      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&h0);
-      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&h1);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(&b[t]);
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < KB / 16; ++i) mma_bf16(acc[t], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], w[2 * i], w[2 * i + 1]);
+        for (int x = 0; x < KB / 16; ++x) mma_bf16(acc[t], w0[2 * x], w1[2 * x], w0[2 * x + 1], w1[2 * x + 1], b[t][2 * x], b[t][2 * x + 1]);
+    }
+    issue_item(ahead, slot);
+    if (ahead.at.slice >= 0) next_item(ahead);
+    slot = slot == items + (NI - 1) * IU * kUnit ? items : slot + IU * kUnit;
+    if (cur.kb + KB >= rank && cur.at.c0 + 8 * c < cur.at.end) {
+      const int64_t off = (int64_t)cur.at.c0 * es;
+      float d[8];
+      if (r0 >= 0) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) d[2 * t] = acc[t][0], d[2 * t + 1] = acc[t][1];
+        bs[0].store(out0 + off, d, tl.scale);
+      }
+      if (r1 >= 0) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) d[2 * t] = acc[t][2], d[2 * t + 1] = acc[t][3];
+        bs[1].store(out1 + off, d, tl.scale);
       }
     }
-    const int col = cur.c0 + 8 * c;
-    if (cur.kb + KB >= rank && col < cur.end) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int row = u ? r1 : r0;
-        if (row < 0) continue;
-        float d[8];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) d[2 * t] = acc[t][2 * u], d[2 * t + 1] = acc[t][2 * u + 1];
-        bs[u].store(a.out, (int64_t)row * a.ldo + col, d, tl.scale);
-      }
-    }
-    cur = nxt;
+    next_item(cur);
   }
   cluster_wait();                         // no CTA leaves while another reads its partial h
 }
@@ -668,16 +721,16 @@ __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(
   const int bpiece = gtid & 7, bfirst = gtid >> 3;
   const int kp16 = (rp + 15) / 16 * 16;   // whole 16-wide steps; what lies past the rank is zero
   auto load_b = [&](int block, int st) {
-    int s, c0, end;
-    if (column_block<64>(a, block, s, c0, end)) {
+    const Block at = column_block<64>(a, block);
+    if (at.slice >= 0) {
 #pragma unroll
       for (int col = bfirst; col < 64; col += RG * 4) {
         // column q * 8 + 2 t + e of a 32-column half is stored as row t * 8 + 2 q + e
         const int lc = col & 31;
         const int r = (col & 32) + (lc >> 1 & 3) * 8 + (lc >> 3) * 2 + (lc & 1);
         const uint32_t dst = bbuf + st * bstage + r * 128 + ((bpiece ^ (r & 7)) << 4);
-        const __nv_bfloat16* src = B + (int64_t)(c0 + col) * a.R;
-        const bool in = c0 + col < end;
+        const __nv_bfloat16* src = B + (int64_t)(at.c0 + col) * a.R;
+        const bool in = at.c0 + col < at.end;
         for (int kb = 0; kb < kp16; kb += 64) {
           const int k = kb + bpiece * 8;
           const bool on = in && k < rank;
@@ -690,16 +743,22 @@ __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(
   constexpr int kStep = CL * NCG;
   int block = cta * NCG + cg;
   load_b(block, 0);
-  int slice, c0, end;
-  for (int it = 0; column_block<64>(a, block, slice, c0, end); ++it, block += kStep) {
+  const int es = F32 ? 4 : 2;
+  const char* base0 = reinterpret_cast<const char*>(a.base) + ((int64_t)row0 * a.ldb + 8 * c) * es;   // used where the row exists
+  const char* base1 = reinterpret_cast<const char*>(a.base) + ((int64_t)row1 * a.ldb + 8 * c) * es;
+  char* out0 = reinterpret_cast<char*>(a.out) + ((int64_t)row0 * a.ldo + 8 * c) * es;
+  char* out1 = reinterpret_cast<char*>(a.out) + ((int64_t)row1 * a.ldo + 8 * c) * es;
+  Block at = column_block<64>(a, block);
+  for (int it = 0; at.slice >= 0; ++it, block += kStep, at = column_block<64>(a, block)) {
     load_b(block + kStep, (it + 1) & 1);
+    const int slice = at.slice, c0 = at.c0, end = at.end;
     BaseCols<F32> bs[2][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int col = c0 + h * 32 + 8 * c;
       if (col < end) {
-        if (row0 >= 0) bs[h][0].load(a.base, (int64_t)row0 * a.ldb + col);
-        if (row1 >= 0) bs[h][1].load(a.base, (int64_t)row1 * a.ldb + col);
+        if (row0 >= 0) bs[h][0].load(base0 + (int64_t)(c0 + h * 32) * es);
+        if (row1 >= 0) bs[h][1].load(base1 + (int64_t)(c0 + h * 32) * es);
       }
     }
     cp_async_wait<1>();
@@ -749,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(
         float d[8];
 #pragma unroll
         for (int t = 0; t < 4; ++t) d[2 * t] = acc[h * 4 + t][2 * u], d[2 * t + 1] = acc[h * 4 + t][2 * u + 1];
-        bs[h][u].store(a.out, (int64_t)row * a.ldo + col, d, tl.scale);
+        bs[h][u].store((u ? out1 : out0) + (int64_t)(c0 + h * 32) * es, d, tl.scale);
       }
     }
     bar_sync(1 + cg, RG * 32);            // the stage is free for the block after the next
@@ -774,7 +833,7 @@ template <bool F32, int MT, bool WIDE>
 void launch_small(const LoraArgs& a, cudaStream_t s) {
   const int cols = (a.S * a.R + 15) / 16 * 16;
   const int parts = F32 ? 3 : 2;
-  const size_t smem = small_ring<MT>() + sizeof(float) * kSmallRows * cols + (size_t)2 * parts * kSmallRows * (cols + 40);
+  const size_t smem = (size_t)small_units<F32, MT, WIDE>() * kThreads * 16 + sizeof(float) * kSmallRows * cols + (size_t)2 * parts * kSmallRows * (cols + 40);
   auto k = lora_small_kernel<F32, MT, WIDE>;
   raise_smem(reinterpret_cast<const void*>(k), smem);
   const int tiles = a.L / kSmallRows + std::min(a.L, a.pool);   // at least the sum of ceil(rows / 16) over the adapters
@@ -832,8 +891,15 @@ void large(const LoraArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-void lora_add(const LoraArgs& a, cudaStream_t s) {
-  if (a.L <= 0 || a.N <= 0 || a.pool <= 0) return;
+void lora_add(const LoraArgs& args, cudaStream_t s) {
+  if (args.L <= 0 || args.N <= 0 || args.pool <= 0) return;
+  LoraArgs a = args;
+  a.block32[0] = a.block64[0] = 0;
+  for (int i = 0; i < kMaxSlices; ++i) {
+    const int width = i < a.S ? a.col_begin[i + 1] - a.col_begin[i] : 0;
+    a.block32[i + 1] = a.block32[i] + (width + 31) / 32;
+    a.block64[i + 1] = a.block64[i] + (width + 63) / 64;
+  }
   const bool big = a.L >= kLargeRows && large_fits(a);
   if (a.f32) big ? large<true>(a, s) : small<true>(a, s);
   else big ? large<false>(a, s) : small<false>(a, s);

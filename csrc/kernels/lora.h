@@ -22,7 +22,9 @@ struct LoraArgs {
   void* out;                  // [T, N], row stride ldo
   int64_t ldo;
   int T, K, N, R, pool, L, S;
-  int col_end[kMaxSlices];    // last column + 1 of every slice
+  int col_begin[kMaxSlices + 1];   // first column of every slice, then N
+  int block32[kMaxSlices + 1];     // blocks of 32 / 64 columns before every slice (set at the launch)
+  int block64[kMaxSlices + 1];
   bool f32;                   // base and out are fp32
 };
 
