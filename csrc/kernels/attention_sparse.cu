@@ -49,14 +49,34 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Streaming 16-byte load: cache lines of K, V and the bounds are used once.
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
+// 16-byte copy into shared memory; zeros where `on` is false.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
   uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+               : "r"(addr)
+               : "memory");
   return v;
 }
+
+// The streaming kernels (scores, attention) run four warps whose lanes copy
+// their own operand pieces into their own slots of a ring in shared memory and
+// read only those back: 16 pieces of 16 bytes per lane and stage, a pipeline
+// without registers and without a barrier.
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kUnit = kThreads * 16;
+constexpr int kStage = 16 * kUnit;           // 32 KB
+constexpr int kStages = 3;                   // 96 KB: two CTAs per SM
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   uint32_t y;
@@ -157,27 +177,70 @@ __global__ void __launch_bounds__(128) page_bounds_kernel(const BoundsArgs a) {
 // same instruction on the operands without their signs.
 // ===========================================================================
 constexpr float kScoreErr = 1.f / 32768.f;   // 2^-15, four times what is derived above
-constexpr int kScoreTile = 64;               // pages of one pass of a CTA's four warps
+constexpr int kScoreTile = 16 * kWarps;      // pages of one pass of a CTA
+constexpr int kScorePasses = 8;              // most passes of a CTA
 
 template <int NH>   // groups of eight query heads
-__global__ void __launch_bounds__(128) page_score_kernel(const SelectArgs a, int chunk_pages) {
+__global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArgs a, int passes) {
+  extern __shared__ __align__(128) uint8_t raw[];
+  __shared__ int phys[kScorePasses * kScoreTile];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.x % a.Hkv, chunk = blockIdx.x / a.Hkv;
   const int r = blockIdx.y;
   const int G = a.Hq / a.Hkv;
+  const int begin = chunk * passes * kScoreTile;
+  const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
+  const int span = min(passes * kScoreTile, a.width - begin);
+  int table[kScorePasses * kScoreTile / kThreads];   // fetched before the length is known
+#pragma unroll
+  for (int i = 0; i < kScorePasses * kScoreTile / kThreads; ++i) {
+    const int p = i * kThreads + tid;
+    table[i] = p < span ? bt[begin + p] : 0;
+  }
   const int L = row_length(a.seq_lens, r, a.width);
   const int n = (L + PAGE - 1) / PAGE;
-  const int begin = chunk * chunk_pages, end = min(n, begin + chunk_pages);
+  const int end = min(n, begin + passes * kScoreTile);
   if (n <= a.budget || begin >= end) return;
   const int tok = a.tok_index[r];
   if (tok < 0 || tok >= a.tokens) {
-    if (threadIdx.x == 0) set_error(kErrBadIndex, (unsigned long long)r);
+    if (tid == 0) set_error(kErrBadIndex, (unsigned long long)r);
     return;
   }
-  const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
+#pragma unroll
+  for (int i = 0; i < kScorePasses * kScoreTile / kThreads; ++i) {
+    const int p = i * kThreads + tid;
+    if (begin + p < end) {
+      if (table[i] < 0 || table[i] >= a.num_pages) {   // recorded; the reserved zero page stands in
+        set_error(kErrBadIndex, (unsigned long long)(begin + p));
+        table[i] = 0;
+      }
+      phys[p] = table[i];
+    }
+  }
+  __syncthreads();
+
+  const uint32_t ring = smem_u32(raw) + tid * 16;
+  const uint4* bounds = reinterpret_cast<const uint4*>(a.bounds);
+  const int pieces = 2 * D / 8;              // of one (page, KV head)
+  auto issue = [&](int it, uint32_t slot) {
+    const int p0 = begin + (it * kWarps + warp) * 16;
+    if (it < passes && p0 < end) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int p = p0 + g + 8 * u;
+        const bool on = p < end;
+        const uint4* src = bounds + ((int64_t)phys[on ? p - begin : 0] * a.Hkv + kvh) * pieces + c;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cp_async16(slot + (u * 8 + j) * kUnit, src + 4 * j, on);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) issue(i, ring + i * kStage);
 
   uint4 q[NH][4];
 #pragma unroll
@@ -187,53 +250,51 @@ __global__ void __launch_bounds__(128) page_score_kernel(const SelectArgs a, int
     for (int j = 0; j < 4; ++j)
       q[t][j] = t * 8 + g < G ? *reinterpret_cast<const uint4*>(qh + 8 * (c + 4 * j)) : make_uint4(0u, 0u, 0u, 0u);
   }
-
   float2* ws = a.ws + ((int64_t)r * a.Hkv + kvh) * a.width;
-  for (int p0 = begin + warp * 16; p0 < end; p0 += kScoreTile) {
-    const int pa = p0 + g, pb = p0 + g + 8;
-    const uint4* ra = nullptr;
-    const uint4* rb = nullptr;
-    if (pa < end)
-      ra = reinterpret_cast<const uint4*>(a.bounds + ((int64_t)table_page(bt, pa, a.num_pages) * a.Hkv + kvh) * 2 * D);
-    if (pb < end)
-      rb = reinterpret_cast<const uint4*>(a.bounds + ((int64_t)table_page(bt, pb, a.num_pages) * a.Hkv + kvh) * 2 * D);
-    uint4 va[8], vb[8];
+  uint32_t slot = ring;
+  for (int it = 0; it < passes; ++it) {
+    const int p0 = begin + (it * kWarps + warp) * 16;
+    if (p0 >= end) break;                    // this warp's later passes lie past the end as well
+    cp_async_wait<kStages - 1>();
+    float s[NH][4][4], m[NH][4];
+#pragma unroll
+    for (int t = 0; t < NH; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = m[t][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      va[j] = ra ? ld_stream(ra + c + 4 * j) : make_uint4(0u, 0u, 0u, 0u);
-      vb[j] = rb ? ld_stream(rb + c + 4 * j) : make_uint4(0u, 0u, 0u, 0u);
-    }
-    float best_a = -INFINITY, best_b = -INFINITY, err_a = 0.f, err_b = 0.f;
+      const uint4 va = lds16(slot + j * kUnit), vb = lds16(slot + (8 + j) * kUnit);
+      const uint32_t* pa4 = reinterpret_cast<const uint32_t*>(&va);
+      const uint32_t* pb4 = reinterpret_cast<const uint32_t*>(&vb);
 #pragma unroll
-    for (int t = 0; t < NH; ++t) {
-      float s[4][4], m[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = m[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t* pa4 = reinterpret_cast<const uint32_t*>(&va[j]);
-        const uint32_t* pb4 = reinterpret_cast<const uint32_t*>(&vb[j]);
+      for (int t = 0; t < NH; ++t) {
         const uint32_t* q4 = reinterpret_cast<const uint32_t*>(&q[t][j & 3]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t b0 = j < 4 ? min_nan(q4[2 * h], 0u) : max_nan(q4[2 * h], 0u);
           const uint32_t b1 = j < 4 ? min_nan(q4[2 * h + 1], 0u) : max_nan(q4[2 * h + 1], 0u);
-          mma_bf16(s[j & 3], pa4[2 * h], pb4[2 * h], pa4[2 * h + 1], pb4[2 * h + 1], b0, b1);
+          mma_bf16(s[t][j & 3], pa4[2 * h], pb4[2 * h], pa4[2 * h + 1], pb4[2 * h + 1], b0, b1);
           constexpr uint32_t kAbs = 0x7fff7fffu;
-          mma_bf16(m, pa4[2 * h] & kAbs, pb4[2 * h] & kAbs, pa4[2 * h + 1] & kAbs, pb4[2 * h + 1] & kAbs, b0 & kAbs,
-                   b1 & kAbs);
+          mma_bf16(m[t], pa4[2 * h] & kAbs, pb4[2 * h] & kAbs, pa4[2 * h + 1] & kAbs, pb4[2 * h + 1] & kAbs,
+                   b0 & kAbs, b1 & kAbs);
         }
       }
+    }
+    issue(it + kStages, slot);
+    slot = slot == ring + (kStages - 1) * kStage ? ring : slot + kStage;
+    float best_a = -INFINITY, best_b = -INFINITY, err_a = 0.f, err_b = 0.f;
+#pragma unroll
+    for (int t = 0; t < NH; ++t) {
       // columns 2c, 2c + 1 of pages g and g + 8
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float v = (s[0][i] + s[1][i]) + (s[2][i] + s[3][i]);
+        const float v = (s[t][0][i] + s[t][1][i]) + (s[t][2][i] + s[t][3][i]);
         if (t * 8 + 2 * c + (i & 1) < G) {
-          const bool fin = isfinite(v) && isfinite(m[i]);
+          const bool fin = isfinite(v) && isfinite(m[t][i]);
           float& b = i < 2 ? best_a : best_b;
           float& e = i < 2 ? err_a : err_b;
           b = fmaxf(b, fin ? v : INFINITY);
-          e = fmaxf(e, fin ? m[i] * kScoreErr : 0.f);
+          e = fmaxf(e, fin ? m[t][i] * kScoreErr : 0.f);
         }
       }
     }
@@ -245,10 +306,11 @@ __global__ void __launch_bounds__(128) page_score_kernel(const SelectArgs a, int
       err_b = fmaxf(err_b, __shfl_xor_sync(kFull, err_b, o));
     }
     if (c == 0) {
-      if (pa < end) ws[pa] = make_float2(best_a, isinf(best_a) ? 0.f : err_a);
-      if (pb < end) ws[pb] = make_float2(best_b, isinf(best_b) ? 0.f : err_b);
+      if (p0 + g < end) ws[p0 + g] = make_float2(best_a, isinf(best_a) ? 0.f : err_a);
+      if (p0 + g + 8 < end) ws[p0 + g + 8] = make_float2(best_b, isinf(best_b) ? 0.f : err_b);
     }
   }
+  cp_async_wait<0>();
 }
 
 // ===========================================================================
@@ -260,9 +322,13 @@ __global__ void __launch_bounds__(128) page_score_kernel(const SelectArgs a, int
 // s > s_k, and of these one with s - e > upper = max over s <= s_k of (s + e) beats
 // all others, so it is in.  The pages in between are compared exactly.
 // ===========================================================================
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelList = 512;                // open pages that are ranked in shared memory
+//
+// s_k comes from a histogram of 1024 equal intervals between the smallest and the
+// largest score and a ranking of the pages of the interval it falls into; where
+// one interval holds too many, from a bisection over the scores' bit patterns.
+// ===========================================================================
+constexpr int kSelList = 512;                // pages that are ranked in shared memory
+constexpr int kSelBins = 1024;
 
 __device__ __forceinline__ uint32_t order_key(float f) {
   const uint32_t u = __float_as_uint(f);
@@ -300,16 +366,19 @@ __device__ __forceinline__ double exact_score(const SelectArgs& a, const __nv_bf
   return best + 0.0;   // -0 becomes +0: equal scores have equal keys
 }
 
-// ITEMS > 0: the row's scores stay in registers (up to ITEMS * 512 pages);
+// ITEMS > 0: the row's scores stay in registers (up to ITEMS * NT pages);
 // ITEMS = 0: they are read again for every pass.
-template <int ITEMS>
-__global__ void __launch_bounds__(kSelThreads) page_select_kernel(const SelectArgs a) {
+template <int NT, int ITEMS>
+__global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
+  constexpr int kSelThreads = NT, kSelWarps = NT / 32;
   pdl_trigger();
   pdl_wait();
   extern __shared__ uint32_t masks[];        // in | open | prefix, `words` each
   __shared__ int cnt[3];
   __shared__ uint32_t red[2][kSelWarps];
-  __shared__ int totals[3];
+  __shared__ int totals[4];
+  __shared__ int hist[kSelBins];
+  __shared__ float found_sk;
   __shared__ int list_idx[kSelList];
   __shared__ double list_val[kSelList];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -333,28 +402,29 @@ __global__ void __launch_bounds__(kSelThreads) page_select_kernel(const SelectAr
   uint32_t* prefix = masks + 2 * words;
   const int trips = (n + kSelThreads - 1) / kSelThreads;
 
-  float sc[ITEMS > 0 ? ITEMS : 1];
+  float2 sc[ITEMS > 0 ? ITEMS : 1];
   if (ITEMS > 0) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int p = i * kSelThreads + tid;
-      sc[i] = p >= mid0 && p < mid1 ? ws[p].x : -INFINITY;
+      sc[i] = p >= mid0 && p < mid1 ? ws[p] : make_float2(-INFINITY, 0.f);
     }
   }
-  // f(trip, page, is it a competing page, its score) for every page of the thread
+  // f(page, is it a competing page, its score, its error bound) for every page of the thread
   auto each = [&](auto&& f) {
     if (ITEMS > 0) {
 #pragma unroll
       for (int i = 0; i < (ITEMS > 0 ? ITEMS : 1); ++i) {
         if (i >= trips) break;
         const int p = i * kSelThreads + tid;
-        f(p, p >= mid0 && p < mid1, sc[i]);
+        f(p, p >= mid0 && p < mid1, sc[i].x, sc[i].y);
       }
     } else {
       for (int i = 0; i < trips; ++i) {
         const int p = i * kSelThreads + tid;
         const bool on = p >= mid0 && p < mid1;
-        f(p, on, on ? ws[p].x : -INFINITY);
+        const float2 v = on ? ws[p] : make_float2(-INFINITY, 0.f);
+        f(p, on, v.x, v.y);
       }
     }
   };
@@ -364,63 +434,108 @@ __global__ void __launch_bounds__(kSelThreads) page_select_kernel(const SelectAr
     __syncthreads();
     if (lane == 0) red[0][warp] = lo, red[1][warp] = hi;
     __syncthreads();
-    out_lo = red[0][0], out_hi = red[1][0];
-#pragma unroll
-    for (int w = 1; w < kSelWarps; ++w) out_lo = min(out_lo, red[0][w]), out_hi = max(out_hi, red[1][w]);
+    out_lo = __reduce_min_sync(kFull, red[0][lane % kSelWarps]);
+    out_hi = __reduce_max_sync(kFull, red[1][lane % kSelWarps]);
   };
 
-  if (tid < 3) cnt[tid] = 0, totals[tid] = 0;
+  if (tid < 3) cnt[tid] = 0;
+  if (tid < 4) totals[tid] = 0;
+  for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
   float lower = INFINITY, upper = -INFINITY, sk = INFINITY;
   if (k > 0) {
-    // s_k: bisection over the order-preserving integer keys
-    uint32_t kmin = 0xffffffffu, kmax = 0u;
-    each([&](int, bool on, float s) {
-      if (on) kmin = min(kmin, order_key(s)), kmax = max(kmax, order_key(s));
+    uint32_t kmin = 0xffffffffu, kmax = 0u, fmaxk = 0u;
+    each([&](int, bool on, float s, float) {
+      if (!on) return;
+      const uint32_t key = order_key(s);
+      kmin = min(kmin, key), kmax = max(kmax, key);
+      if (s < INFINITY) fmaxk = max(fmaxk, key);
     });
     uint32_t lo, hi;
-    block_minmax(kmin, kmax, lo, hi);   // (its barriers publish cnt = 0)
-    ++hi;                               // count(>= lo) >= k, count(>= hi) < k
-    bool split = false;
-    for (int it = 0; hi - lo > 1; ++it) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      int mine = 0;
-      each([&](int, bool on, float s) { mine += on && order_key(s) >= mid; });
-      mine = __reduce_add_sync(kFull, mine);
-      if (lane == 0 && mine) atomicAdd(&cnt[it % 3], mine);
-      if (tid == 0) cnt[(it + 1) % 3] = 0;   // last read before the previous barrier
-      __syncthreads();
-      const int total = cnt[it % 3];
-      if (total >= k) lo = mid; else hi = mid;
-      if (total == k) {
-        split = true;
-        break;
+    block_minmax(kmin, fmaxk, lo, hi);  // (its barriers publish the zeroed counters)
+    // intervals of the finite scores, +infinity in the last one; monotone in the score
+    const float vmin = key_value(lo), vmax = hi >= lo ? key_value(hi) : vmin;
+    const float width = vmax - vmin;
+    const float scale = width > 0.f && width < INFINITY ? (kSelBins - 1) / width : 0.f;
+    auto bin_of = [&](float s) { return s < INFINITY ? min(kSelBins - 2, (int)((s - vmin) * scale)) : kSelBins - 1; };
+    each([&](int, bool on, float s, float) {
+      if (on) atomicAdd(&hist[bin_of(s)], 1);
+    });
+    __syncthreads();
+    // the first warp finds the interval of the k-th largest: 32 bins per lane, from the top
+    if (warp == 0) {
+      int sum = 0;
+      for (int i = 0; i < 32; ++i) sum += hist[kSelBins - 1 - lane * 32 - (i + lane) % 32];
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kFull, incl, o);
+        if (lane >= o) incl += v;
       }
+      const uint32_t reach = __ballot_sync(kFull, incl >= k);
+      const int src = __ffs(reach) - 1;
+      int above = __shfl_sync(kFull, incl - sum, src);
+      // the 32 bins of that lane, one per lane
+      const int mine = hist[kSelBins - 1 - src * 32 - lane];
+      int in2 = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kFull, in2, o);
+        if (lane >= o) in2 += v;
+      }
+      const int at = __ffs(__ballot_sync(kFull, above + in2 >= k)) - 1;
+      above += __shfl_sync(kFull, in2 - mine, at);
+      const int members = __shfl_sync(kFull, mine, at);
+      if (lane == 0) cnt[0] = kSelBins - 1 - src * 32 - at, cnt[1] = k - above, cnt[2] = members;
     }
-    if (split) {                        // s_k is the smallest key of the k that reach `lo`
-      uint32_t m = 0xffffffffu, dummy;
-      each([&](int, bool on, float s) {
-        if (on && order_key(s) >= lo) m = min(m, order_key(s));
+    __syncthreads();
+    const int bin = cnt[0], place = cnt[1], members = cnt[2];
+    if (members <= kSelList) {
+      float* vals = reinterpret_cast<float*>(list_val);
+      each([&](int, bool on, float s, float) {
+        if (on && bin_of(s) == bin) vals[atomicAdd(&totals[3], 1)] = s;
       });
-      block_minmax(m, 0u, lo, dummy);
+      __syncthreads();
+      for (int i = tid; i < members; i += kSelThreads) {
+        const float v = vals[i];
+        int rank = 0;
+        for (int j = 0; j < members; ++j) rank += vals[j] > v || (vals[j] == v && j < i);
+        if (rank == place - 1) found_sk = v;
+      }
+      __syncthreads();
+      sk = found_sk;
+    } else {
+      // bisection over the order-preserving integer keys
+      block_minmax(kmin, kmax, lo, hi);
+      if (tid < 3) cnt[tid] = 0;
+      __syncthreads();
+      ++hi;                             // count(>= lo) >= k, count(>= hi) < k
+      for (int it = 0; hi - lo > 1; ++it) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        int mine = 0;
+        each([&](int, bool on, float s, float) { mine += on && order_key(s) >= mid; });
+        mine = __reduce_add_sync(kFull, mine);
+        if (lane == 0 && mine) atomicAdd(&cnt[it % 3], mine);
+        if (tid == 0) cnt[(it + 1) % 3] = 0;   // last read before the previous barrier
+        __syncthreads();
+        if (cnt[it % 3] >= k) lo = mid; else hi = mid;
+      }
+      sk = key_value(lo);
     }
-    sk = key_value(lo);
     uint32_t low_key = 0xffffffffu, up_key = 0u;
-    each([&](int p, bool on, float s) {
+    each([&](int, bool on, float s, float e) {
       if (!on) return;
-      const float e = ws[p].y;
       if (s >= sk) low_key = min(low_key, order_key(s - e));
       if (s <= sk) up_key = max(up_key, order_key(s + e));
     });
-    block_minmax(low_key, up_key, low_key, up_key);
-    lower = key_value(low_key);
-    upper = key_value(up_key);
+    block_minmax(low_key, up_key, lo, hi);
+    lower = key_value(lo);
+    upper = key_value(hi);
   }
   __syncthreads();
-  each([&](int p, bool on, float s) {
+  each([&](int p, bool on, float s, float e) {
     bool in = p < n && !on;             // the first and the last pages
     bool open = false;
     if (on && k > 0) {
-      const float e = ws[p].y;
       if (s > sk) {
         in = s - e > upper;
         open = !in;
@@ -571,7 +686,7 @@ __global__ void __launch_bounds__(kSelThreads) page_select_kernel(const SelectAr
 // tokens; the sum of the weights is kept in fp32 from the same rounded values,
 // so the rounding does not scale the output.
 // ===========================================================================
-constexpr int kSpWarps = 4;
+constexpr int kSpWarps = kWarps;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t x;
@@ -597,12 +712,12 @@ struct SparseSmem {
 };
 
 template <int NH>
-__global__ void __launch_bounds__(kSpWarps * 32) decode_sparse_kernel(const SparseArgs a, int cl) {
-  extern __shared__ __align__(16) uint8_t raw[];
-  SparseSmem<NH>& sm = *reinterpret_cast<SparseSmem<NH>*>(raw);
+__global__ void __launch_bounds__(kThreads, 2) decode_sparse_kernel(const SparseArgs a, int cl) {
+  extern __shared__ __align__(128) uint8_t raw[];
+  SparseSmem<NH>& sm = *reinterpret_cast<SparseSmem<NH>*>(raw);   // over the ring, after the last page
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int part = cl > 1 ? (int)cluster_rank() : 0;
   const int unit = blockIdx.x / cl;
@@ -612,10 +727,63 @@ __global__ void __launch_bounds__(kSpWarps * 32) decode_sparse_kernel(const Spar
   const int n = (L + PAGE - 1) / PAGE;
   const int tok = a.tok_index[r];
   const bool tok_ok = tok >= 0 && tok < a.tokens;
-  if (!tok_ok && threadIdx.x == 0) set_error(kErrBadIndex, (unsigned long long)r);
+  if (!tok_ok && tid == 0) set_error(kErrBadIndex, (unsigned long long)r);
   const int count = tok_ok ? min(n, a.budget) : 0;
   const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
   const int32_t* sel = a.sel + ((int64_t)r * a.Hkv + kvh) * a.budget;
+
+  // this warp's pages: entries w, w + stride, ... of the list; lane j holds the
+  // j-th of a window of 32 (first token, physical page), the next window under way
+  const int stride = cl * kSpWarps, w = part * kSpWarps + warp;
+  const int mine = count > w ? (count - w + stride - 1) / stride : 0;
+  int win_tok, win_phys, next_page = -1;
+  auto fetch_window = [&](int i) { next_page = i + lane < mine ? sel[w + (i + lane) * stride] : -1; };
+  auto open_window = [&](int i) {
+    win_tok = L;                        // nothing valid in the page
+    win_phys = 0;
+    if (i + lane < mine) {
+      if (next_page < 0 || next_page >= n) {
+        set_error(kErrBadIndex, (unsigned long long)r);
+      } else {
+        win_tok = next_page * PAGE;
+        win_phys = table_page(bt, next_page, a.num_pages);
+      }
+    }
+    fetch_window(i + 32);
+  };
+  fetch_window(0);
+
+  // a lane's pieces of a page: K rows g and g + 8, pieces c, c + 4, ...; V rows 2c,
+  // 2c + 1, 2c + 8, 2c + 9, piece g of both halves of the dimensions
+  const uint32_t ring = smem_u32(raw) + tid * 16;
+  const __nv_bfloat16* kl = a.kcache + (int64_t)kvh * PAGE * D + g * D + c * 8;
+  const __nv_bfloat16* vl = a.vcache + (int64_t)kvh * PAGE * D + 2 * c * D + g * 8;
+  const int64_t page_elems = (int64_t)a.Hkv * PAGE * D;
+  auto issue = [&](int i, uint32_t slot) -> int {   // the page's first token
+    int t0 = L;
+    if (i < mine) {
+      if ((i & 31) == 0) open_window(i);
+      t0 = __shfl_sync(kFull, win_tok, i & 31);
+      const int64_t at = __shfl_sync(kFull, win_phys, i & 31) * page_elems;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        cp_async16(slot + j * kUnit, kl + at + j * 32, true);
+        cp_async16(slot + (4 + j) * kUnit, kl + at + 8 * D + j * 32, true);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int t = (x & 1) + (x >> 1) * 8;
+        const bool on = t0 + 2 * c + t < L;         // zeros past the sequence's end
+        cp_async16(slot + (8 + x) * kUnit, vl + at + t * D, on);
+        cp_async16(slot + (12 + x) * kUnit, vl + at + t * D + 64, on);
+      }
+    }
+    cp_async_commit();
+    return t0;
+  };
+  int first_tok[kStages];
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) first_tok[i] = issue(i, ring + i * kStage);
 
   uint4 q[NH][4];
 #pragma unroll
@@ -635,60 +803,34 @@ __global__ void __launch_bounds__(kSpWarps * 32) decode_sparse_kernel(const Spar
     for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
   }
 
-  // this warp's pages: entries w, w + stride, ... of the list; lane j holds the
-  // j-th of the current window of 32 (first token, physical page)
-  const int stride = cl * kSpWarps, w = part * kSpWarps + warp;
-  const int mine = count > w ? (count - w + stride - 1) / stride : 0;
-  int win_tok = 0, win_phys = 0;
+  uint32_t slot = ring;
   for (int i = 0; i < mine; ++i) {
-    if ((i & 31) == 0) {
-      const int e = w + (i + lane) * stride;
-      win_tok = L;                      // nothing valid in the page
-      win_phys = 0;
-      if (i + lane < mine) {
-        const int lp = sel[e];
-        if (lp < 0 || lp >= n) {
-          set_error(kErrBadIndex, (unsigned long long)r);
-        } else {
-          win_tok = lp * PAGE;
-          win_phys = table_page(bt, lp, a.num_pages);
-        }
-      }
-    }
-    const int t0 = __shfl_sync(kFull, win_tok, i & 31);
-    const int64_t phys = __shfl_sync(kFull, win_phys, i & 31);
-    const int64_t base = (phys * a.Hkv + kvh) * PAGE * D;
-    const uint4* ka = reinterpret_cast<const uint4*>(a.kcache + base + g * D);
-    const uint4* kb = ka + 8 * D / 8;
-    uint4 k0[4], k1[4], v[2][4];        // v[half of the dims][token 2c, 2c + 1, 2c + 8, 2c + 9]
+    cp_async_wait<kStages - 1>();
+    const int t0 = first_tok[0];
+#pragma unroll
+    for (int x = 0; x + 1 < kStages; ++x) first_tok[x] = first_tok[x + 1];
+    uint32_t p[NH][2];
+    float s[NH][2][4];
+#pragma unroll
+    for (int t = 0; t < NH; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) s[t][x][0] = s[t][x][1] = s[t][x][2] = s[t][x][3] = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      k0[j] = ld_stream(ka + c + 4 * j);
-      k1[j] = ld_stream(kb + c + 4 * j);
+      const uint4 k0 = lds16(slot + j * kUnit), k1 = lds16(slot + (4 + j) * kUnit);
+#pragma unroll
+      for (int t = 0; t < NH; ++t) {
+        mma_bf16(s[t][0], k0.x, k1.x, k0.y, k1.y, q[t][j].x, q[t][j].y);
+        mma_bf16(s[t][1], k0.z, k1.z, k0.w, k1.w, q[t][j].z, q[t][j].w);
+      }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int t = 2 * c + (x & 1) + (x >> 1) * 8;
-        v[h][x] = t0 + t < L ? ld_stream(a.vcache + base + t * D + h * 64 + g * 8) : make_uint4(0u, 0u, 0u, 0u);
-      }
-    uint32_t p[NH][2];
-#pragma unroll
     for (int t = 0; t < NH; ++t) {
-      float s[2][4];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        mma_bf16(s[0], k0[j].x, k1[j].x, k0[j].y, k1[j].y, q[t][j].x, q[t][j].y);
-        mma_bf16(s[1], k0[j].z, k1[j].z, k0[j].w, k1[j].w, q[t][j].z, q[t][j].w);
-      }
       // x[0], x[1]: token g, heads 2c, 2c + 1; x[2], x[3]: token g + 8
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        x[e] = t0 + g + (e >> 1) * 8 < L ? (s[0][e] + s[1][e]) * a.scale_log2 : -INFINITY;
+        x[e] = t0 + g + (e >> 1) * 8 < L ? (s[t][0][e] + s[t][1][e]) * a.scale_log2 : -INFINITY;
       float pr[4];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -713,6 +855,9 @@ __global__ void __launch_bounds__(kSpWarps * 32) decode_sparse_kernel(const Spar
       p[t][0] = movmatrix_trans(plo);
       p[t][1] = movmatrix_trans(phi);
     }
+    uint4 v[2][4];                      // v[half of the dimensions][token 2c, 2c + 1, 2c + 8, 2c + 9]
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[0][x] = lds16(slot + (8 + x) * kUnit), v[1][x] = lds16(slot + (12 + x) * kUnit);
     const uint32_t* vw = reinterpret_cast<const uint32_t*>(v);   // [half][token][word]
 #pragma unroll
     for (int i8 = 0; i8 < 8; ++i8) {
@@ -725,7 +870,11 @@ __global__ void __launch_bounds__(kSpWarps * 32) decode_sparse_kernel(const Spar
 #pragma unroll
       for (int t = 0; t < NH; ++t) mma_bf16(o[t][i8], a0, a1, a2, a3, p[t][0], p[t][1]);
     }
+    first_tok[kStages - 1] = issue(i + kStages, slot);
+    slot = slot == ring + (kStages - 1) * kStage ? ring : slot + kStage;
   }
+  cp_async_wait<0>();
+  __syncthreads();                      // the ring's memory becomes the warps' results
 
   // join: o[t][i][0..1] = dim 8g + i, heads 2c, 2c + 1; [2..3] = dim 64 + 8g + i
 #pragma unroll
@@ -808,35 +957,44 @@ void page_bounds(const BoundsArgs& a, cudaStream_t s) {
   launch_k(page_bounds_kernel, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, s, 1, b);
 }
 
+namespace {
+void raise_smem(const void* k, size_t smem) {
+  if (smem <= 48 * 1024) return;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) launch_failed(e);
+}
+}  // namespace
+
 void select_pages(const SelectArgs& a, cudaStream_t s) {
   if (a.rows <= 0) return;
-  const int chunk = kScoreTile;
-  const int chunks = (a.width + chunk - 1) / chunk;
-  const dim3 grid((unsigned)(chunks * a.Hkv), (unsigned)a.rows);
   if (a.width > a.budget) {
-    if (a.Hq / a.Hkv <= 8) launch_k(page_score_kernel<1>, grid, dim3(128), 0, s, 1, a, chunk);
-    else launch_k(page_score_kernel<2>, grid, dim3(128), 0, s, 1, a, chunk);
+    // up to eight passes of 64 pages per CTA, fewer where that leaves SMs without work
+    const int64_t tiles = (int64_t)a.rows * a.Hkv * ((a.width + kScoreTile - 1) / kScoreTile);
+    const int64_t want = tiles / (4 * sm_count());
+    const int passes = want < 1 ? 1 : want > kScorePasses ? kScorePasses : (int)want;
+    const int chunk = passes * kScoreTile;
+    const dim3 grid((unsigned)((a.width + chunk - 1) / chunk * a.Hkv), (unsigned)a.rows);
+    auto k = a.Hq / a.Hkv <= 8 ? page_score_kernel<1> : page_score_kernel<2>;
+    raise_smem(reinterpret_cast<const void*>(k), kStages * kStage);
+    launch_k(k, grid, dim3(kThreads), kStages * kStage, s, 1, a, passes);
   }
   const size_t smem = (size_t)((a.width + 31) / 32) * 3 * sizeof(uint32_t);   // at most 24 KB
-  const dim3 sgrid((unsigned)a.Hkv, (unsigned)a.rows);
-  const int items = (a.width + kSelThreads - 1) / kSelThreads;
-  if (items <= 1) launch_k(page_select_kernel<1>, sgrid, dim3(kSelThreads), smem, s, 1, a);
-  else if (items <= 4) launch_k(page_select_kernel<4>, sgrid, dim3(kSelThreads), smem, s, 1, a);
-  else if (items <= 16) launch_k(page_select_kernel<16>, sgrid, dim3(kSelThreads), smem, s, 1, a);
-  else launch_k(page_select_kernel<0>, sgrid, dim3(kSelThreads), smem, s, 1, a);
+  const dim3 grid((unsigned)a.Hkv, (unsigned)a.rows);
+  if (a.width <= 512) launch_k(page_select_kernel<256, 2>, grid, dim3(256), smem, s, 1, a);
+  else if (a.width <= 2048) launch_k(page_select_kernel<512, 4>, grid, dim3(512), smem, s, 1, a);
+  else if (a.width <= 8192) launch_k(page_select_kernel<1024, 8>, grid, dim3(1024), smem, s, 1, a);
+  else launch_k(page_select_kernel<1024, 0>, grid, dim3(1024), smem, s, 1, a);
 }
 
 void decode_sparse(const SparseArgs& a, cudaStream_t s) {
   if (a.rows <= 0) return;
   const int64_t units = (int64_t)a.rows * a.Hkv;
-  const int64_t slots = (int64_t)sm_count() * 3;
+  const int64_t slots = (int64_t)sm_count() * 2;
   int cl = 1;
   while (cl < 8 && units * cl * 2 <= slots && a.budget >= kSpWarps * cl * 2) cl *= 2;
-  const bool wide = a.Hq / a.Hkv > 8;
-  const size_t smem = wide ? sizeof(SparseSmem<2>) : sizeof(SparseSmem<1>);   // 33 KB / 17 KB
-  const dim3 grid((unsigned)(units * cl));
-  if (wide) launch_k(decode_sparse_kernel<2>, grid, dim3(kSpWarps * 32), smem, s, (unsigned)cl, a, cl);
-  else launch_k(decode_sparse_kernel<1>, grid, dim3(kSpWarps * 32), smem, s, (unsigned)cl, a, cl);
+  auto k = a.Hq / a.Hkv <= 8 ? decode_sparse_kernel<1> : decode_sparse_kernel<2>;
+  raise_smem(reinterpret_cast<const void*>(k), kStages * kStage);   // covers the join's 17 / 33 KB
+  launch_k(k, dim3((unsigned)(units * cl)), dim3(kThreads), kStages * kStage, s, (unsigned)cl, a, cl);
 }
 
 }  // namespace attn
