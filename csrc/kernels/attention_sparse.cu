@@ -49,15 +49,13 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16-byte copy into shared memory; zeros where `on` is false.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  const int n = on ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Streaming 16-byte load: K and V are used once.
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   uint4 v;
@@ -67,16 +65,6 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
                : "memory");
   return v;
 }
-
-// The streaming kernels (scores, attention) run four warps whose lanes copy
-// their own operand pieces into their own slots of a ring in shared memory and
-// read only those back: 16 pieces of 16 bytes per lane and stage, a pipeline
-// without registers and without a barrier.
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kUnit = kThreads * 16;
-constexpr int kStage = 16 * kUnit;           // 32 KB
-constexpr int kStages = 3;                   // 96 KB: two CTAs per SM
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   uint32_t y;
@@ -99,6 +87,13 @@ __device__ __forceinline__ int table_page(const int32_t* bt, int idx, int num_pa
     return 0;
   }
   return p;
+}
+
+// Waits for copies under way after another wait ran out, up to the same limit.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 <= wait_limit_ns()) {
+  }
 }
 
 // A row's KV length; a length beyond the block table is recorded and cut.
@@ -163,12 +158,13 @@ __global__ void __launch_bounds__(128) page_bounds_kernel(const BoundsArgs a) {
 }
 
 // ===========================================================================
-// Page scores.  A warp takes 16 pages at a time as the 16 rows of m16n8k16;
-// lane (g, c) = (lane / 4, lane % 4) loads 16-byte pieces c, c + 4, ... of the
-// bounds of pages g and g + 8.  A piece is eight consecutive dimensions, which
-// serve two k-steps: the order of k is free as long as the queries use the
-// same one, so no shared memory is needed.  lo and hi lie behind one another,
-// so pieces 0..15 meet min(q, 0) and pieces 16..31 meet max(q, 0).
+// Page scores.  A warp takes 16 pages at a time as the 16 rows of m16n8k16.  One
+// bulk copy per page (512 bytes: lo, then hi) brings them into the warp's own
+// ring; rows lie 576 bytes apart, so that the 16-byte pieces c, c + 4, ... which
+// lane (g, c) = (lane / 4, lane % 4) reads of pages g and g + 8 hit all banks.  A
+// piece is eight consecutive dimensions, which serve two k-steps: the order of
+// k is free as long as the queries use the same one.  Pieces 0..15 (lo) meet
+// min(q, 0) and pieces 16..31 (hi) meet max(q, 0).
 //
 // Error bound: a k16 step adds 16 exact products to the accumulator with at
 // most 17 roundings or truncations at the largest addend, 2^-23 each; four
@@ -177,70 +173,72 @@ __global__ void __launch_bounds__(128) page_bounds_kernel(const BoundsArgs a) {
 // same instruction on the operands without their signs.
 // ===========================================================================
 constexpr float kScoreErr = 1.f / 32768.f;   // 2^-15, four times what is derived above
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
 constexpr int kScoreTile = 16 * kWarps;      // pages of one pass of a CTA
 constexpr int kScorePasses = 8;              // most passes of a CTA
+constexpr int kScoreStages = 3;
+constexpr int kRow = 576, kRowBytes = 512;   // a page's place and its bytes
+constexpr int kScoreStage = 16 * kRow;
+constexpr int kScoreSmem = kWarps * kScoreStages * kScoreStage;   // 108 KB: two CTAs per SM
 
 template <int NH>   // groups of eight query heads
 __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArgs a, int passes) {
   extern __shared__ __align__(128) uint8_t raw[];
-  __shared__ int phys[kScorePasses * kScoreTile];
-  pdl_trigger();
-  pdl_wait();
+  __shared__ __align__(8) uint64_t full[kWarps][kScoreStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.x % a.Hkv, chunk = blockIdx.x / a.Hkv;
   const int r = blockIdx.y;
   const int G = a.Hq / a.Hkv;
-  const int begin = chunk * passes * kScoreTile;
+  const int begin = chunk * passes * kScoreTile + warp * 16;   // this warp's first page; the next ones 64 further
+  if (lane < kScoreStages) mbar_init(&full[warp][lane], 1);
+  fence_barrier_init();
+  __syncwarp();
+  pdl_wait();
   const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
-  const int span = min(passes * kScoreTile, a.width - begin);
-  int table[kScorePasses * kScoreTile / kThreads];   // fetched before the length is known
+  // lane l holds page l % 16 of passes l / 16, 2 + l / 16, ...; fetched before the length is known
+  int table[kScorePasses / 2];
 #pragma unroll
-  for (int i = 0; i < kScorePasses * kScoreTile / kThreads; ++i) {
-    const int p = i * kThreads + tid;
-    table[i] = p < span ? bt[begin + p] : 0;
+  for (int i = 0; i < kScorePasses / 2; ++i) {
+    const int pass = 2 * i + (lane >> 4), p = begin + pass * kScoreTile + (lane & 15);
+    table[i] = pass < passes && p < a.width ? bt[p] : 0;
   }
+  const int tok = a.tok_index[r];
   const int L = row_length(a.seq_lens, r, a.width);
   const int n = (L + PAGE - 1) / PAGE;
-  const int end = min(n, begin + passes * kScoreTile);
+  const int end = min(n, (chunk + 1) * passes * kScoreTile);
   if (n <= a.budget || begin >= end) return;
-  const int tok = a.tok_index[r];
   if (tok < 0 || tok >= a.tokens) {
-    if (tid == 0) set_error(kErrBadIndex, (unsigned long long)r);
+    if (lane == 0) set_error(kErrBadIndex, (unsigned long long)r);
     return;
   }
+  const int mine = (end - begin + kScoreTile - 1) / kScoreTile;   // passes of this warp
+  uint8_t* ring = raw + warp * kScoreStages * kScoreStage;
+  auto issue = [&](int it, int st) {
+    if (it >= mine) return;
+    int phys = 0;
 #pragma unroll
-  for (int i = 0; i < kScorePasses * kScoreTile / kThreads; ++i) {
-    const int p = i * kThreads + tid;
-    if (begin + p < end) {
-      if (table[i] < 0 || table[i] >= a.num_pages) {   // recorded; the reserved zero page stands in
-        set_error(kErrBadIndex, (unsigned long long)(begin + p));
-        table[i] = 0;
-      }
-      phys[p] = table[i];
+    for (int i = 0; i < kScorePasses / 2; ++i) {
+      const int v = __shfl_sync(kFull, table[i], (it & 1) * 16 + (lane & 15));
+      if (it >> 1 == i) phys = v;
     }
-  }
-  __syncthreads();
-
-  const uint32_t ring = smem_u32(raw) + tid * 16;
-  const uint4* bounds = reinterpret_cast<const uint4*>(a.bounds);
-  const int pieces = 2 * D / 8;              // of one (page, KV head)
-  auto issue = [&](int it, uint32_t slot) {
-    const int p0 = begin + (it * kWarps + warp) * 16;
-    if (it < passes && p0 < end) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int p = p0 + g + 8 * u;
-        const bool on = p < end;
-        const uint4* src = bounds + ((int64_t)phys[on ? p - begin : 0] * a.Hkv + kvh) * pieces + c;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) cp_async16(slot + (u * 8 + j) * kUnit, src + 4 * j, on);
+    const int p0 = begin + it * kScoreTile;
+    const int count = min(16, end - p0);
+    if (lane == 0) mbar_arrive_expect_tx(&full[warp][st], count * kRowBytes);
+    __syncwarp();
+    if (lane < count) {
+      if (phys < 0 || phys >= a.num_pages) {   // recorded; the reserved zero page stands in
+        set_error(kErrBadIndex, (unsigned long long)(p0 + lane));
+        phys = 0;
       }
+      bulk_load(ring + st * kScoreStage + lane * kRow, a.bounds + ((int64_t)phys * a.Hkv + kvh) * 2 * D, kRowBytes,
+                &full[warp][st]);
     }
-    cp_async_commit();
+    __syncwarp();
   };
 #pragma unroll
-  for (int i = 0; i < kStages; ++i) issue(i, ring + i * kStage);
+  for (int i = 0; i < kScoreStages; ++i) issue(i, i);
 
   uint4 q[NH][4];
 #pragma unroll
@@ -251,11 +249,20 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
       q[t][j] = t * 8 + g < G ? *reinterpret_cast<const uint4*>(qh + 8 * (c + 4 * j)) : make_uint4(0u, 0u, 0u, 0u);
   }
   float2* ws = a.ws + ((int64_t)r * a.Hkv + kvh) * a.width;
-  uint32_t slot = ring;
-  for (int it = 0; it < passes; ++it) {
-    const int p0 = begin + (it * kWarps + warp) * 16;
-    if (p0 >= end) break;                    // this warp's later passes lie past the end as well
-    cp_async_wait<kStages - 1>();
+  const uint32_t at0 = smem_u32(ring) + g * kRow + c * 16;
+  int st = 0;
+  uint32_t parity = 0;
+  for (int it = 0; it < mine; ++it) {
+    const int p0 = begin + it * kScoreTile;
+    if (!__all_sync(kFull, mbar_wait(&full[warp][st], parity, 30))) {
+      // recorded; leave once the copies under way have landed or had their time
+      for (int i = 0; i < kScoreStages && it + i < mine; ++i) {
+        const int x = st + i;
+        drain(&full[warp][x % kScoreStages], parity ^ (x >= kScoreStages ? 1u : 0u));
+      }
+      return;
+    }
+    const uint32_t at = at0 + st * kScoreStage;
     float s[NH][4][4], m[NH][4];
 #pragma unroll
     for (int t = 0; t < NH; ++t)
@@ -263,7 +270,8 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
       for (int i = 0; i < 4; ++i) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = m[t][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint4 va = lds16(slot + j * kUnit), vb = lds16(slot + (8 + j) * kUnit);
+      // rows past the last page hold what the ring held; their columns are not stored
+      const uint4 va = lds16(at + j * 64), vb = lds16(at + 8 * kRow + j * 64);
       const uint32_t* pa4 = reinterpret_cast<const uint32_t*>(&va);
       const uint32_t* pb4 = reinterpret_cast<const uint32_t*>(&vb);
 #pragma unroll
@@ -280,8 +288,10 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
         }
       }
     }
-    issue(it + kStages, slot);
-    slot = slot == ring + (kStages - 1) * kStage ? ring : slot + kStage;
+    __syncwarp();
+    fence_proxy_async_smem();
+    issue(it + kScoreStages, st);
+    if (++st == kScoreStages) st = 0, parity ^= 1;
     float best_a = -INFINITY, best_b = -INFINITY, err_a = 0.f, err_b = 0.f;
 #pragma unroll
     for (int t = 0; t < NH; ++t) {
@@ -310,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
       if (p0 + g + 8 < end) ws[p0 + g + 8] = make_float2(best_b, isinf(best_b) ? 0.f : err_b);
     }
   }
-  cp_async_wait<0>();
+  pdl_trigger();
 }
 
 // ===========================================================================
@@ -320,12 +330,14 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
 // last ones, at least k pages have an exact score >= lower = min over s >= s_k
 // of (s - e), so a page with s + e < lower is out; at most k - 1 pages have
 // s > s_k, and of these one with s - e > upper = max over s <= s_k of (s + e) beats
-// all others, so it is in.  The pages in between are compared exactly.
-// ===========================================================================
+// all others, so it is in.  The pages in between are open and compared exactly
+// where they are more than the places left.
 //
-// s_k comes from a histogram of 1024 equal intervals between the smallest and the
-// largest score and a ranking of the pages of the interval it falls into; where
-// one interval holds too many, from a bisection over the scores' bit patterns.
+// The scores stay in registers, a warp holding consecutive pages.  s_k comes from
+// a histogram of 1024 equal intervals between the smallest and the largest score
+// and a ranking of the pages of the interval it falls into.  Where an interval
+// holds too many pages, too many are open or the row is too long for registers,
+// a slower general routine takes over.
 // ===========================================================================
 constexpr int kSelList = 512;                // pages that are ranked in shared memory
 constexpr int kSelBins = 1024;
@@ -342,22 +354,41 @@ __device__ __forceinline__ unsigned long long order_key64(double f) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
+struct SelectSmem {
+  int hist[kSelBins];
+  float list_s[kSelList], list_e[kSelList];
+  int list_idx[kSelList];
+  double list_val[kSelList];
+  uint32_t red[2][32];
+  int count_in[32], count_open[32];
+  int cnt[4], totals[4];
+  float sk;
+};
+
+// One (row, KV head) of a selection.
+struct SelectUnit {
+  float2* ws;
+  int32_t* sel;
+  const __nv_bfloat16* q;        // the group's query heads
+  const int32_t* bt;
+  int kvh, G, n, first, mid1, k;   // pages, first competing, last competing + 1, places for them
+};
+
 // Exact score of one page by one warp: four dimensions per lane, fp64.
-__device__ __forceinline__ double exact_score(const SelectArgs& a, const __nv_bfloat16* q, const __nv_bfloat16* b,
-                                              int G, int lane) {
-  float lo[4], hi[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    lo[i] = __bfloat162float(b[lane * 4 + i]);
-    hi[i] = __bfloat162float(b[D + lane * 4 + i]);
-  }
+__device__ __forceinline__ double exact_score(const SelectArgs& a, const SelectUnit& u, int page, int lane) {
+  const __nv_bfloat16* b = a.bounds + ((int64_t)table_page(u.bt, page, a.num_pages) * a.Hkv + u.kvh) * 2 * D + lane * 4;
+  const uint2 lo2 = *reinterpret_cast<const uint2*>(b), hi2 = *reinterpret_cast<const uint2*>(b + D);
+  const __nv_bfloat16* lo = reinterpret_cast<const __nv_bfloat16*>(&lo2);
+  const __nv_bfloat16* hi = reinterpret_cast<const __nv_bfloat16*>(&hi2);
   double best = -INFINITY;
-  for (int h = 0; h < G; ++h) {
+  for (int h = 0; h < u.G; ++h) {
+    const uint2 q2 = *reinterpret_cast<const uint2*>(u.q + h * D + lane * 4);
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(&q2);
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const double x = (double)__bfloat162float(q[h * D + lane * 4 + i]);
-      sum += fmax(x * (double)lo[i], x * (double)hi[i]);
+      const double x = (double)__bfloat162float(q[i]);
+      sum += fmax(x * (double)__bfloat162float(lo[i]), x * (double)__bfloat162float(hi[i]));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
@@ -366,315 +397,365 @@ __device__ __forceinline__ double exact_score(const SelectArgs& a, const __nv_bf
   return best + 0.0;   // -0 becomes +0: equal scores have equal keys
 }
 
-// ITEMS > 0: the row's scores stay in registers (up to ITEMS * NT pages);
-// ITEMS = 0: they are read again for every pass.
-template <int NT, int ITEMS>
-__global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
-  constexpr int kSelThreads = NT, kSelWarps = NT / 32;
-  pdl_trigger();
-  pdl_wait();
-  extern __shared__ uint32_t masks[];        // in | open | prefix, `words` each
-  __shared__ int cnt[3];
-  __shared__ uint32_t red[2][kSelWarps];
-  __shared__ int totals[4];
-  __shared__ int hist[kSelBins];
-  __shared__ float found_sk;
-  __shared__ int list_idx[kSelList];
-  __shared__ double list_val[kSelList];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int kvh = blockIdx.x, r = blockIdx.y;
-  const int L = row_length(a.seq_lens, r, a.width);
-  const int n = (L + PAGE - 1) / PAGE;
-  int32_t* sel = a.sel + ((int64_t)r * a.Hkv + kvh) * a.budget;
-  const int tok = a.tok_index[r];
-  if (n <= a.budget || tok < 0 || tok >= a.tokens) {
-    // everything fits; a row of a bad token (recorded by the score kernel) takes nothing
-    const int keep = n <= a.budget ? n : 0;
-    for (int i = tid; i < a.budget; i += kSelThreads) sel[i] = i < keep ? i : -1;
-    return;
-  }
-  float2* ws = a.ws + ((int64_t)r * a.Hkv + kvh) * a.width;
-  const int mid0 = a.first, mid1 = n - a.last;            // pages that compete
-  const int k = a.budget - a.first - a.last;              // for k places; k < mid1 - mid0
-  const int words = (n + 31) / 32;
+__device__ __forceinline__ void block_minmax(SelectSmem& sm, uint32_t lo, uint32_t hi, uint32_t& out_lo, uint32_t& out_hi) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x / 32;
+  lo = __reduce_min_sync(kFull, lo);
+  hi = __reduce_max_sync(kFull, hi);
+  __syncthreads();
+  if (lane == 0) sm.red[0][warp] = lo, sm.red[1][warp] = hi;
+  __syncthreads();
+  out_lo = __reduce_min_sync(kFull, sm.red[0][lane % warps]);
+  out_hi = __reduce_max_sync(kFull, sm.red[1][lane % warps]);
+}
+
+// The general routine: bisections over the scores' bit patterns, the scores read
+// again for every pass, the pages' state in bit masks.
+__device__ __noinline__ void select_general(const SelectArgs& a, const SelectUnit& u, SelectSmem& sm, uint32_t* masks) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, NT = blockDim.x, warps = NT / 32;
+  const int words = (u.n + 31) / 32;
   uint32_t* in_mask = masks;
   uint32_t* open_mask = masks + words;
-  uint32_t* prefix = masks + 2 * words;
-  const int trips = (n + kSelThreads - 1) / kSelThreads;
-
-  float2 sc[ITEMS > 0 ? ITEMS : 1];
-  if (ITEMS > 0) {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int p = i * kSelThreads + tid;
-      sc[i] = p >= mid0 && p < mid1 ? ws[p] : make_float2(-INFINITY, 0.f);
+  float sk = INFINITY, lower = INFINITY, upper = -INFINITY;
+  __syncthreads();
+  if (tid < 4) sm.cnt[tid] = 0, sm.totals[tid] = 0;
+  if (u.k > 0) {
+    uint32_t kmin = 0xffffffffu, kmax = 0u, lo, hi;
+    for (int p = u.first + tid; p < u.mid1; p += NT) {
+      const uint32_t key = order_key(u.ws[p].x);
+      kmin = min(kmin, key), kmax = max(kmax, key);
+    }
+    block_minmax(sm, kmin, kmax, lo, hi);
+    ++hi;                               // count(>= lo) >= k, count(>= hi) < k
+    for (int it = 0; hi - lo > 1; ++it) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      int mine = 0;
+      for (int p = u.first + tid; p < u.mid1; p += NT) mine += order_key(u.ws[p].x) >= mid;
+      mine = __reduce_add_sync(kFull, mine);
+      if (lane == 0 && mine) atomicAdd(&sm.cnt[it % 3], mine);
+      if (tid == 0) sm.cnt[(it + 1) % 3] = 0;   // last read before the previous barrier
+      __syncthreads();
+      if (sm.cnt[it % 3] >= u.k) lo = mid; else hi = mid;
+    }
+    sk = key_value(lo);
+    uint32_t low_key = 0xffffffffu, up_key = 0u;
+    for (int p = u.first + tid; p < u.mid1; p += NT) {
+      const float2 v = u.ws[p];
+      if (v.x >= sk) low_key = min(low_key, order_key(v.x - v.y));
+      if (v.x <= sk) up_key = max(up_key, order_key(v.x + v.y));
+    }
+    block_minmax(sm, low_key, up_key, lo, hi);
+    lower = key_value(lo);
+    upper = key_value(hi);
+  }
+  for (int w = warp; w < words; w += warps) {
+    const int p = w * 32 + lane;
+    bool in = p < u.n && (p < u.first || p >= u.mid1), open = false;
+    if (p >= u.first && p < u.mid1 && u.k > 0) {
+      const float2 v = u.ws[p];
+      if (v.x > sk) in = v.x - v.y > upper, open = !in;
+      else open = v.x + v.y >= lower;
+    }
+    const uint32_t bi = __ballot_sync(kFull, in), bo = __ballot_sync(kFull, open);
+    if (lane == 0) {
+      in_mask[w] = bi;
+      open_mask[w] = bo;
+      if (bi) atomicAdd(&sm.totals[0], __popc(bi));
+      if (bo) atomicAdd(&sm.totals[1], __popc(bo));
     }
   }
-  // f(page, is it a competing page, its score, its error bound) for every page of the thread
-  auto each = [&](auto&& f) {
-    if (ITEMS > 0) {
-#pragma unroll
-      for (int i = 0; i < (ITEMS > 0 ? ITEMS : 1); ++i) {
-        if (i >= trips) break;
-        const int p = i * kSelThreads + tid;
-        f(p, p >= mid0 && p < mid1, sc[i].x, sc[i].y);
-      }
-    } else {
-      for (int i = 0; i < trips; ++i) {
-        const int p = i * kSelThreads + tid;
-        const bool on = p >= mid0 && p < mid1;
-        const float2 v = on ? ws[p] : make_float2(-INFINITY, 0.f);
-        f(p, on, v.x, v.y);
+  __syncthreads();
+  const int n_open = sm.totals[1];
+  const int need = a.budget - sm.totals[0];   // 0 <= need <= n_open
+  if (need == n_open) {
+    for (int w = tid; w < words; w += NT) in_mask[w] |= open_mask[w];
+  } else {
+    // exact scores over the fp32 ones, which are no longer needed; bisection over
+    // their 64-bit keys, then ties by index
+    double* exact = reinterpret_cast<double*>(u.ws);
+    for (int w = warp; w < words; w += warps) {
+      uint32_t m = open_mask[w];
+      while (m) {
+        const int p = w * 32 + __ffs(m) - 1;
+        m &= m - 1;
+        const bool finite = isfinite(u.ws[p].x);
+        __syncwarp();
+        const double v = finite ? exact_score(a, u, p, lane) : INFINITY;
+        if (lane == 0) exact[p] = v;
       }
     }
-  };
-  auto block_minmax = [&](uint32_t lo, uint32_t hi, uint32_t& out_lo, uint32_t& out_hi) {
-    lo = __reduce_min_sync(kFull, lo);
-    hi = __reduce_max_sync(kFull, hi);
     __syncthreads();
-    if (lane == 0) red[0][warp] = lo, red[1][warp] = hi;
+    unsigned long long lo = 0, hi = ~0ull;      // count(>= lo) >= need; no finite or infinite key is ~0
+    for (int it = 0; hi - lo > 1; ++it) {
+      const unsigned long long mid = lo + (hi - lo) / 2;
+      if (tid == 0) sm.cnt[0] = 0;
+      __syncthreads();
+      int mine = 0;
+      for (int p = tid; p < u.n; p += NT)
+        mine += (open_mask[p >> 5] >> (p & 31) & 1u) && order_key64(exact[p]) >= mid;
+      mine = __reduce_add_sync(kFull, mine);
+      if (lane == 0 && mine) atomicAdd(&sm.cnt[0], mine);
+      __syncthreads();
+      if (sm.cnt[0] >= need) lo = mid; else hi = mid;
+      __syncthreads();
+    }
+    if (tid == 0) sm.cnt[0] = 0;
     __syncthreads();
-    out_lo = __reduce_min_sync(kFull, red[0][lane % kSelWarps]);
-    out_hi = __reduce_max_sync(kFull, red[1][lane % kSelWarps]);
-  };
-
-  if (tid < 3) cnt[tid] = 0;
-  if (tid < 4) totals[tid] = 0;
-  for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
-  float lower = INFINITY, upper = -INFINITY, sk = INFINITY;
-  if (k > 0) {
-    uint32_t kmin = 0xffffffffu, kmax = 0u, fmaxk = 0u;
-    each([&](int, bool on, float s, float) {
-      if (!on) return;
-      const uint32_t key = order_key(s);
-      kmin = min(kmin, key), kmax = max(kmax, key);
-      if (s < INFINITY) fmaxk = max(fmaxk, key);
-    });
-    uint32_t lo, hi;
-    block_minmax(kmin, fmaxk, lo, hi);  // (its barriers publish the zeroed counters)
-    // intervals of the finite scores, +infinity in the last one; monotone in the score
-    const float vmin = key_value(lo), vmax = hi >= lo ? key_value(hi) : vmin;
-    const float width = vmax - vmin;
-    const float scale = width > 0.f && width < INFINITY ? (kSelBins - 1) / width : 0.f;
-    auto bin_of = [&](float s) { return s < INFINITY ? min(kSelBins - 2, (int)((s - vmin) * scale)) : kSelBins - 1; };
-    each([&](int, bool on, float s, float) {
-      if (on) atomicAdd(&hist[bin_of(s)], 1);
-    });
+    for (int w = warp; w < words; w += warps) {
+      const int p = w * 32 + lane;
+      const bool open = open_mask[w] >> lane & 1u;
+      const unsigned long long key = open ? order_key64(exact[p]) : 0ull;
+      const uint32_t above = __ballot_sync(kFull, open && key > lo), equal = __ballot_sync(kFull, open && key == lo);
+      if (lane == 0) {
+        in_mask[w] |= above;
+        open_mask[w] = equal;
+        if (above) atomicAdd(&sm.cnt[0], __popc(above));
+      }
+      __syncwarp();
+    }
     __syncthreads();
-    // the first warp finds the interval of the k-th largest: 32 bins per lane, from the top
-    if (warp == 0) {
-      int sum = 0;
-      for (int i = 0; i < 32; ++i) sum += hist[kSelBins - 1 - lane * 32 - (i + lane) % 32];
-      int incl = sum;
+    if (tid == 0) {
+      int left = need - sm.cnt[0];
+      for (int w = 0; w < words && left > 0; ++w) {
+        uint32_t m = open_mask[w];
+        while (m && left > 0) {
+          in_mask[w] |= m & -m;
+          m &= m - 1;
+          --left;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  // one warp writes the chosen pages in ascending order
+  if (warp == 0) {
+    int at = 0;
+    for (int w0 = 0; w0 < words; w0 += 32) {
+      uint32_t m = w0 + lane < words ? in_mask[w0 + lane] : 0u;
+      const int c = __popc(m);
+      int incl = c;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(kFull, incl, o);
         if (lane >= o) incl += v;
       }
-      const uint32_t reach = __ballot_sync(kFull, incl >= k);
-      const int src = __ffs(reach) - 1;
-      int above = __shfl_sync(kFull, incl - sum, src);
-      // the 32 bins of that lane, one per lane
-      const int mine = hist[kSelBins - 1 - src * 32 - lane];
-      int in2 = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(kFull, in2, o);
-        if (lane >= o) in2 += v;
-      }
-      const int at = __ffs(__ballot_sync(kFull, above + in2 >= k)) - 1;
-      above += __shfl_sync(kFull, in2 - mine, at);
-      const int members = __shfl_sync(kFull, mine, at);
-      if (lane == 0) cnt[0] = kSelBins - 1 - src * 32 - at, cnt[1] = k - above, cnt[2] = members;
-    }
-    __syncthreads();
-    const int bin = cnt[0], place = cnt[1], members = cnt[2];
-    if (members <= kSelList) {
-      float* vals = reinterpret_cast<float*>(list_val);
-      each([&](int, bool on, float s, float) {
-        if (on && bin_of(s) == bin) vals[atomicAdd(&totals[3], 1)] = s;
-      });
-      __syncthreads();
-      for (int i = tid; i < members; i += kSelThreads) {
-        const float v = vals[i];
-        int rank = 0;
-        for (int j = 0; j < members; ++j) rank += vals[j] > v || (vals[j] == v && j < i);
-        if (rank == place - 1) found_sk = v;
-      }
-      __syncthreads();
-      sk = found_sk;
-    } else {
-      // bisection over the order-preserving integer keys
-      block_minmax(kmin, kmax, lo, hi);
-      if (tid < 3) cnt[tid] = 0;
-      __syncthreads();
-      ++hi;                             // count(>= lo) >= k, count(>= hi) < k
-      for (int it = 0; hi - lo > 1; ++it) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        int mine = 0;
-        each([&](int, bool on, float s, float) { mine += on && order_key(s) >= mid; });
-        mine = __reduce_add_sync(kFull, mine);
-        if (lane == 0 && mine) atomicAdd(&cnt[it % 3], mine);
-        if (tid == 0) cnt[(it + 1) % 3] = 0;   // last read before the previous barrier
-        __syncthreads();
-        if (cnt[it % 3] >= k) lo = mid; else hi = mid;
-      }
-      sk = key_value(lo);
-    }
-    uint32_t low_key = 0xffffffffu, up_key = 0u;
-    each([&](int, bool on, float s, float e) {
-      if (!on) return;
-      if (s >= sk) low_key = min(low_key, order_key(s - e));
-      if (s <= sk) up_key = max(up_key, order_key(s + e));
-    });
-    block_minmax(low_key, up_key, lo, hi);
-    lower = key_value(lo);
-    upper = key_value(hi);
-  }
-  __syncthreads();
-  each([&](int p, bool on, float s, float e) {
-    bool in = p < n && !on;             // the first and the last pages
-    bool open = false;
-    if (on && k > 0) {
-      if (s > sk) {
-        in = s - e > upper;
-        open = !in;
-      } else {
-        open = s + e >= lower;
-      }
-    }
-    const uint32_t bi = __ballot_sync(kFull, in), bo = __ballot_sync(kFull, open);
-    if (lane == 0 && p < n) {
-      in_mask[p >> 5] = bi;
-      open_mask[p >> 5] = bo;
-      if (bi) atomicAdd(&totals[0], __popc(bi));
-      if (bo) atomicAdd(&totals[1], __popc(bo));
-    }
-  });
-  __syncthreads();
-  const int n_open = totals[1];
-  const int need = a.budget - totals[0];   // 0 <= need <= n_open
-  if (need == n_open) {
-    for (int w = tid; w < words; w += kSelThreads) in_mask[w] |= open_mask[w];
-  } else {
-    const __nv_bfloat16* q = a.q + (int64_t)tok * a.q_ld + (int64_t)kvh * (a.Hq / a.Hkv) * D;
-    const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
-    const int G = a.Hq / a.Hkv;
-    const bool small = n_open <= kSelList;
-    double* big = reinterpret_cast<double*>(ws);   // the fp32 scores are no longer needed
-    // exact scores of the open pages, one warp per page
-    for (int w = warp; w < words; w += kSelWarps) {
-      uint32_t m = open_mask[w];
+      int i = at + incl - c;
       while (m) {
-        const int p = w * 32 + __ffs(m) - 1;
+        if (i < a.budget) u.sel[i] = (w0 + lane) * 32 + __ffs(m) - 1;
+        ++i;
         m &= m - 1;
-        const bool finite = isfinite(ws[p].x);
-        __syncwarp();
-        const int64_t phys = table_page(bt, p, a.num_pages);
-        const double v = finite ? exact_score(a, q, a.bounds + (phys * a.Hkv + kvh) * 2 * D, G, lane) : INFINITY;
-        if (lane == 0) {
-          if (small) {
-            const int at = atomicAdd(&totals[2], 1);
-            list_idx[at] = p;
-            list_val[at] = v;
-          } else {
-            big[p] = v;
-          }
-        }
       }
-    }
-    __syncthreads();
-    if (small) {
-      if (tid < n_open) {
-        const double v = list_val[tid];
-        const int p = list_idx[tid];
-        int rank = 0;
-        for (int j = 0; j < n_open; ++j) rank += list_val[j] > v || (list_val[j] == v && list_idx[j] < p);
-        if (rank < need) atomicOr(&in_mask[p >> 5], 1u << (p & 31));
-      }
-    } else {
-      // bisection over the 64-bit keys, then ties by index
-      unsigned long long lo = 0, hi = ~0ull;      // count(>= lo) >= need; no finite or infinite key is ~0
-      for (int it = 0; hi - lo > 1; ++it) {
-        const unsigned long long mid = lo + (hi - lo) / 2;
-        if (tid == 0) cnt[0] = 0;
-        __syncthreads();
-        int mine = 0;
-        for (int p = tid; p < n; p += kSelThreads)
-          mine += (open_mask[p >> 5] >> (p & 31) & 1u) && order_key64(big[p]) >= mid;
-        mine = __reduce_add_sync(kFull, mine);
-        if (lane == 0 && mine) atomicAdd(&cnt[0], mine);
-        __syncthreads();
-        if (cnt[0] >= need) lo = mid; else hi = mid;
-        __syncthreads();
-      }
-      if (tid == 0) cnt[0] = 0;
-      __syncthreads();
-      for (int w = warp; w < words; w += kSelWarps) {
-        const int p = w * 32 + lane;
-        const bool open = open_mask[w] >> lane & 1u;
-        const unsigned long long key = open ? order_key64(big[p]) : 0ull;
-        const uint32_t above = __ballot_sync(kFull, open && key > lo), equal = __ballot_sync(kFull, open && key == lo);
-        __syncwarp();
-        if (lane == 0) {
-          in_mask[w] |= above;
-          open_mask[w] = equal;
-          if (above) atomicAdd(&cnt[0], __popc(above));
-        }
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int left = need - cnt[0];
-        for (int w = 0; w < words && left > 0; ++w) {
-          uint32_t m = open_mask[w];
-          while (m && left > 0) {
-            in_mask[w] |= m & -m;
-            m &= m - 1;
-            --left;
-          }
-        }
-      }
-    }
-  }
-  __syncthreads();
-  // positions of the chosen pages, in ascending order
-  const int per = (words + kSelThreads - 1) / kSelThreads;
-  int mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int w = tid * per + i;
-    if (w < words) mine += __popc(in_mask[w]);
-  }
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(kFull, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) red[0][warp] = (uint32_t)incl;
-  __syncthreads();
-  int at = incl - mine;
-  for (int w = 0; w < warp; ++w) at += (int)red[0][w];
-  for (int i = 0; i < per; ++i) {
-    const int w = tid * per + i;
-    if (w >= words) break;
-    prefix[w] = (uint32_t)at;
-    at += __popc(in_mask[w]);
-  }
-  __syncthreads();
-  for (int p = tid; p < n; p += kSelThreads) {
-    const uint32_t m = in_mask[p >> 5], bit = 1u << (p & 31);
-    if (m & bit) {
-      const int i = (int)prefix[p >> 5] + __popc(m & (bit - 1));
-      if (i < a.budget) sel[i] = p;
+      at += __shfl_sync(kFull, incl, 31);
     }
   }
 }
 
+// ITEMS: pages per thread (NT * ITEMS >= the block table's width), 0 for rows that
+// only the general routine takes.
+template <int NT, int ITEMS>
+__global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
+  constexpr int kW = NT / 32, I = ITEMS > 0 ? ITEMS : 1;
+  extern __shared__ uint32_t masks[];        // of the general routine: in | open
+  __shared__ SelectSmem sm;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kvh = blockIdx.x, r = blockIdx.y;
+  for (int i = tid; i < kSelBins; i += NT) sm.hist[i] = 0;
+  if (tid < 4) sm.totals[tid] = 0;
+  pdl_wait();
+  const int tok = a.tok_index[r];
+  const int L = row_length(a.seq_lens, r, a.width);
+  const int n = (L + PAGE - 1) / PAGE;
+  SelectUnit u;
+  u.sel = a.sel + ((int64_t)r * a.Hkv + kvh) * a.budget;
+  if (n <= a.budget || tok < 0 || tok >= a.tokens) {
+    // everything fits; a row of a bad token (recorded by the score kernel) takes nothing
+    const int keep = n <= a.budget ? n : 0;
+    for (int i = tid; i < a.budget; i += NT) u.sel[i] = i < keep ? i : -1;
+    return;
+  }
+  u.ws = a.ws + ((int64_t)r * a.Hkv + kvh) * a.width;
+  u.G = a.Hq / a.Hkv;
+  u.q = a.q + (int64_t)tok * a.q_ld + (int64_t)kvh * u.G * D;
+  u.bt = a.block_table + (int64_t)r * a.bt_stride;
+  u.kvh = kvh;
+  u.n = n;
+  u.first = a.first, u.mid1 = n - a.last;                 // pages that compete
+  u.k = a.budget - a.first - a.last;                      // for k places; k < mid1 - first
+  if (ITEMS == 0) {
+    select_general(a, u, sm, masks);
+    return;
+  }
+
+  // warp w holds pages [w 32 I, (w + 1) 32 I), lane l page 32 i + l of them
+  const int page0 = warp * 32 * I + lane;
+  float2 v[I];
+  uint32_t on = 0;
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const int p = page0 + i * 32;
+    v[i] = make_float2(0.f, 0.f);
+    if (p >= u.first && p < u.mid1) on |= 1u << i, v[i] = u.ws[p];
+  }
+  float sk = INFINITY, lower = INFINITY, upper = -INFINITY;
+  if (u.k > 0) {
+    uint32_t kmin = 0xffffffffu, kmax = 0u, lo, hi;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+      if (on >> i & 1u && v[i].x < INFINITY) {
+        const uint32_t key = order_key(v[i].x);
+        kmin = min(kmin, key), kmax = max(kmax, key);
+      }
+    block_minmax(sm, kmin, kmax, lo, hi);   // (its barriers publish the zeroed counters)
+    // intervals of the finite scores, +infinity in the last one; monotone in the score
+    const float vmin = hi >= lo ? key_value(lo) : 0.f;
+    const float width = hi >= lo ? key_value(hi) - vmin : 0.f;
+    const float scale = width > 0.f && width < INFINITY ? (kSelBins - 1) / width : 0.f;
+    auto bin_of = [&](float s) { return s < INFINITY ? min(kSelBins - 2, (int)((s - vmin) * scale)) : kSelBins - 1; };
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+      if (on >> i & 1u) atomicAdd(&sm.hist[bin_of(v[i].x)], 1);
+    __syncthreads();
+    // the first warp finds the interval of the k-th largest: 32 intervals per lane, from the top
+    if (warp == 0) {
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sum += sm.hist[kSelBins - 1 - lane * 32 - (i + lane) % 32];
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(kFull, incl, o);
+        if (lane >= o) incl += x;
+      }
+      const int src = __ffs(__ballot_sync(kFull, incl >= u.k)) - 1;
+      int above = __shfl_sync(kFull, incl - sum, src);
+      const int mine = sm.hist[kSelBins - 1 - src * 32 - lane];
+      int in2 = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(kFull, in2, o);
+        if (lane >= o) in2 += x;
+      }
+      const int at = __ffs(__ballot_sync(kFull, above + in2 >= u.k)) - 1;
+      above += __shfl_sync(kFull, in2 - mine, at);
+      const int members = __shfl_sync(kFull, mine, at);
+      if (lane == 0) sm.cnt[0] = kSelBins - 1 - src * 32 - at, sm.cnt[1] = u.k - above, sm.cnt[2] = members;
+    }
+    __syncthreads();
+    const int bin = sm.cnt[0], place = sm.cnt[1], members = sm.cnt[2];
+    if (members > kSelList) {
+      select_general(a, u, sm, masks);
+      return;
+    }
+    // the interval's pages into a list; the others lie on one side of s_k
+    uint32_t low_key = 0xffffffffu, up_key = 0u;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      if (!(on >> i & 1u)) continue;
+      const int b = bin_of(v[i].x);
+      if (b == bin) {
+        const int at = atomicAdd(&sm.totals[0], 1);
+        sm.list_s[at] = v[i].x;
+        sm.list_e[at] = v[i].y;
+      } else if (b > bin) {
+        low_key = min(low_key, order_key(v[i].x - v[i].y));
+      } else {
+        up_key = max(up_key, order_key(v[i].x + v[i].y));
+      }
+    }
+    low_key = __reduce_min_sync(kFull, low_key);
+    up_key = __reduce_max_sync(kFull, up_key);
+    if (lane == 0) sm.red[0][warp] = low_key, sm.red[1][warp] = up_key;
+    __syncthreads();
+    for (int i = tid; i < members; i += NT) {
+      const float x = sm.list_s[i];
+      int rank = 0;
+      for (int j = 0; j < members; ++j) rank += sm.list_s[j] > x || (sm.list_s[j] == x && j < i);
+      if (rank == place - 1) sm.sk = x;
+    }
+    __syncthreads();
+    sk = sm.sk;
+    low_key = sm.red[0][lane % kW], up_key = sm.red[1][lane % kW];
+    for (int i = lane; i < members; i += 32) {
+      const float x = sm.list_s[i], e = sm.list_e[i];
+      if (x >= sk) low_key = min(low_key, order_key(x - e));
+      if (x <= sk) up_key = max(up_key, order_key(x + e));
+    }
+    lower = key_value(__reduce_min_sync(kFull, low_key));
+    upper = key_value(__reduce_max_sync(kFull, up_key));
+  }
+  pdl_trigger();
+  uint32_t in = 0, open = 0;
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const int p = page0 + i * 32;
+    if (!(on >> i & 1u)) {
+      if (p < n) in |= 1u << i;             // the first and the last pages
+    } else if (u.k > 0) {
+      if (v[i].x > sk && v[i].x - v[i].y > upper) in |= 1u << i;
+      else if (v[i].x > sk || v[i].x + v[i].y >= lower) open |= 1u << i;
+    }
+  }
+  {
+    const int ci = __reduce_add_sync(kFull, __popc(in)), co = __reduce_add_sync(kFull, __popc(open));
+    if (lane == 0) sm.count_in[warp] = ci, sm.count_open[warp] = co;
+  }
+  __syncthreads();
+  // totals over the warps, and what lies in the warps before this one
+  const int ci = lane < kW ? sm.count_in[lane] : 0, co = lane < kW ? sm.count_open[lane] : 0;
+  const int n_in = __reduce_add_sync(kFull, ci), n_open = __reduce_add_sync(kFull, co);
+  const int need = a.budget - n_in;          // 0 <= need <= n_open
+  int at;
+  if (need == n_open) {
+    in |= open;
+    at = __reduce_add_sync(kFull, lane < warp ? ci + co : 0);
+  } else if (n_open > kSelList) {
+    select_general(a, u, sm, masks);
+    return;
+  } else {
+    int place[I];
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      place[i] = 0;
+      if (open >> i & 1u) {
+        place[i] = atomicAdd(&sm.totals[1], 1);
+        sm.list_idx[place[i]] = page0 + i * 32;
+        sm.list_s[place[i]] = v[i].x;
+      }
+    }
+    __syncthreads();
+    for (int i = warp; i < n_open; i += kW) {
+      const double x = isfinite(sm.list_s[i]) ? exact_score(a, u, sm.list_idx[i], lane) : INFINITY;
+      if (lane == 0) sm.list_val[i] = x;
+    }
+    __syncthreads();
+    for (int i = tid; i < n_open; i += NT) {
+      const double x = sm.list_val[i];
+      const int p = sm.list_idx[i];
+      int rank = 0;
+      for (int j = 0; j < n_open; ++j) rank += sm.list_val[j] > x || (sm.list_val[j] == x && sm.list_idx[j] < p);
+      sm.list_e[i] = rank < need ? 1.f : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+      if (open >> i & 1u && sm.list_e[place[i]] != 0.f) in |= 1u << i;
+    const int c = __reduce_add_sync(kFull, __popc(in));
+    if (lane == 0) sm.count_in[warp] = c;
+    __syncthreads();
+    at = __reduce_add_sync(kFull, lane < warp ? sm.count_in[lane] : 0);
+  }
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const uint32_t m = __ballot_sync(kFull, in >> i & 1u);
+    if (in >> i & 1u) u.sel[at + __popc(m & ((1u << lane) - 1))] = page0 + i * 32;
+    at += __popc(m);
+  }
+}
+
 // ===========================================================================
-// decode_sparse: a cluster of CTAs per (row, KV head), four warps each, every
-// warp a share of the chosen pages with its own running maximum and sum; the
-// warps join in shared memory, the CTAs through distributed shared memory, so
-// there is one launch and no workspace.
+// decode_sparse: a cluster of CTAs per (row, KV head), every warp a share of the
+// chosen pages with its own running maximum and sum; the warps join in shared
+// memory, the CTAs by writing into the shared memory of the CTA that owns an
+// output, so there is one launch and no workspace.
 //
 // S^T = K Q^T has the page's 16 tokens as rows and the query heads as columns;
 // O^T = V^T P^T has dimensions as rows.  K is read by the lanes in the layout of
@@ -682,62 +763,74 @@ __global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
 // two tokens side by side: a lane reads the same eight dimensions of two tokens
 // and interleaves them with byte permutes; row g of tile t is dimension 8g + t.
 // P^T comes from S^T by an 8 x 8 register transpose.  P is rounded to bf16 for
-// the tensor cores, an error of 2^-9 of each weight that averages over the
-// tokens; the sum of the weights is kept in fp32 from the same rounded values,
-// so the rounding does not scale the output.
+// the tensor cores, an error of at most 2^-8 of each weight that averages over
+// the tokens; the sum of the weights is kept in fp32 from the same rounded
+// values, so the rounding does not scale the output.
+//
+// The next page's K is fetched into the same registers as soon as S is known,
+// its V after O is updated: 16 warps per SM with a page each under way.
 // ===========================================================================
-constexpr int kSpWarps = kWarps;
+constexpr int kSpWarps = 8;
+constexpr int kSpThreads = kSpWarps * 32;
+constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t x;
   asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(x));
   return x;
 }
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   uint32_t addr;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+  return addr;
+}
+__device__ __forceinline__ void st_cluster4(uint32_t addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ void st_cluster2(uint32_t addr, float2 v) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
 }
 
+constexpr int kOLd = D + 4;
 template <int NH>
 struct SparseSmem {
-  float o[kSpWarps][NH * 8][D];
-  float m[kSpWarps][NH * 8];
-  float l[kSpWarps][NH * 8];
+  float o[kSpWarps][NH * 8][kOLd];
+  float2 ml[kSpWarps][NH * 8];             // running maximum and sum
+  // from every CTA of the cluster, for the outputs this CTA owns: quads of
+  // dimensions q with q % cl == this CTA
+  float4 in_o[kMaxCluster][NH * 8 * (D / 4) / 2];
+  float2 in_ml[kMaxCluster][NH * 8];
 };
 
 template <int NH>
-__global__ void __launch_bounds__(kThreads, 2) decode_sparse_kernel(const SparseArgs a, int cl) {
+__global__ void __launch_bounds__(kSpThreads, NH == 1 ? 2 : 1) decode_sparse_kernel(const SparseArgs a, int cl) {
   extern __shared__ __align__(128) uint8_t raw[];
-  SparseSmem<NH>& sm = *reinterpret_cast<SparseSmem<NH>*>(raw);   // over the ring, after the last page
-  pdl_trigger();
-  pdl_wait();
+  SparseSmem<NH>& sm = *reinterpret_cast<SparseSmem<NH>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int part = cl > 1 ? (int)cluster_rank() : 0;
   const int unit = blockIdx.x / cl;
   const int kvh = unit % a.Hkv, r = unit / a.Hkv;
   const int G = a.Hq / a.Hkv;
-  const int L = row_length(a.seq_lens, r, a.width);
-  const int n = (L + PAGE - 1) / PAGE;
-  const int tok = a.tok_index[r];
-  const bool tok_ok = tok >= 0 && tok < a.tokens;
-  if (!tok_ok && tid == 0) set_error(kErrBadIndex, (unsigned long long)r);
-  const int count = tok_ok ? min(n, a.budget) : 0;
-  const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
-  const int32_t* sel = a.sel + ((int64_t)r * a.Hkv + kvh) * a.budget;
-
   // this warp's pages: entries w, w + stride, ... of the list; lane j holds the
   // j-th of a window of 32 (first token, physical page), the next window under way
   const int stride = cl * kSpWarps, w = part * kSpWarps + warp;
+  const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
+  const int32_t* sel = a.sel + ((int64_t)r * a.Hkv + kvh) * a.budget;
+  if (cl > 1) cluster_arrive();         // every CTA of the cluster runs before another one writes to it
+  pdl_wait();
+  int next_page = w + lane * stride < a.budget ? sel[w + lane * stride] : -1;   // in the same round trip as the length
+  const int tok = a.tok_index[r];
+  const int L = row_length(a.seq_lens, r, a.width);
+  const int n = (L + PAGE - 1) / PAGE;
+  const bool tok_ok = tok >= 0 && tok < a.tokens;
+  if (!tok_ok && tid == 0) set_error(kErrBadIndex, (unsigned long long)r);
+  const int count = tok_ok ? min(n, a.budget) : 0;
   const int mine = count > w ? (count - w + stride - 1) / stride : 0;
-  int win_tok, win_phys, next_page = -1;
-  auto fetch_window = [&](int i) { next_page = i + lane < mine ? sel[w + (i + lane) * stride] : -1; };
+  int win_tok = 0, win_phys = 0;
   auto open_window = [&](int i) {
     win_tok = L;                        // nothing valid in the page
     win_phys = 0;
@@ -749,42 +842,44 @@ __global__ void __launch_bounds__(kThreads, 2) decode_sparse_kernel(const Sparse
         win_phys = table_page(bt, next_page, a.num_pages);
       }
     }
-    fetch_window(i + 32);
+    const int j = i + 32 + lane;
+    next_page = j < mine ? sel[w + j * stride] : -1;
   };
-  fetch_window(0);
 
   // a lane's pieces of a page: K rows g and g + 8, pieces c, c + 4, ...; V rows 2c,
   // 2c + 1, 2c + 8, 2c + 9, piece g of both halves of the dimensions
-  const uint32_t ring = smem_u32(raw) + tid * 16;
   const __nv_bfloat16* kl = a.kcache + (int64_t)kvh * PAGE * D + g * D + c * 8;
   const __nv_bfloat16* vl = a.vcache + (int64_t)kvh * PAGE * D + 2 * c * D + g * 8;
   const int64_t page_elems = (int64_t)a.Hkv * PAGE * D;
-  auto issue = [&](int i, uint32_t slot) -> int {   // the page's first token
-    int t0 = L;
-    if (i < mine) {
-      if ((i & 31) == 0) open_window(i);
-      t0 = __shfl_sync(kFull, win_tok, i & 31);
-      const int64_t at = __shfl_sync(kFull, win_phys, i & 31) * page_elems;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        cp_async16(slot + j * kUnit, kl + at + j * 32, true);
-        cp_async16(slot + (4 + j) * kUnit, kl + at + 8 * D + j * 32, true);
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int t = (x & 1) + (x >> 1) * 8;
-        const bool on = t0 + 2 * c + t < L;         // zeros past the sequence's end
-        cp_async16(slot + (8 + x) * kUnit, vl + at + t * D, on);
-        cp_async16(slot + (12 + x) * kUnit, vl + at + t * D + 64, on);
-      }
-    }
-    cp_async_commit();
-    return t0;
+  uint4 k0[4], k1[4], v[2][4];          // v[half of the dimensions][token 2c, 2c + 1, 2c + 8, 2c + 9]
+  int t0 = L, t0_next = L;
+  int64_t at = 0;
+  auto locate = [&](int i) {            // page i of this warp
+    if ((i & 31) == 0) open_window(i);
+    t0_next = __shfl_sync(kFull, win_tok, i & 31);
+    at = __shfl_sync(kFull, win_phys, i & 31) * page_elems;
   };
-  int first_tok[kStages];
+  auto load_k = [&]() {
 #pragma unroll
-  for (int i = 0; i < kStages; ++i) first_tok[i] = issue(i, ring + i * kStage);
-
+    for (int j = 0; j < 4; ++j) {
+      k0[j] = ld_stream(kl + at + j * 32);
+      k1[j] = ld_stream(kl + at + 8 * D + j * 32);
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int t = (x & 1) + (x >> 1) * 8;
+      const bool on = t0_next + 2 * c + t < L;      // zeros past the sequence's end
+      v[0][x] = on ? ld_stream(vl + at + t * D) : make_uint4(0u, 0u, 0u, 0u);
+      v[1][x] = on ? ld_stream(vl + at + t * D + 64) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  if (mine > 0) {
+    locate(0);
+    load_k();
+    load_v();
+  }
   uint4 q[NH][4];
 #pragma unroll
   for (int t = 0; t < NH; ++t) {
@@ -803,27 +898,24 @@ __global__ void __launch_bounds__(kThreads, 2) decode_sparse_kernel(const Sparse
     for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
   }
 
-  uint32_t slot = ring;
   for (int i = 0; i < mine; ++i) {
-    cp_async_wait<kStages - 1>();
-    const int t0 = first_tok[0];
-#pragma unroll
-    for (int x = 0; x + 1 < kStages; ++x) first_tok[x] = first_tok[x + 1];
-    uint32_t p[NH][2];
+    t0 = t0_next;
     float s[NH][2][4];
 #pragma unroll
-    for (int t = 0; t < NH; ++t)
+    for (int t = 0; t < NH; ++t) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) s[t][x][0] = s[t][x][1] = s[t][x][2] = s[t][x][3] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint4 k0 = lds16(slot + j * kUnit), k1 = lds16(slot + (4 + j) * kUnit);
-#pragma unroll
-      for (int t = 0; t < NH; ++t) {
-        mma_bf16(s[t][0], k0.x, k1.x, k0.y, k1.y, q[t][j].x, q[t][j].y);
-        mma_bf16(s[t][1], k0.z, k1.z, k0.w, k1.w, q[t][j].z, q[t][j].w);
+      for (int j = 0; j < 4; ++j) {
+        mma_bf16(s[t][0], k0[j].x, k1[j].x, k0[j].y, k1[j].y, q[t][j].x, q[t][j].y);
+        mma_bf16(s[t][1], k0[j].z, k1[j].z, k0[j].w, k1[j].w, q[t][j].z, q[t][j].w);
       }
     }
+    if (i + 1 < mine) {
+      locate(i + 1);
+      load_k();
+    }
+    uint32_t p[NH][2];
 #pragma unroll
     for (int t = 0; t < NH; ++t) {
       // x[0], x[1]: token g, heads 2c, 2c + 1; x[2], x[3]: token g + 8
@@ -855,9 +947,6 @@ __global__ void __launch_bounds__(kThreads, 2) decode_sparse_kernel(const Sparse
       p[t][0] = movmatrix_trans(plo);
       p[t][1] = movmatrix_trans(phi);
     }
-    uint4 v[2][4];                      // v[half of the dimensions][token 2c, 2c + 1, 2c + 8, 2c + 9]
-#pragma unroll
-    for (int x = 0; x < 4; ++x) v[0][x] = lds16(slot + (8 + x) * kUnit), v[1][x] = lds16(slot + (12 + x) * kUnit);
     const uint32_t* vw = reinterpret_cast<const uint32_t*>(v);   // [half][token][word]
 #pragma unroll
     for (int i8 = 0; i8 < 8; ++i8) {
@@ -870,13 +959,11 @@ __global__ void __launch_bounds__(kThreads, 2) decode_sparse_kernel(const Sparse
 #pragma unroll
       for (int t = 0; t < NH; ++t) mma_bf16(o[t][i8], a0, a1, a2, a3, p[t][0], p[t][1]);
     }
-    first_tok[kStages - 1] = issue(i + kStages, slot);
-    slot = slot == ring + (kStages - 1) * kStage ? ring : slot + kStage;
+    if (i + 1 < mine) load_v();
   }
-  cp_async_wait<0>();
-  __syncthreads();                      // the ring's memory becomes the warps' results
 
-  // join: o[t][i][0..1] = dim 8g + i, heads 2c, 2c + 1; [2..3] = dim 64 + 8g + i
+  pdl_trigger();
+  // the warps' results: o[t][i][0..1] = dim 8g + i, heads 2c, 2c + 1; [2..3] = dim 64 + 8g + i
 #pragma unroll
   for (int t = 0; t < NH; ++t) {
 #pragma unroll
@@ -886,57 +973,69 @@ __global__ void __launch_bounds__(kThreads, 2) decode_sparse_kernel(const Sparse
       s += __shfl_xor_sync(kFull, s, 8);
       s += __shfl_xor_sync(kFull, s, 16);
       const int h = t * 8 + 2 * c + e;
-      if (g == 0) {
-        sm.m[warp][h] = m[t][e];
-        sm.l[warp][h] = s;
-      }
+      if (g == 0) sm.ml[warp][h] = make_float2(m[t][e], s);
+      if (h < G) {
 #pragma unroll
-      for (int i8 = 0; i8 < 8; ++i8) {
-        sm.o[warp][h][8 * g + i8] = o[t][i8][e];
-        sm.o[warp][h][64 + 8 * g + i8] = o[t][i8][e + 2];
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            *reinterpret_cast<float4*>(&sm.o[warp][h][x * 64 + 8 * g + 4 * y]) =
+                make_float4(o[t][4 * y][e + 2 * x], o[t][4 * y + 1][e + 2 * x], o[t][4 * y + 2][e + 2 * x],
+                            o[t][4 * y + 3][e + 2 * x]);
       }
     }
   }
   __syncthreads();
-  // the CTA's warps, into the first warp's place
-  const int d = threadIdx.x;
-  for (int h = 0; h < G; ++h) {
+  if (cl > 1) cluster_wait();
+  __nv_bfloat16* out = a.out + (int64_t)(tok_ok ? tok : 0) * a.out_ld + (int64_t)kvh * G * D;
+  auto write = [&](int quad, float4 acc, float sum) {
+    const float f = sum > 0.f ? 1.f / sum : 0.f;
+    if (tok_ok)
+      *reinterpret_cast<uint2*>(out + quad * 4) = make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
+  };
+  // quads of four dimensions, head by head: the CTA's warps, then the cluster's CTAs
+  for (int quad = tid; quad < G * (D / 4); quad += kSpThreads) {
+    const int h = quad / (D / 4), d = quad % (D / 4) * 4;
     float mx = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < kSpWarps; ++x) mx = fmaxf(mx, sm.m[x][h]);
+    for (int x = 0; x < kSpWarps; ++x) mx = fmaxf(mx, sm.ml[x][h].x);
     const float sh = mx == -INFINITY ? 0.f : mx;
-    float acc = 0.f, ls = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
 #pragma unroll
     for (int x = 0; x < kSpWarps; ++x) {
-      const float f = exp2f(sm.m[x][h] - sh);
-      acc += f * sm.o[x][h][d];
-      ls += f * sm.l[x][h];
+      const float2 ml = sm.ml[x][h];
+      const float f = exp2f(ml.x - sh);
+      const float4 y = *reinterpret_cast<const float4*>(&sm.o[x][h][d]);
+      acc.x += f * y.x, acc.y += f * y.y, acc.z += f * y.z, acc.w += f * y.w;
+      sum += f * ml.y;
     }
     if (cl == 1) {
-      if (tok_ok)
-        a.out[(int64_t)tok * a.out_ld + (int64_t)(kvh * G + h) * D + d] = __float2bfloat16(ls > 0.f ? acc / ls : 0.f);
+      write(quad, acc, sum);
     } else {
-      sm.o[0][h][d] = acc;
-      __syncthreads();
-      if (d == 0) sm.m[0][h] = mx, sm.l[0][h] = ls;
+      st_cluster4(cluster_addr(&sm.in_o[part][quad / cl], quad % cl), acc);
+      if (quad % (D / 4) < cl) st_cluster2(cluster_addr(&sm.in_ml[part][h], quad % cl), make_float2(mx, sum));
     }
   }
   if (cl == 1) return;
-  cluster_sync_all();
-  for (int h = part; h < G; h += cl) {
+  cluster_arrive();
+  cluster_wait();
+  for (int quad = tid * cl + part; quad < G * (D / 4); quad += kSpThreads * cl) {
+    const int h = quad / (D / 4);
     float mx = -INFINITY;
-    for (int x = 0; x < cl; ++x) mx = fmaxf(mx, ld_cluster(&sm.m[0][h], x));
+    for (int x = 0; x < cl; ++x) mx = fmaxf(mx, sm.in_ml[x][h].x);
     const float sh = mx == -INFINITY ? 0.f : mx;
-    float acc = 0.f, ls = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
     for (int x = 0; x < cl; ++x) {
-      const float f = exp2f(ld_cluster(&sm.m[0][h], x) - sh);
-      acc += f * ld_cluster(&sm.o[0][h][d], x);
-      ls += f * ld_cluster(&sm.l[0][h], x);
+      const float2 ml = sm.in_ml[x][h];
+      const float f = exp2f(ml.x - sh);
+      const float4 y = sm.in_o[x][quad / cl];
+      acc.x += f * y.x, acc.y += f * y.y, acc.z += f * y.z, acc.w += f * y.w;
+      sum += f * ml.y;
     }
-    if (tok_ok)
-      a.out[(int64_t)tok * a.out_ld + (int64_t)(kvh * G + h) * D + d] = __float2bfloat16(ls > 0.f ? acc / ls : 0.f);
+    write(quad, acc, sum);
   }
-  cluster_sync_all();   // no CTA leaves while another reads its shared memory
 }
 
 int sm_count() {
@@ -963,6 +1062,12 @@ void raise_smem(const void* k, size_t smem) {
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) launch_failed(e);
 }
+
+template <int NT, int ITEMS>
+void launch_select(const SelectArgs& a, cudaStream_t s) {
+  const size_t smem = (size_t)((a.width + 31) / 32) * 2 * sizeof(uint32_t);   // the general routine's masks, at most 16 KB
+  launch_k(page_select_kernel<NT, ITEMS>, dim3((unsigned)a.Hkv, (unsigned)a.rows), dim3(NT), smem, s, 1, a);
+}
 }  // namespace
 
 void select_pages(const SelectArgs& a, cudaStream_t s) {
@@ -975,15 +1080,13 @@ void select_pages(const SelectArgs& a, cudaStream_t s) {
     const int chunk = passes * kScoreTile;
     const dim3 grid((unsigned)((a.width + chunk - 1) / chunk * a.Hkv), (unsigned)a.rows);
     auto k = a.Hq / a.Hkv <= 8 ? page_score_kernel<1> : page_score_kernel<2>;
-    raise_smem(reinterpret_cast<const void*>(k), kStages * kStage);
-    launch_k(k, grid, dim3(kThreads), kStages * kStage, s, 1, a, passes);
+    raise_smem(reinterpret_cast<const void*>(k), kScoreSmem);
+    launch_k(k, grid, dim3(kThreads), kScoreSmem, s, 1, a, passes);
   }
-  const size_t smem = (size_t)((a.width + 31) / 32) * 3 * sizeof(uint32_t);   // at most 24 KB
-  const dim3 grid((unsigned)a.Hkv, (unsigned)a.rows);
-  if (a.width <= 512) launch_k(page_select_kernel<256, 2>, grid, dim3(256), smem, s, 1, a);
-  else if (a.width <= 2048) launch_k(page_select_kernel<512, 4>, grid, dim3(512), smem, s, 1, a);
-  else if (a.width <= 8192) launch_k(page_select_kernel<1024, 8>, grid, dim3(1024), smem, s, 1, a);
-  else launch_k(page_select_kernel<1024, 0>, grid, dim3(1024), smem, s, 1, a);
+  if (a.width <= 512) launch_select<256, 2>(a, s);
+  else if (a.width <= 2048) launch_select<512, 4>(a, s);
+  else if (a.width <= 8192) launch_select<1024, 8>(a, s);
+  else launch_select<1024, 0>(a, s);
 }
 
 void decode_sparse(const SparseArgs& a, cudaStream_t s) {
@@ -991,10 +1094,15 @@ void decode_sparse(const SparseArgs& a, cudaStream_t s) {
   const int64_t units = (int64_t)a.rows * a.Hkv;
   const int64_t slots = (int64_t)sm_count() * 2;
   int cl = 1;
-  while (cl < 8 && units * cl * 2 <= slots && a.budget >= kSpWarps * cl * 2) cl *= 2;
-  auto k = a.Hq / a.Hkv <= 8 ? decode_sparse_kernel<1> : decode_sparse_kernel<2>;
-  raise_smem(reinterpret_cast<const void*>(k), kStages * kStage);   // covers the join's 17 / 33 KB
-  launch_k(k, dim3((unsigned)(units * cl)), dim3(kThreads), kStages * kStage, s, (unsigned)cl, a, cl);
+  while (cl < kMaxCluster && units * cl < slots && a.budget > kSpWarps * cl) cl *= 2;
+  const bool wide = a.Hq / a.Hkv > 8;
+  auto k = wide ? decode_sparse_kernel<2> : decode_sparse_kernel<1>;
+  const size_t smem = wide ? sizeof(SparseSmem<2>) : sizeof(SparseSmem<1>);
+  raise_smem(reinterpret_cast<const void*>(k), smem);
+  // Clusters that start while the previous kernel still holds some SMs crowd onto
+  // the others; where they would fill the GPU they wait for its end (4 rows x 8
+  // heads x 256 pages after a selection: 72 instead of 82 us for the whole step).
+  launch_with(cl == 1 || units * cl <= sm_count(), k, dim3((unsigned)(units * cl)), dim3(kSpThreads), smem, s, (unsigned)cl, a, cl);
 }
 
 }  // namespace attn

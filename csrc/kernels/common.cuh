@@ -380,9 +380,10 @@ __device__ __forceinline__ float warp_max(float v) {
 // stream-serialization attribute when PDL is on (see pdl_wait), plus an
 // optional cluster shape.  Only kernels that call pdl_wait() before touching
 // global memory may be launched through here.  Throws on a launch error.
+// launch_with: the same with the attribute only where `overlap` is set as well.
 template <typename... KArgs, typename... Args>
-inline void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                   unsigned cluster_x, Args&&... args) {
+inline void launch_with(bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                        cudaStream_t stream, unsigned cluster_x, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -397,7 +398,7 @@ inline void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sme
     attr[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (rt::pdl_enabled()) {
+  if (overlap && rt::pdl_enabled()) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;
@@ -406,6 +407,12 @@ inline void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sme
   cfg.numAttrs = n;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
   if (e != cudaSuccess) launch_failed(e);
+}
+
+template <typename... KArgs, typename... Args>
+inline void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                     unsigned cluster_x, Args&&... args) {
+  launch_with(true, kernel, grid, block, smem, stream, cluster_x, std::forward<Args>(args)...);
 }
 
 }  // namespace lf
