@@ -27,6 +27,7 @@
 #include <stdint.h>
 
 #include <stdexcept>
+#include <cstdlib>
 
 #include "attention_sparse.h"
 #include "common.cuh"
@@ -57,15 +58,6 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
                : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -87,13 +79,6 @@ __device__ __forceinline__ int table_page(const int32_t* bt, int idx, int num_pa
     return 0;
   }
   return p;
-}
-
-// Waits for copies under way after another wait ran out, up to the same limit.
-__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 <= wait_limit_ns()) {
-  }
 }
 
 // A row's KV length; a length beyond the block table is recorded and cut.
@@ -158,13 +143,16 @@ __global__ void __launch_bounds__(128) page_bounds_kernel(const BoundsArgs a) {
 }
 
 // ===========================================================================
-// Page scores.  A warp takes 16 pages at a time as the 16 rows of m16n8k16.  One
-// bulk copy per page (512 bytes: lo, then hi) brings them into the warp's own
-// ring; rows lie 576 bytes apart, so that the 16-byte pieces c, c + 4, ... which
-// lane (g, c) = (lane / 4, lane % 4) reads of pages g and g + 8 hit all banks.  A
-// piece is eight consecutive dimensions, which serve two k-steps: the order of
-// k is free as long as the queries use the same one.  Pieces 0..15 (lo) meet
-// min(q, 0) and pieces 16..31 (hi) meet max(q, 0).
+// Page scores.  A warp takes 16 pages at a time as the 16 rows of m16n8k16; lane
+// (g, c) = (lane / 4, lane % 4) loads 16-byte pieces c, c + 4, ... of the bounds
+// of pages g and g + 8, the next 16 pages' while these are multiplied.  A piece is
+// eight consecutive dimensions, which serve two k-steps: the order of k is free
+// as long as the queries use the same one, so no shared memory is needed.
+// Pieces 0..15 (lo) meet min(q, 0) and pieces 16..31 (hi) meet max(q, 0).
+//
+// Plain loads, because they move 64 bytes per clock and SM in this pattern; the
+// same pieces by cp.async take 27 cycles per warp instruction (19 bytes per clock)
+// and a bulk copy per page 16 cycles (32), where the memory delivers 23.
 //
 // Error bound: a k16 step adds 16 exact products to the accumulator with at
 // most 17 roundings or truncations at the largest addend, 2^-23 each; four
@@ -177,26 +165,17 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kScoreTile = 16 * kWarps;      // pages of one pass of a CTA
 constexpr int kScorePasses = 8;              // most passes of a CTA
-constexpr int kScoreStages = 3;
-constexpr int kRow = 576, kRowBytes = 512;   // a page's place and its bytes
-constexpr int kScoreStage = 16 * kRow;
-constexpr int kScoreSmem = kWarps * kScoreStages * kScoreStage;   // 108 KB: two CTAs per SM
 
 template <int NH>   // groups of eight query heads
 __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArgs a, int passes) {
-  extern __shared__ __align__(128) uint8_t raw[];
-  __shared__ __align__(8) uint64_t full[kWarps][kScoreStages];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.x % a.Hkv, chunk = blockIdx.x / a.Hkv;
   const int r = blockIdx.y;
   const int G = a.Hq / a.Hkv;
   const int begin = chunk * passes * kScoreTile + warp * 16;   // this warp's first page; the next ones 64 further
-  if (lane < kScoreStages) mbar_init(&full[warp][lane], 1);
-  fence_barrier_init();
-  __syncwarp();
-  pdl_wait();
   const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
+  pdl_wait();
   // lane l holds page l % 16 of passes l / 16, 2 + l / 16, ...; fetched before the length is known
   int table[kScorePasses / 2];
 #pragma unroll
@@ -214,32 +193,36 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
     return;
   }
   const int mine = (end - begin + kScoreTile - 1) / kScoreTile;   // passes of this warp
-  uint8_t* ring = raw + warp * kScoreStages * kScoreStage;
-  auto issue = [&](int it, int st) {
-    if (it >= mine) return;
-    int phys = 0;
 #pragma unroll
-    for (int i = 0; i < kScorePasses / 2; ++i) {
-      const int v = __shfl_sync(kFull, table[i], (it & 1) * 16 + (lane & 15));
-      if (it >> 1 == i) phys = v;
+  for (int i = 0; i < kScorePasses / 2; ++i) {
+    const int p = begin + (2 * i + (lane >> 4)) * kScoreTile + (lane & 15);
+    if (table[i] < 0 || table[i] >= a.num_pages) {   // recorded; the reserved zero page stands in
+      if (p < end) set_error(kErrBadIndex, (unsigned long long)p);
+      table[i] = 0;
     }
-    const int p0 = begin + it * kScoreTile;
-    const int count = min(16, end - p0);
-    if (lane == 0) mbar_arrive_expect_tx(&full[warp][st], count * kRowBytes);
-    __syncwarp();
-    if (lane < count) {
-      if (phys < 0 || phys >= a.num_pages) {   // recorded; the reserved zero page stands in
-        set_error(kErrBadIndex, (unsigned long long)(p0 + lane));
-        phys = 0;
-      }
-      bulk_load(ring + st * kScoreStage + lane * kRow, a.bounds + ((int64_t)phys * a.Hkv + kvh) * 2 * D, kRowBytes,
-                &full[warp][st]);
-    }
-    __syncwarp();
+  }
+  const uint4* bounds = reinterpret_cast<const uint4*>(a.bounds) + kvh * (2 * D / 8) + c;
+  const int64_t page_pieces = (int64_t)a.Hkv * (2 * D / 8);
+  struct Tile {
+    uint4 a[8], b[8];
   };
+  auto load = [&](int it, Tile& t) {
+    int v = table[0];
 #pragma unroll
-  for (int i = 0; i < kScoreStages; ++i) issue(i, i);
-
+    for (int i = 1; i < kScorePasses / 2; ++i)
+      if (it >> 1 == i) v = table[i];
+    const int pa = __shfl_sync(kFull, v, (it & 1) * 16 + g), pb = __shfl_sync(kFull, v, (it & 1) * 16 + g + 8);
+    // entries past the row's end read page 0 or the table's; their scores are not stored
+    const uint4* ra = bounds + pa * page_pieces;
+    const uint4* rb = bounds + pb * page_pieces;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      t.a[j] = ld_stream(ra + 4 * j);
+      t.b[j] = ld_stream(rb + 4 * j);
+    }
+  };
+  Tile t0;
+  load(0, t0);
   uint4 q[NH][4];
 #pragma unroll
   for (int t = 0; t < NH; ++t) {
@@ -249,62 +232,39 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
       q[t][j] = t * 8 + g < G ? *reinterpret_cast<const uint4*>(qh + 8 * (c + 4 * j)) : make_uint4(0u, 0u, 0u, 0u);
   }
   float2* ws = a.ws + ((int64_t)r * a.Hkv + kvh) * a.width;
-  const uint32_t at0 = smem_u32(ring) + g * kRow + c * 16;
-  int st = 0;
-  uint32_t parity = 0;
-  for (int it = 0; it < mine; ++it) {
+  auto score = [&](int it, const Tile& tile) {
     const int p0 = begin + it * kScoreTile;
-    if (!__all_sync(kFull, mbar_wait(&full[warp][st], parity, 30))) {
-      // recorded; leave once the copies under way have landed or had their time
-      for (int i = 0; i < kScoreStages && it + i < mine; ++i) {
-        const int x = st + i;
-        drain(&full[warp][x % kScoreStages], parity ^ (x >= kScoreStages ? 1u : 0u));
-      }
-      return;
-    }
-    const uint32_t at = at0 + st * kScoreStage;
-    float s[NH][4][4], m[NH][4];
+    float best_a = -INFINITY, best_b = -INFINITY, err_a = 0.f, err_b = 0.f;
 #pragma unroll
-    for (int t = 0; t < NH; ++t)
+    for (int t = 0; t < NH; ++t) {
+      float s[4][4], m[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = m[t][i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = m[i] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // rows past the last page hold what the ring held; their columns are not stored
-      const uint4 va = lds16(at + j * 64), vb = lds16(at + 8 * kRow + j * 64);
-      const uint32_t* pa4 = reinterpret_cast<const uint32_t*>(&va);
-      const uint32_t* pb4 = reinterpret_cast<const uint32_t*>(&vb);
-#pragma unroll
-      for (int t = 0; t < NH; ++t) {
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t* pa4 = reinterpret_cast<const uint32_t*>(&tile.a[j]);
+        const uint32_t* pb4 = reinterpret_cast<const uint32_t*>(&tile.b[j]);
         const uint32_t* q4 = reinterpret_cast<const uint32_t*>(&q[t][j & 3]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t b0 = j < 4 ? min_nan(q4[2 * h], 0u) : max_nan(q4[2 * h], 0u);
           const uint32_t b1 = j < 4 ? min_nan(q4[2 * h + 1], 0u) : max_nan(q4[2 * h + 1], 0u);
-          mma_bf16(s[t][j & 3], pa4[2 * h], pb4[2 * h], pa4[2 * h + 1], pb4[2 * h + 1], b0, b1);
+          mma_bf16(s[j & 3], pa4[2 * h], pb4[2 * h], pa4[2 * h + 1], pb4[2 * h + 1], b0, b1);
           constexpr uint32_t kAbs = 0x7fff7fffu;
-          mma_bf16(m[t], pa4[2 * h] & kAbs, pb4[2 * h] & kAbs, pa4[2 * h + 1] & kAbs, pb4[2 * h + 1] & kAbs,
-                   b0 & kAbs, b1 & kAbs);
+          mma_bf16(m, pa4[2 * h] & kAbs, pb4[2 * h] & kAbs, pa4[2 * h + 1] & kAbs, pb4[2 * h + 1] & kAbs, b0 & kAbs,
+                   b1 & kAbs);
         }
       }
-    }
-    __syncwarp();
-    fence_proxy_async_smem();
-    issue(it + kScoreStages, st);
-    if (++st == kScoreStages) st = 0, parity ^= 1;
-    float best_a = -INFINITY, best_b = -INFINITY, err_a = 0.f, err_b = 0.f;
-#pragma unroll
-    for (int t = 0; t < NH; ++t) {
       // columns 2c, 2c + 1 of pages g and g + 8
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float v = (s[t][0][i] + s[t][1][i]) + (s[t][2][i] + s[t][3][i]);
+        const float v = (s[0][i] + s[1][i]) + (s[2][i] + s[3][i]);
         if (t * 8 + 2 * c + (i & 1) < G) {
-          const bool fin = isfinite(v) && isfinite(m[t][i]);
+          const bool fin = isfinite(v) && isfinite(m[i]);
           float& b = i < 2 ? best_a : best_b;
           float& e = i < 2 ? err_a : err_b;
           b = fmaxf(b, fin ? v : INFINITY);
-          e = fmaxf(e, fin ? m[t][i] * kScoreErr : 0.f);
+          e = fmaxf(e, fin ? m[i] * kScoreErr : 0.f);
         }
       }
     }
@@ -318,6 +278,22 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
     if (c == 0) {
       if (p0 + g < end) ws[p0 + g] = make_float2(best_a, isinf(best_a) ? 0.f : err_a);
       if (p0 + g + 8 < end) ws[p0 + g + 8] = make_float2(best_b, isinf(best_b) ? 0.f : err_b);
+    }
+  };
+  if (NH == 1) {
+    Tile t1;
+    for (int it = 0; it < mine; it += 2) {
+      if (it + 1 < mine) load(it + 1, t1);
+      score(it, t0);
+      if (it + 1 < mine) {
+        if (it + 2 < mine) load(it + 2, t0);
+        score(it + 1, t1);
+      }
+    }
+  } else {   // 16 heads: their operands leave no registers for a second tile
+    for (int it = 0; it < mine; ++it) {
+      score(it, t0);
+      if (it + 1 < mine) load(it + 1, t0);
     }
   }
   pdl_trigger();
@@ -358,7 +334,7 @@ struct SelectSmem {
   int hist[kSelBins];
   float list_s[kSelList], list_e[kSelList];
   int list_idx[kSelList];
-  double list_val[kSelList];
+  unsigned long long list_key[kSelList];
   uint32_t red[2][32];
   int count_in[32], count_open[32];
   int cnt[4], totals[4];
@@ -374,14 +350,15 @@ struct SelectUnit {
   int kvh, G, n, first, mid1, k;   // pages, first competing, last competing + 1, places for them
 };
 
-// Exact score of one page by one warp: four dimensions per lane, fp64.
-__device__ __forceinline__ double exact_score(const SelectArgs& a, const SelectUnit& u, int page, int lane) {
+// Exact score of one page for heads [h0, h1) by one warp: four dimensions per lane, fp64.
+__device__ __forceinline__ double exact_score(const SelectArgs& a, const SelectUnit& u, int page, int lane, int h0,
+                                              int h1) {
   const __nv_bfloat16* b = a.bounds + ((int64_t)table_page(u.bt, page, a.num_pages) * a.Hkv + u.kvh) * 2 * D + lane * 4;
   const uint2 lo2 = *reinterpret_cast<const uint2*>(b), hi2 = *reinterpret_cast<const uint2*>(b + D);
   const __nv_bfloat16* lo = reinterpret_cast<const __nv_bfloat16*>(&lo2);
   const __nv_bfloat16* hi = reinterpret_cast<const __nv_bfloat16*>(&hi2);
   double best = -INFINITY;
-  for (int h = 0; h < u.G; ++h) {
+  for (int h = h0; h < h1; ++h) {
     const uint2 q2 = *reinterpret_cast<const uint2*>(u.q + h * D + lane * 4);
     const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(&q2);
     double sum = 0.0;
@@ -479,7 +456,7 @@ __device__ __noinline__ void select_general(const SelectArgs& a, const SelectUni
         m &= m - 1;
         const bool finite = isfinite(u.ws[p].x);
         __syncwarp();
-        const double v = finite ? exact_score(a, u, p, lane) : INFINITY;
+        const double v = finite ? exact_score(a, u, p, lane, 0, u.G) : INFINITY;
         if (lane == 0) exact[p] = v;
       }
     }
@@ -718,20 +695,23 @@ __global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
       if (open >> i & 1u) {
         place[i] = atomicAdd(&sm.totals[1], 1);
         sm.list_idx[place[i]] = page0 + i * 32;
-        sm.list_s[place[i]] = v[i].x;
+        sm.list_key[place[i]] = isfinite(v[i].x) ? 0ull : order_key64(INFINITY);
       }
     }
     __syncthreads();
-    for (int i = warp; i < n_open; i += kW) {
-      const double x = isfinite(sm.list_s[i]) ? exact_score(a, u, sm.list_idx[i], lane) : INFINITY;
-      if (lane == 0) sm.list_val[i] = x;
+    // a warp per page and head; the page's score is the heads' largest
+    for (int i = warp; i < n_open * u.G; i += kW) {
+      const int o = i / u.G, h = i % u.G;
+      if (sm.list_key[o] == order_key64(INFINITY)) continue;   // stays so: no finite score reaches it
+      const double x = exact_score(a, u, sm.list_idx[o], lane, h, h + 1);
+      if (lane == 0) atomicMax(&sm.list_key[o], order_key64(x));
     }
     __syncthreads();
     for (int i = tid; i < n_open; i += NT) {
-      const double x = sm.list_val[i];
+      const unsigned long long x = sm.list_key[i];
       const int p = sm.list_idx[i];
       int rank = 0;
-      for (int j = 0; j < n_open; ++j) rank += sm.list_val[j] > x || (sm.list_val[j] == x && sm.list_idx[j] < p);
+      for (int j = 0; j < n_open; ++j) rank += sm.list_key[j] > x || (sm.list_key[j] == x && sm.list_idx[j] < p);
       sm.list_e[i] = rank < need ? 1.f : 0.f;
     }
     __syncthreads();
@@ -770,8 +750,6 @@ __global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
 // The next page's K is fetched into the same registers as soon as S is known,
 // its V after O is updated: 16 warps per SM with a page each under way.
 // ===========================================================================
-constexpr int kSpWarps = 8;
-constexpr int kSpThreads = kSpWarps * 32;
 constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -795,20 +773,20 @@ __device__ __forceinline__ void st_cluster2(uint32_t addr, float2 v) {
 }
 
 constexpr int kOLd = D + 4;
-template <int NH>
+template <int NH, int W>
 struct SparseSmem {
-  float o[kSpWarps][NH * 8][kOLd];
-  float2 ml[kSpWarps][NH * 8];             // running maximum and sum
+  float o[W][NH * 8][kOLd];
+  float2 ml[W][NH * 8];             // running maximum and sum
   // from every CTA of the cluster, for the outputs this CTA owns: quads of
   // dimensions q with q % cl == this CTA
   float4 in_o[kMaxCluster][NH * 8 * (D / 4) / 2];
   float2 in_ml[kMaxCluster][NH * 8];
 };
 
-template <int NH>
-__global__ void __launch_bounds__(kSpThreads, NH == 1 ? 2 : 1) decode_sparse_kernel(const SparseArgs a, int cl) {
+template <int NH, int W>   // W warps
+__global__ void __launch_bounds__(W * 32, (NH == 1 ? 16 : 8) / W) decode_sparse_kernel(const SparseArgs a, int cl) {
   extern __shared__ __align__(128) uint8_t raw[];
-  SparseSmem<NH>& sm = *reinterpret_cast<SparseSmem<NH>*>(raw);
+  SparseSmem<NH, W>& sm = *reinterpret_cast<SparseSmem<NH, W>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int part = cl > 1 ? (int)cluster_rank() : 0;
@@ -817,7 +795,7 @@ __global__ void __launch_bounds__(kSpThreads, NH == 1 ? 2 : 1) decode_sparse_ker
   const int G = a.Hq / a.Hkv;
   // this warp's pages: entries w, w + stride, ... of the list; lane j holds the
   // j-th of a window of 32 (first token, physical page), the next window under way
-  const int stride = cl * kSpWarps, w = part * kSpWarps + warp;
+  const int stride = cl * W, w = part * W + warp;
   const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
   const int32_t* sel = a.sel + ((int64_t)r * a.Hkv + kvh) * a.budget;
   if (cl > 1) cluster_arrive();         // every CTA of the cluster runs before another one writes to it
@@ -875,11 +853,6 @@ __global__ void __launch_bounds__(kSpThreads, NH == 1 ? 2 : 1) decode_sparse_ker
       v[1][x] = on ? ld_stream(vl + at + t * D + 64) : make_uint4(0u, 0u, 0u, 0u);
     }
   };
-  if (mine > 0) {
-    locate(0);
-    load_k();
-    load_v();
-  }
   uint4 q[NH][4];
 #pragma unroll
   for (int t = 0; t < NH; ++t) {
@@ -899,6 +872,9 @@ __global__ void __launch_bounds__(kSpThreads, NH == 1 ? 2 : 1) decode_sparse_ker
   }
 
   for (int i = 0; i < mine; ++i) {
+    locate(i);
+    load_k();
+    load_v();
     t0 = t0_next;
     float s[NH][2][4];
 #pragma unroll
@@ -910,10 +886,6 @@ __global__ void __launch_bounds__(kSpThreads, NH == 1 ? 2 : 1) decode_sparse_ker
         mma_bf16(s[t][0], k0[j].x, k1[j].x, k0[j].y, k1[j].y, q[t][j].x, q[t][j].y);
         mma_bf16(s[t][1], k0[j].z, k1[j].z, k0[j].w, k1[j].w, q[t][j].z, q[t][j].w);
       }
-    }
-    if (i + 1 < mine) {
-      locate(i + 1);
-      load_k();
     }
     uint32_t p[NH][2];
 #pragma unroll
@@ -959,7 +931,6 @@ __global__ void __launch_bounds__(kSpThreads, NH == 1 ? 2 : 1) decode_sparse_ker
 #pragma unroll
       for (int t = 0; t < NH; ++t) mma_bf16(o[t][i8], a0, a1, a2, a3, p[t][0], p[t][1]);
     }
-    if (i + 1 < mine) load_v();
   }
 
   pdl_trigger();
@@ -994,16 +965,16 @@ __global__ void __launch_bounds__(kSpThreads, NH == 1 ? 2 : 1) decode_sparse_ker
       *reinterpret_cast<uint2*>(out + quad * 4) = make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
   };
   // quads of four dimensions, head by head: the CTA's warps, then the cluster's CTAs
-  for (int quad = tid; quad < G * (D / 4); quad += kSpThreads) {
+  for (int quad = tid; quad < G * (D / 4); quad += (W * 32)) {
     const int h = quad / (D / 4), d = quad % (D / 4) * 4;
     float mx = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < kSpWarps; ++x) mx = fmaxf(mx, sm.ml[x][h].x);
+    for (int x = 0; x < W; ++x) mx = fmaxf(mx, sm.ml[x][h].x);
     const float sh = mx == -INFINITY ? 0.f : mx;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
 #pragma unroll
-    for (int x = 0; x < kSpWarps; ++x) {
+    for (int x = 0; x < W; ++x) {
       const float2 ml = sm.ml[x][h];
       const float f = exp2f(ml.x - sh);
       const float4 y = *reinterpret_cast<const float4*>(&sm.o[x][h][d]);
@@ -1020,7 +991,7 @@ __global__ void __launch_bounds__(kSpThreads, NH == 1 ? 2 : 1) decode_sparse_ker
   if (cl == 1) return;
   cluster_arrive();
   cluster_wait();
-  for (int quad = tid * cl + part; quad < G * (D / 4); quad += kSpThreads * cl) {
+  for (int quad = tid * cl + part; quad < G * (D / 4); quad += (W * 32) * cl) {
     const int h = quad / (D / 4);
     float mx = -INFINITY;
     for (int x = 0; x < cl; ++x) mx = fmaxf(mx, sm.in_ml[x][h].x);
@@ -1075,34 +1046,44 @@ void select_pages(const SelectArgs& a, cudaStream_t s) {
   if (a.width > a.budget) {
     // up to eight passes of 64 pages per CTA, fewer where that leaves SMs without work
     const int64_t tiles = (int64_t)a.rows * a.Hkv * ((a.width + kScoreTile - 1) / kScoreTile);
-    const int64_t want = tiles / (4 * sm_count());
+    const int64_t want = getenv("OV_P") ? atoi(getenv("OV_P")) : tiles / (4 * sm_count());
     const int passes = want < 1 ? 1 : want > kScorePasses ? kScorePasses : (int)want;
     const int chunk = passes * kScoreTile;
     const dim3 grid((unsigned)((a.width + chunk - 1) / chunk * a.Hkv), (unsigned)a.rows);
     auto k = a.Hq / a.Hkv <= 8 ? page_score_kernel<1> : page_score_kernel<2>;
-    raise_smem(reinterpret_cast<const void*>(k), kScoreSmem);
-    launch_k(k, grid, dim3(kThreads), kScoreSmem, s, 1, a, passes);
+    launch_k(k, grid, dim3(kThreads), 0, s, 1, a, passes);
   }
   if (a.width <= 512) launch_select<256, 2>(a, s);
-  else if (a.width <= 2048) launch_select<512, 4>(a, s);
+  else if (a.width <= 2048) launch_select<256, 8>(a, s);
   else if (a.width <= 8192) launch_select<1024, 8>(a, s);
   else launch_select<1024, 0>(a, s);
 }
 
-void decode_sparse(const SparseArgs& a, cudaStream_t s) {
-  if (a.rows <= 0) return;
+namespace {
+template <int NH, int W>
+void launch_decode(const SparseArgs& a, cudaStream_t s) {
   const int64_t units = (int64_t)a.rows * a.Hkv;
-  const int64_t slots = (int64_t)sm_count() * 2;
+  // CTAs per unit: as many as run at the same time (16 warps per SM, 8 for wide
+  // groups) and get two pages per warp
+  const int64_t slots = (int64_t)sm_count() * ((NH == 1 ? 16 : 8) / W);
   int cl = 1;
-  while (cl < kMaxCluster && units * cl < slots && a.budget > kSpWarps * cl) cl *= 2;
-  const bool wide = a.Hq / a.Hkv > 8;
-  auto k = wide ? decode_sparse_kernel<2> : decode_sparse_kernel<1>;
-  const size_t smem = wide ? sizeof(SparseSmem<2>) : sizeof(SparseSmem<1>);
-  raise_smem(reinterpret_cast<const void*>(k), smem);
+  while (cl < kMaxCluster && units * cl * 2 <= slots && a.budget > W * cl) cl *= 2;
+  auto k = decode_sparse_kernel<NH, W>;
+  raise_smem(reinterpret_cast<const void*>(k), sizeof(SparseSmem<NH, W>));
   // Clusters that start while the previous kernel still holds some SMs crowd onto
   // the others; where they would fill the GPU they wait for its end (4 rows x 8
   // heads x 256 pages after a selection: 72 instead of 82 us for the whole step).
-  launch_with(cl == 1 || units * cl <= sm_count(), k, dim3((unsigned)(units * cl)), dim3(kSpThreads), smem, s, (unsigned)cl, a, cl);
+  launch_with(cl == 1 || units * cl * W <= sm_count() * 8, k, dim3((unsigned)(units * cl)), dim3(W * 32),
+              sizeof(SparseSmem<NH, W>), s, (unsigned)cl, a, cl);
+}
+}  // namespace
+
+void decode_sparse(const SparseArgs& a, cudaStream_t s) {
+  if (a.rows <= 0) return;
+  // eight warps per CTA where clusters of eight CTAs still leave SMs without work
+  const bool few = (int64_t)a.rows * a.Hkv * kMaxCluster <= sm_count();
+  if (a.Hq / a.Hkv <= 8) few ? launch_decode<1, 8>(a, s) : launch_decode<1, 4>(a, s);
+  else few ? launch_decode<2, 8>(a, s) : launch_decode<2, 4>(a, s);
 }
 
 }  // namespace attn
