@@ -27,7 +27,6 @@
 #include <stdint.h>
 
 #include <stdexcept>
-#include <cstdlib>
 
 #include "attention_sparse.h"
 #include "common.cuh"
@@ -145,14 +144,15 @@ __global__ void __launch_bounds__(128) page_bounds_kernel(const BoundsArgs a) {
 // ===========================================================================
 // Page scores.  A warp takes 16 pages at a time as the 16 rows of m16n8k16; lane
 // (g, c) = (lane / 4, lane % 4) loads 16-byte pieces c, c + 4, ... of the bounds
-// of pages g and g + 8, the next 16 pages' while these are multiplied.  A piece is
+// of pages g and g + 8, sixteen warps per SM with a tile each under way.  A piece is
 // eight consecutive dimensions, which serve two k-steps: the order of k is free
 // as long as the queries use the same one, so no shared memory is needed.
 // Pieces 0..15 (lo) meet min(q, 0) and pieces 16..31 (hi) meet max(q, 0).
 //
-// Plain loads, because they move 64 bytes per clock and SM in this pattern; the
-// same pieces by cp.async take 27 cycles per warp instruction (19 bytes per clock)
-// and a bulk copy per page 16 cycles (32), where the memory delivers 23.
+// Plain loads, because the same pieces by cp.async take 27 cycles per warp
+// instruction (19 bytes per clock, where the memory delivers 23), and a bulk copy
+// per page 130 cycles of the issuing warp; a second tile in registers halves the
+// warps (64 rows x 8 heads x 2048 pages: 92 us so, 97, 97 and 102 the other ways).
 //
 // Error bound: a k16 step adds 16 exact products to the accumulator with at
 // most 17 roundings or truncations at the largest addend, 2^-23 each; four
@@ -164,10 +164,10 @@ constexpr float kScoreErr = 1.f / 32768.f;   // 2^-15, four times what is derive
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kScoreTile = 16 * kWarps;      // pages of one pass of a CTA
-constexpr int kScorePasses = 8;              // most passes of a CTA
+constexpr int kScorePasses = 2;              // most passes of a CTA
 
 template <int NH>   // groups of eight query heads
-__global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArgs a, int passes) {
+__global__ void __launch_bounds__(kThreads, NH == 1 ? 4 : 2) page_score_kernel(const SelectArgs a, int passes) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.x % a.Hkv, chunk = blockIdx.x / a.Hkv;
@@ -176,13 +176,9 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
   const int begin = chunk * passes * kScoreTile + warp * 16;   // this warp's first page; the next ones 64 further
   const int32_t* bt = a.block_table + (int64_t)r * a.bt_stride;
   pdl_wait();
-  // lane l holds page l % 16 of passes l / 16, 2 + l / 16, ...; fetched before the length is known
-  int table[kScorePasses / 2];
-#pragma unroll
-  for (int i = 0; i < kScorePasses / 2; ++i) {
-    const int pass = 2 * i + (lane >> 4), p = begin + pass * kScoreTile + (lane & 15);
-    table[i] = pass < passes && p < a.width ? bt[p] : 0;
-  }
+  // lane l holds page l % 16 of pass l / 16; fetched before the length is known
+  const int lane_page = begin + (lane >> 4) * kScoreTile + (lane & 15);
+  int table = (lane >> 4) < passes && lane_page < a.width ? bt[lane_page] : 0;
   const int tok = a.tok_index[r];
   const int L = row_length(a.seq_lens, r, a.width);
   const int n = (L + PAGE - 1) / PAGE;
@@ -193,13 +189,9 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
     return;
   }
   const int mine = (end - begin + kScoreTile - 1) / kScoreTile;   // passes of this warp
-#pragma unroll
-  for (int i = 0; i < kScorePasses / 2; ++i) {
-    const int p = begin + (2 * i + (lane >> 4)) * kScoreTile + (lane & 15);
-    if (table[i] < 0 || table[i] >= a.num_pages) {   // recorded; the reserved zero page stands in
-      if (p < end) set_error(kErrBadIndex, (unsigned long long)p);
-      table[i] = 0;
-    }
+  if (table < 0 || table >= a.num_pages) {   // recorded; the reserved zero page stands in
+    if (lane_page < end) set_error(kErrBadIndex, (unsigned long long)lane_page);
+    table = 0;
   }
   const uint4* bounds = reinterpret_cast<const uint4*>(a.bounds) + kvh * (2 * D / 8) + c;
   const int64_t page_pieces = (int64_t)a.Hkv * (2 * D / 8);
@@ -207,11 +199,7 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
     uint4 a[8], b[8];
   };
   auto load = [&](int it, Tile& t) {
-    int v = table[0];
-#pragma unroll
-    for (int i = 1; i < kScorePasses / 2; ++i)
-      if (it >> 1 == i) v = table[i];
-    const int pa = __shfl_sync(kFull, v, (it & 1) * 16 + g), pb = __shfl_sync(kFull, v, (it & 1) * 16 + g + 8);
+    const int pa = __shfl_sync(kFull, table, it * 16 + g), pb = __shfl_sync(kFull, table, it * 16 + g + 8);
     // entries past the row's end read page 0 or the table's; their scores are not stored
     const uint4* ra = bounds + pa * page_pieces;
     const uint4* rb = bounds + pb * page_pieces;
@@ -280,21 +268,9 @@ __global__ void __launch_bounds__(kThreads, 2) page_score_kernel(const SelectArg
       if (p0 + g + 8 < end) ws[p0 + g + 8] = make_float2(best_b, isinf(best_b) ? 0.f : err_b);
     }
   };
-  if (NH == 1) {
-    Tile t1;
-    for (int it = 0; it < mine; it += 2) {
-      if (it + 1 < mine) load(it + 1, t1);
-      score(it, t0);
-      if (it + 1 < mine) {
-        if (it + 2 < mine) load(it + 2, t0);
-        score(it + 1, t1);
-      }
-    }
-  } else {   // 16 heads: their operands leave no registers for a second tile
-    for (int it = 0; it < mine; ++it) {
-      score(it, t0);
-      if (it + 1 < mine) load(it + 1, t0);
-    }
+  for (int it = 0; it < mine; ++it) {
+    if (it > 0) load(it, t0);
+    score(it, t0);
   }
   pdl_trigger();
 }
@@ -1044,10 +1020,10 @@ void launch_select(const SelectArgs& a, cudaStream_t s) {
 void select_pages(const SelectArgs& a, cudaStream_t s) {
   if (a.rows <= 0) return;
   if (a.width > a.budget) {
-    // up to eight passes of 64 pages per CTA, fewer where that leaves SMs without work
+    // two passes of 64 pages per CTA where that fills the GPU (64 rows of 2048 pages: 191 us a
+    // step, 198 with one, 192 with eight; a ragged batch of 17: 38, 40, 43)
     const int64_t tiles = (int64_t)a.rows * a.Hkv * ((a.width + kScoreTile - 1) / kScoreTile);
-    const int64_t want = getenv("OV_P") ? atoi(getenv("OV_P")) : tiles / (4 * sm_count());
-    const int passes = want < 1 ? 1 : want > kScorePasses ? kScorePasses : (int)want;
+    const int passes = tiles > 4 * sm_count() ? kScorePasses : 1;
     const int chunk = passes * kScoreTile;
     const dim3 grid((unsigned)((a.width + chunk - 1) / chunk * a.Hkv), (unsigned)a.rows);
     auto k = a.Hq / a.Hkv <= 8 ? page_score_kernel<1> : page_score_kernel<2>;

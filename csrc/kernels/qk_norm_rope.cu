@@ -8,12 +8,12 @@
 // V heads are copied.  All arithmetic is fp32 with one rounding to bf16 at the
 // store; the sum of squares of a head stays in registers.
 //
-// Bound by memory: every head is read once and written once.  D / 8 lanes own
-// one head, 16 bytes each, so the two elements of a rotation pair sit D / 16
-// lanes apart and meet by one shuffle, and the sum of squares is a shuffle
-// reduction over the same lanes: no shared memory and no barrier.  A CTA owns
-// one token; its lanes load the token's (cos, sin) row and the two weights
-// once and keep them while they walk the heads.
+// Bound by memory: every head is read once and written once.  D / 16 lanes own
+// one head, each 16 bytes of its first half and the 16 bytes D / 2 further on, so
+// both elements of a rotation pair lie in one lane and the sum of squares takes
+// three shuffles for 16 elements: no shared memory and no barrier.  A CTA owns one
+// token; its lanes load the token's (cos, sin) row and the two weights once and
+// keep them while they walk the heads.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -44,89 +44,121 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 }
 
 // Heads whose loads are in flight together per lane group.
-constexpr int kBatch = 4;
+constexpr int kBatch = 3;
 
 template <int D, int NT>
 __global__ void __launch_bounds__(NT) qk_norm_rope_kernel(const QkNormRopeArgs a) {
-  constexpr int kLanes = D / 8;          // lanes of one head
+  constexpr int kLanes = D / 16;         // lanes of one head
+  constexpr int kHalf = D / 16;          // 16-byte pieces of half a head
   constexpr int kGroups = NT / kLanes;   // heads a CTA works on at a time
   pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x;
   const int group = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
-  const bool upper = l >= kLanes / 2;    // this lane holds elements of the second half
-  const int pair = (l % (kLanes / 2)) * 8;
   const int heads = a.Hq + 2 * a.Hkv;
-  const uint4* row = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.qkv) + (int64_t)t * a.ld);
-
+  const uint4* row = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.qkv) + (int64_t)t * a.ld) + l;
+  uint4 v[kBatch][2];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int h = h0 + b * kGroups;
+      if (h < heads) {
+        v[b][0] = row[h * 2 * kHalf];
+        v[b][1] = row[h * 2 * kHalf + kHalf];
+      } else {
+        v[b][0] = v[b][1] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  };
   const int pos = a.positions[t];
   const int slot = a.slots[t];
+  load(group);                           // under way before the position is known
+  const uint4* wq = reinterpret_cast<const uint4*>(a.q_weight) + l;
+  const uint4* wk = reinterpret_cast<const uint4*>(a.k_weight) + l;
+  const uint4 wq0 = wq[0], wq1 = wq[kHalf], wk0 = wk[0], wk1 = wk[kHalf];
   const bool pos_ok = pos >= 0 && pos < a.max_pos;
   const bool slot_ok = slot >= 0 && (int64_t)slot < a.num_slots;
-  if (threadIdx.x == 0 && (!pos_ok || (slot >= 0 && !slot_ok))) set_error(kErrBadIndex, (unsigned long long)t);
 
   float cs[8], sn[8];
   {
     // a position outside the table is recorded and not rotated
-    const float4* tab = reinterpret_cast<const float4*>(a.cos_sin) + ((int64_t)(pos_ok ? pos : 0) * (D / 2) + pair) / 2;
+    const float4* tab = reinterpret_cast<const float4*>(a.cos_sin) + ((int64_t)(pos_ok ? pos : 0) * (D / 2) + l * 8) / 2;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 v = pos_ok ? tab[i] : make_float4(1.f, 0.f, 1.f, 0.f);
-      cs[2 * i] = v.x;
-      sn[2 * i] = upper ? v.y : -v.y;
-      cs[2 * i + 1] = v.z;
-      sn[2 * i + 1] = upper ? v.w : -v.w;
+      const float4 x = pos_ok ? tab[i] : make_float4(1.f, 0.f, 1.f, 0.f);
+      cs[2 * i] = x.x;
+      sn[2 * i] = x.y;
+      cs[2 * i + 1] = x.z;
+      sn[2 * i + 1] = x.w;
     }
   }
-  const uint4 wq = reinterpret_cast<const uint4*>(a.q_weight)[l];
-  const uint4 wk = reinterpret_cast<const uint4*>(a.k_weight)[l];
+  if (threadIdx.x == 0 && (!pos_ok || (slot >= 0 && !slot_ok))) set_error(kErrBadIndex, (unsigned long long)t);
 
   const int64_t pg = slot_ok ? slot / a.page : 0;
   const int off = slot_ok ? slot % a.page : 0;
-  uint4* qrow = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.q_out) + (int64_t)t * a.q_ld);
+  uint4* qrow = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.q_out) + (int64_t)t * a.q_ld) + l;
+  uint4* krow = reinterpret_cast<uint4*>(a.kcache) + (pg * a.Hkv * a.page + off) * 2 * kHalf + l;
+  uint4* vrow = reinterpret_cast<uint4*>(a.vcache) + (pg * a.Hkv * a.page + off) * 2 * kHalf + l;
 
   for (int h0 = group; h0 - group < heads; h0 += kBatch * kGroups) {   // uniform trip count over the CTA
-    uint4 v[kBatch];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int h = h0 + b * kGroups;
-      v[b] = h < heads ? row[h * kLanes + l] : make_uint4(0u, 0u, 0u, 0u);
-    }
+    if (h0 != group) load(h0);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int h = h0 + b * kGroups;
       if (h - group >= heads) break;     // uniform: no lane group of this CTA has such a head
-      float x[8], w[8], o[8];
-      unpack8(v[b], x);
+      if (__all_sync(0xffffffffu, h >= a.Hq + a.Hkv)) {   // V heads only (or none)
+        if (h < heads && slot_ok) {
+          uint4* dst = vrow + (int64_t)(h - a.Hq - a.Hkv) * a.page * 2 * kHalf;
+          dst[0] = v[b][0];
+          dst[kHalf] = v[b][1];
+        }
+        continue;
+      }
+      float x[8], y[8], w[8];
+      unpack8(v[b][0], x);
+      unpack8(v[b][1], y);
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
 #pragma unroll
       for (int m = kLanes / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
       const float inv = rsqrtf(ss * (1.f / D) + a.eps);
-      unpack8(h < a.Hq ? wq : wk, w);
+      unpack8(h < a.Hq ? wq0 : wk0, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
+      unpack8(h < a.Hq ? wq1 : wk1, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * w[i];
+      float o[8], p[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float other = __shfl_xor_sync(0xffffffffu, x[i], kLanes / 2);
-        o[i] = x[i] * cs[i] + other * sn[i];
+        o[i] = x[i] * cs[i] - y[i] * sn[i];
+        p[i] = y[i] * cs[i] + x[i] * sn[i];
       }
       if (h < a.Hq) {
-        qrow[h * kLanes + l] = pack8(o);
+        qrow[h * 2 * kHalf] = pack8(o);
+        qrow[h * 2 * kHalf + kHalf] = pack8(p);
       } else if (h < heads && slot_ok) {
         const bool is_k = h < a.Hq + a.Hkv;
-        const int kh = h - a.Hq - (is_k ? 0 : a.Hkv);
-        uint4* dst = reinterpret_cast<uint4*>(is_k ? a.kcache : a.vcache);
-        dst[((pg * a.Hkv + kh) * a.page + off) * kLanes + l] = is_k ? pack8(o) : v[b];
+        uint4* dst = (is_k ? krow : vrow) + (int64_t)(h - a.Hq - (is_k ? 0 : a.Hkv)) * a.page * 2 * kHalf;
+        dst[0] = is_k ? pack8(o) : v[b][0];
+        dst[kHalf] = is_k ? pack8(p) : v[b][1];
       }
     }
   }
 }
 
+// Few tokens (two per SM at most) are bound by latency: 256 threads each, so that a
+// head group has one or two heads (256 rows of 48 heads of 128: 2.8 us, 3.7 with 64
+// threads).  Many are bound by memory: 64 threads, whose 1 KB rounds of loads and
+// stores interleave best (8192 rows: 37.2 us, 41.2 with 128, 69 with 256).
 template <int D>
 void launch_d(const QkNormRopeArgs& a, cudaStream_t s) {
-  launch_k(qk_norm_rope_kernel<D, 128>, dim3(a.T), dim3(128), 0, s, 1, a);
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (a.T <= 2 * sms) launch_k(qk_norm_rope_kernel<D, 256>, dim3(a.T), dim3(256), 0, s, 1, a);
+  else launch_k(qk_norm_rope_kernel<D, 64>, dim3(a.T), dim3(64), 0, s, 1, a);
 }
 
 }  // namespace
