@@ -13,14 +13,12 @@
 // CTA multiplies an eighth of K, the partial h are added through distributed
 // shared memory in rank order, and every CTA expands an eighth of the columns.
 // So the whole operator is one launch without a workspace, x and the weights
-// are read by one CTA each, and a row's result depends neither on the other
-// rows nor on the order of arrival.  Only the adapter's rank is read, of A and
-// of B: inside a tile, h has S * ceil8(rank) columns ("compact" below).
+// are read by one CTA each, and a result does not depend on the order of arrival.  Only the adapter's rank is read, of A and
+// of B: inside a tile, h has S * rank columns, the rank rounded up to 8 (16 in the large kernel) ("compact" below).
 //
-// Two kernels.  The small one (TM = 16, weights straight from global memory into
-// the MMA operands) is for decode, where reading the weights bounds the call;
-// the large one (TM = 32 or 64, x, A and B staged in shared memory) is for
-// prefill, where x, base and out do, and the weights come from L2 once per tile.
+// Two kernels.  The small one (TM = 16, mma.sync) is for decode, where reading the
+// weights bounds the call; the large one (TM = 64, tcgen05) is for prefill, where
+// x, base and out do, and the weights come from L2 once per tile.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -49,12 +47,6 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -76,10 +68,6 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void bar_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t x;
   asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(x));
@@ -200,14 +188,14 @@ struct BaseCols {
   }
 };
 
-// The idx-th block of W (32 or 64) columns that does not cross a slice: its
+// The idx-th block of W (32 or 128) columns that does not cross a slice: its
 // slice (-1 past the last block), first column and the slice's end.
 struct Block {
   int slice, c0, end;
 };
 template <int W>
 __device__ __forceinline__ Block column_block(const LoraArgs& a, int idx) {
-  const int* first = W == 32 ? a.block32 : a.block64;
+  const int* first = W == 32 ? a.block32 : a.block128;
   if (idx >= first[kMaxSlices]) return Block{-1, 0, 0};
   int s = 0;
 #pragma unroll
@@ -537,84 +525,122 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
 }
 
 // ===========================================================================
-// Large tiles: TM = 64 rows (32 where S * R > 256, so that the partial h and its
-// parts fit).  Shrink h = x A^T over chunks of 64 k in a three-stage cp.async
-// ring; a warp owns 32 rows and a share of the compact columns.  The partial h
-// are reduced in slices: CTA q of CL adds rows [q TM / CL, ...) of all CTAs, splits
-// them into bf16 parts and stores those into every CTA's shared memory, a fraction
-// of the traffic of every CTA reading everything.  Expand: a warp owns 16 rows,
-// the row groups of a column group share its 64 columns of B (two stages).
-// Shared-memory rows are 128 bytes with the 16-byte pieces xor-ed by row % 8.
+// Large tiles: 64 rows, both products on the fifth-generation tensor cores.
+//
+// Shrink: h = x A^T accumulates in tensor memory over chunks of 64 k, x rows and
+// the adapter's A rows in a three-stage cp.async ring with the 128-byte swizzle
+// the instruction reads.  Each CTA of the cluster has a share of K; the partial h
+// go to shared memory and are reduced in slices: CTA q of CL adds rows
+// [q 64 / CL, ...) of all CTAs, splits them into bf16 parts and stores those into
+// every CTA's shared memory, a fraction of the traffic of every CTA reading
+// everything.  Expand: blocks of 128 columns of B (two stages) against the parts
+// of h into one of two accumulators, read back in the 16 x 256-bit shape, in which
+// a lane holds two adjacent columns of rows g and g + 8; B's columns are stored in
+// an order that makes them eight consecutive columns over four tiles.
+//
+// The same tiles on mma.sync took 131 us for 8192 rows of ranks up to 64 beside a
+// QKV projection: fragment loads, copies and products filled one another's time.
+// A CTA holds 256 columns of tensor memory and at least 80 KB of shared memory,
+// so that two, and never more, share an SM.
 // ===========================================================================
+constexpr int TML = 64;                  // rows of a large tile
 constexpr int kStages = 3;
-constexpr int kLargeCols = kMaxSlices * kMaxRank;
-constexpr int kLargeRows = 768;         // listed rows from which the large tiles are used
+constexpr int kLargeCols = 256;          // most compact columns (one accumulator)
+constexpr int kLargeRows = 768;          // listed rows from which the large tiles are used
+constexpr int kTmemCols = 256;
+constexpr int kBN = 128;                 // columns of a block of the expansion
 
-template <int TM>
-__host__ __device__ constexpr int large_groups() { return kWarps / (TM / 16); }   // column groups of the expansion
-
-struct LargeSmem {
-  size_t hs, total;     // [stages | partial h | B stages] below hs
-};
-template <int TM>
-__host__ __device__ inline LargeSmem large_smem(int cols_max, int R, int parts) {
-  const size_t stages = (size_t)kStages * 128 * (TM + cols_max);
-  const size_t part = (size_t)TM * (cols_max + 4) * 4;
-  const size_t b = (size_t)large_groups<TM>() * 2 * 64 * ((R + 63) / 64 * 128);
-  size_t low = part > b ? part : b;
-  const size_t hs = (size_t)parts * TM * ((cols_max + 15) / 16 * 16 + 24) * 2;
-  if (low + hs < stages) low = stages - hs;
-  low = (low + 127) / 128 * 128;
-  return {low, low + hs};
+// 16 lanes x 8 groups of 8 columns: r[4 x + 0 / 1] = row g, columns 8 x + 2 c, + 1;
+// r[4 x + 2 / 3] = row g + 8.
+__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
 }
 
-template <bool F32, int TM, int NTW, int CL>
-__global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(const LoraArgs a, int cols_max, int smem_hs) {
+struct LargeSmem {
+  size_t hs, total;     // [ring | partial h | B stages] below hs; the ring may reach over it
+};
+__host__ __device__ inline LargeSmem large_smem(int cols_max, int R, int parts) {
+  const size_t ring = (size_t)kStages * 128 * (TML + cols_max);
+  const size_t part = (size_t)TML * (cols_max + 4) * 4;
+  const size_t b = (size_t)2 * kBN * ((R + 63) / 64 * 128);
+  const size_t low = ((part > b ? part : b) + 1023) / 1024 * 1024;
+  const size_t hs = (size_t)parts * ((cols_max + 63) / 64) * (TML * 128);
+  size_t total = low + hs > ring ? low + hs : ring;
+  if (total < 80 * 1024) total = 80 * 1024;
+  return {low, total + 1024};   // and the alignment to 1024
+}
+
+template <bool F32, int CL>
+__global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs a, int cols_max, int smem_hs) {
   constexpr int kParts = F32 ? 3 : 2;
-  constexpr int WR = TM / 32;             // row groups of the shrink
-  constexpr int WQ = kWarps / WR;         // column shares
-  constexpr int NCG = large_groups<TM>();
-  extern __shared__ __align__(128) uint8_t raw[];
-  __shared__ int tile_rows[TM];
-  __shared__ const __nv_bfloat16* row_src[TM + kLargeCols];   // first element of every staged row, null for a zero row
-  pdl_trigger();
-  pdl_wait();
+  extern __shared__ __align__(128) uint8_t raw_unaligned[];
+  __shared__ int tile_rows[TML];
+  __shared__ const __nv_bfloat16* row_src[TML + kLargeCols];   // first element of every staged row, null for a zero row
+  __shared__ __align__(8) uint64_t empty[kStages], done[2];
+  __shared__ uint32_t tmem_base;
+  uint8_t* raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int cta = (int)cluster_rank();
-  const Tile tl = find_tile<TM>(a, blockIdx.x / CL);
-  if (tl.adapter < 0) return;
+  pdl_wait();
+  const Tile tl = find_tile<TML>(a, blockIdx.x / CL);
+  if (tl.adapter < 0) return;             // the whole cluster
   const int rank = tl.rank;
-  const int rp = (rank + 7) / 8 * 8;
+  const int rp = (rank + 15) / 16 * 16;   // whole 16-wide steps; what lies past the rank is zero
   const int cols = a.S * rp;
-  const int ntiles = cols / 8;
-  const int hld = (cols_max + 15) / 16 * 16 + 24;       // hld / 8 is odd: ldmatrix rows hit all banks
   const int pld = cols_max + 4;
   float* part = reinterpret_cast<float*>(raw);
-  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(raw + smem_hs);
+  uint8_t* hs = raw + smem_hs;            // [part][64 columns][64 rows][128 bytes]
+  const int hpart = (cols_max + 63) / 64 * (TML * 128);
   const uint32_t raw_u = smem_u32(raw);
+  if (warp == 0) {
+    tmem_alloc(&tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&empty[i], 1);
+    mbar_init(&done[0], 1);
+    mbar_init(&done[1], 1);
+    fence_barrier_init();
+  }
 
   // ---- shrink
+  const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
   {
-    const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) + (int64_t)tl.adapter * a.S * a.R * a.K;
-    const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
-    const int chunks = (a.K + 63) / 64;
-    const int per_cta = (chunks + CL - 1) / CL;
-    const int ch0 = cta * per_cta, n = min(chunks, ch0 + per_cta) - ch0;
-    const int stage_bytes = 128 * (TM + cols);
-    for (int r = tid; r < TM + cols; r += kThreads) {
+    const __nv_bfloat16* A =
+        reinterpret_cast<const __nv_bfloat16*>(a.a) + ((int64_t)tl.adapter * a.S_all + a.s0) * a.R * a.K;
+    for (int r = tid; r < TML + cols; r += kThreads) {
       const __nv_bfloat16* src = nullptr;
-      if (r < TM) {
+      if (r < TML) {
         const int row = tile_row(a, tl, r);
         tile_rows[r] = row;
         if (row >= 0) src = x + (int64_t)row * a.ldx;
       } else {
-        const int j = r - TM, s = j / rp, q = j - s * rp;
+        const int j = r - TML, s = j / rp, q = j - s * rp;
         if (q < rank) src = A + (int64_t)(s * a.R + q) * a.K;
       }
       row_src[r] = src;
     }
-    __syncthreads();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  const int sub = warp & 3, half = warp >> 2;      // this warp's rows (16 sub ...) and columns of an accumulator
+  const uint32_t tmem_row = tmem + ((uint32_t)(sub * 32) << 16);
+  {
+    const int chunks = (a.K + 63) / 64;
+    const int per_cta = (chunks + CL - 1) / CL;
+    const int ch0 = cta * per_cta, n = cols > 0 ? max(0, min(chunks, ch0 + per_cta) - ch0) : 0;
+    const int stage_bytes = 128 * (TML + cols);
     // thread t copies piece t % 8 of rows t / 8, t / 8 + 32, ...
     const int piece = tid & 7, rfirst = tid >> 3;
     const uint32_t dst0 = raw_u + rfirst * 128 + ((piece ^ (rfirst & 7)) << 4);
@@ -623,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(
         const uint32_t dst = dst0 + (i % kStages) * stage_bytes;
         const int k = (ch0 + i) * 64 + piece * 8;
         const bool in = k < a.K;
-        for (int r = rfirst, o = 0; r < TM + cols; r += 32, o += 32 * 128) {
+        for (int r = rfirst, o = 0; r < TML + cols; r += 32, o += 32 * 128) {
           const __nv_bfloat16* src = row_src[r];
           const bool on = in && src != nullptr;
           cp_async16(dst + o, on ? src + k : x, on);
@@ -631,64 +657,55 @@ __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(
       }
       cp_async_commit();
     };
-    const int wr = warp % WR, wq = warp / WR;
-    const int per = (ntiles + 2 * WQ - 1) / (2 * WQ) * 2;       // even: ldmatrix brings tiles in pairs
-    const int t0 = wq * per, tn = min(ntiles, t0 + per) - t0;   // may be <= 0
-    float acc[2][NTW][4];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int t = 0; t < NTW; ++t) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.f;
     for (int i = 0; i < kStages - 1; ++i) load_stage(i);
+    const uint32_t idesc = idesc_bf16_f32(TML, cols);
     for (int i = 0; i < n; ++i) {
       cp_async_wait<kStages - 2>();
+      fence_proxy_async_smem();
       __syncthreads();
-      load_stage(i + kStages - 1);
-      const uint32_t st = raw_u + (i % kStages) * stage_bytes;
+      if (warp == 0 && elect_one()) {
+        const uint32_t st = raw_u + (i % kStages) * stage_bytes;
+        const uint64_t xd = sw128_kmajor_desc(st), ad = sw128_kmajor_desc(st + TML * 128);
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        uint32_t xa[2][4];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const int r = wr * 32 + m * 16 + (lane & 15);
-          ldsm_x4(st + r * 128 + (((ks * 2 + (lane >> 4)) ^ (r & 7)) << 4), xa[m]);
-        }
-#pragma unroll
-        for (int t = 0; t < NTW; t += 2) {
-          if (t >= tn) break;
-          // an odd last tile's partner lies past the compact columns: the row is clamped, the result unused
-          const int r = TM + min((t0 + t + (lane >> 4)) * 8 + (lane & 7), cols - 1);
-          uint32_t b[4];
-          ldsm_x4(st + r * 128 + (((ks * 2 + (lane >> 3 & 1)) ^ (r & 7)) << 4), b);
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            mma_bf16(acc[m][t], xa[m][0], xa[m][1], xa[m][2], xa[m][3], b[0], b[1]);
-            mma_bf16(acc[m][t + 1], xa[m][0], xa[m][1], xa[m][2], xa[m][3], b[2], b[3]);
-          }
-        }
+        for (int ks = 0; ks < 4; ++ks) umma_f16_ss(tmem, xd + 2 * ks, ad + 2 * ks, idesc, (i | ks) != 0);
+        umma_commit(&empty[i % kStages]);
       }
+      __syncwarp();
+      if (i > 0 && i + kStages - 1 < n) mbar_wait(&empty[(i - 1) % kStages], ((i - 1) / kStages) & 1, 40);
+      load_stage(i + kStages - 1);
     }
+    // A wait that runs out records an error: the step's results are void, the control flow stays.
+    if (n > 0) mbar_wait(&empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, 41);
     cp_async_wait<0>();
     __syncthreads();                      // the ring's memory becomes the partial h
+    tc_fence_after();
+    for (int c0 = half * 64; c0 < cols; c0 += 128) {
+      uint32_t r[32];
+      tmem_ld_16x256b_x8(tmem_row + c0, r);
+      tmem_wait_ld();
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int t = 0; t < NTW; ++t) {
-        if (t >= tn) break;
-        float* p = part + (wr * 32 + m * 16 + g) * pld + (t0 + t) * 8 + 2 * c;
-        *reinterpret_cast<float2*>(p) = make_float2(acc[m][t][0], acc[m][t][1]);
-        *reinterpret_cast<float2*>(p + 8 * pld) = make_float2(acc[m][t][2], acc[m][t][3]);
+      for (int xg = 0; xg < 8; ++xg) {
+        const int col = c0 + xg * 8 + 2 * c;
+        if (col >= cols) continue;
+        float* p = part + (sub * 16 + g) * pld + col;
+        const bool live = n > 0;          // a CTA without a share of K adds zero
+        *reinterpret_cast<float2*>(p) =
+            live ? make_float2(__uint_as_float(r[4 * xg]), __uint_as_float(r[4 * xg + 1])) : make_float2(0.f, 0.f);
+        *reinterpret_cast<float2*>(p + 8 * pld) =
+            live ? make_float2(__uint_as_float(r[4 * xg + 2]), __uint_as_float(r[4 * xg + 3])) : make_float2(0.f, 0.f);
       }
+    }
+    tc_fence_before();
   }
   cluster_arrive();
   cluster_wait();
   {
-    constexpr int kOwn = TM / CL;         // rows this CTA adds up
+    constexpr int kOwn = TML / CL;        // rows this CTA adds up
     uint32_t part_at[CL], hs_at[CL];
 #pragma unroll
     for (int q = 0; q < CL; ++q) {
       part_at[q] = cluster_addr(part + cta * kOwn * pld, q);
-      hs_at[q] = cluster_addr(hs + cta * kOwn * hld, q);
+      hs_at[q] = cluster_addr(hs, q);
     }
     const int quads = cols / 4;
     for (int i = tid; i < kOwn * quads; i += kThreads) {
@@ -700,126 +717,141 @@ __global__ void __launch_bounds__(kThreads, NTW <= 6 ? 2 : 1) lora_large_kernel(
       for (int q = 1; q < CL; ++q) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
       uint2 p[kParts];
       split4<kParts>(v[0], p);
+      const int hr = cta * kOwn + row;
+      const uint32_t off = (j >> 6) * (TML * 128) + hr * 128 + (((j & 63) >> 3 ^ (hr & 7)) << 4) + (j & 7) * 2;
 #pragma unroll
       for (int q = 0; q < CL; ++q)
 #pragma unroll
-        for (int s = 0; s < kParts; ++s) st_cluster2(hs_at[q] + ((s * TM + row) * hld + j) * 2, p[s]);
+        for (int s = 0; s < kParts; ++s) st_cluster2(hs_at[q] + s * hpart + off, p[s]);
     }
   }
+  asm volatile("fence.proxy.async;" ::: "memory");   // the tensor cores will read what was just stored
   cluster_arrive();                       // all parts of h are in place, all partials read
   cluster_wait();
+  asm volatile("fence.proxy.async;" ::: "memory");
 
   // ---- expand
   const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b) + (int64_t)tl.adapter * a.N * a.R;
-  constexpr int RG = TM / 16;             // warps of a column group
-  const int rg = warp % RG, cg = warp / RG;
-  const int gtid = rg * 32 + lane;        // thread of the column group
-  const uint32_t bbuf = raw_u + cg * 2 * 64 * ((a.R + 63) / 64 * 128);
-  const int bstage = 64 * ((a.R + 63) / 64 * 128);
-  const int row0 = tile_rows[rg * 16 + g], row1 = tile_rows[rg * 16 + g + 8];
-  // thread t of the group copies piece t % 8 of columns t / 8, t / 8 + RG * 4, ...
-  const int bpiece = gtid & 7, bfirst = gtid >> 3;
-  const int kp16 = (rp + 15) / 16 * 16;   // whole 16-wide steps; what lies past the rank is zero
-  auto load_b = [&](int block, int st) {
-    const Block at = column_block<64>(a, block);
+  const int bstage = kBN * ((a.R + 63) / 64 * 128);
+  const int piece = tid & 7, cfirst = tid >> 3;
+  auto load_b = [&](const Block& at, int st) {
     if (at.slice >= 0) {
 #pragma unroll
-      for (int col = bfirst; col < 64; col += RG * 4) {
-        // column q * 8 + 2 t + e of a 32-column half is stored as row t * 8 + 2 q + e
-        const int lc = col & 31;
-        const int r = (col & 32) + (lc >> 1 & 3) * 8 + (lc >> 3) * 2 + (lc & 1);
-        const uint32_t dst = bbuf + st * bstage + r * 128 + ((bpiece ^ (r & 7)) << 4);
-        const __nv_bfloat16* src = B + (int64_t)(at.c0 + col) * a.R;
-        const bool in = at.c0 + col < at.end;
-        for (int kb = 0; kb < kp16; kb += 64) {
-          const int k = kb + bpiece * 8;
-          const bool on = in && k < rank;
-          if (k < kp16) cp_async16(dst + kb * 128, on ? src + k : B, on);
+      for (int i = 0; i < kBN / 32; ++i) {
+        // column q * 8 + 2 t + e of 32 is stored as row t * 8 + 2 q + e
+        const int lc = cfirst, r = i * 32 + (lc >> 1 & 3) * 8 + (lc >> 3) * 2 + (lc & 1);
+        const uint32_t dst = raw_u + st * bstage + r * 128 + ((piece ^ (r & 7)) << 4);
+        const int col = at.c0 + i * 32 + lc;
+        const __nv_bfloat16* src = B + (int64_t)col * a.R;
+        for (int kb = 0; kb < rp; kb += 64) {
+          const int k = kb + piece * 8;
+          const bool on = col < at.end && k < rank;
+          if (k < rp) cp_async16(dst + kb * (kBN * 2), on ? src + k : B, on);
         }
       }
     }
     cp_async_commit();
   };
-  constexpr int kStep = CL * NCG;
-  int block = cta * NCG + cg;
-  load_b(block, 0);
+  // past the rank nothing counts, not even a NaN: the piece the rank ends in
+  auto trim_b = [&](int st) {
+    if ((rank & 7) == 0 || piece != (rank >> 3 & 7)) return;
+#pragma unroll
+    for (int i = 0; i < kBN / 32; ++i) {
+      const int lc = cfirst, r = i * 32 + (lc >> 1 & 3) * 8 + (lc >> 3) * 2 + (lc & 1);
+      uint16_t* p = reinterpret_cast<uint16_t*>(raw + st * bstage + (rank >> 6) * (kBN * 128) + r * 128 + ((piece ^ (r & 7)) << 4));
+      for (int e = rank & 7; e < 8; ++e) p[e] = 0;
+    }
+  };
+  const int row0 = tile_rows[sub * 16 + g], row1 = tile_rows[sub * 16 + g + 8];
   const int es = F32 ? 4 : 2;
-  const char* base0 = reinterpret_cast<const char*>(a.base) + ((int64_t)row0 * a.ldb + 8 * c) * es;   // used where the row exists
-  const char* base1 = reinterpret_cast<const char*>(a.base) + ((int64_t)row1 * a.ldb + 8 * c) * es;
-  char* out0 = reinterpret_cast<char*>(a.out) + ((int64_t)row0 * a.ldo + 8 * c) * es;
-  char* out1 = reinterpret_cast<char*>(a.out) + ((int64_t)row1 * a.ldo + 8 * c) * es;
-  Block at = column_block<64>(a, block);
-  for (int it = 0; at.slice >= 0; ++it, block += kStep, at = column_block<64>(a, block)) {
-    load_b(block + kStep, (it + 1) & 1);
-    const int slice = at.slice, c0 = at.c0, end = at.end;
+  // used where the row exists
+  const char* base0 = reinterpret_cast<const char*>(a.base) + ((int64_t)row0 * a.ldb + half * 64 + 8 * c) * es;
+  const char* base1 = reinterpret_cast<const char*>(a.base) + ((int64_t)row1 * a.ldb + half * 64 + 8 * c) * es;
+  char* out0 = reinterpret_cast<char*>(a.out) + ((int64_t)row0 * a.ldo + half * 64 + 8 * c) * es;
+  char* out1 = reinterpret_cast<char*>(a.out) + ((int64_t)row1 * a.ldo + half * 64 + 8 * c) * es;
+  const uint32_t idesc = idesc_bf16_f32(TML, kBN);
+  const uint32_t hs_u = smem_u32(hs);
+  int block = cta;
+  Block at = column_block<kBN>(a, block);
+  load_b(at, 0);
+  for (int it = 0; at.slice >= 0; ++it) {
+    const Block next = column_block<kBN>(a, block + CL);
+    load_b(next, (it + 1) & 1);           // that stage's product was waited for
     BaseCols<F32> bs[2][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int col = c0 + h * 32 + 8 * c;
-      if (col < end) {
-        if (row0 >= 0) bs[h][0].load(base0 + (int64_t)(c0 + h * 32) * es);
-        if (row1 >= 0) bs[h][1].load(base1 + (int64_t)(c0 + h * 32) * es);
+      if (at.c0 + half * 64 + h * 32 + 8 * c < at.end) {
+        if (row0 >= 0) bs[h][0].load(base0 + (int64_t)(at.c0 + h * 32) * es);
+        if (row1 >= 0) bs[h][1].load(base1 + (int64_t)(at.c0 + h * 32) * es);
       }
     }
     cp_async_wait<1>();
-    bar_sync(1 + cg, RG * 32);
-    float acc[8][4];
-#pragma unroll
-    for (int t = 0; t < 8; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-    const uint32_t bst = bbuf + (it & 1) * bstage;
-    for (int k = 0; k < rp; k += 16) {
-      uint32_t h[kParts][4];
-#pragma unroll
+    trim_b(it & 1);
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    const uint32_t acc_col = (it & 1) * kBN;
+    if (warp == 0 && elect_one()) {
+      tc_fence_after();
+      const uint32_t bst = raw_u + (it & 1) * bstage;
+      uint32_t on = 0;
       for (int q = 0; q < kParts; ++q)
-        ldsm_x4(smem_u32(hs + (q * TM + rg * 16 + (lane & 15)) * hld + slice * rp + k + (lane >> 4) * 8), h[q]);
-      // a last step of eight: the upper half of h belongs to the next slice
-      if (k + 8 >= rp) {
-#pragma unroll
-        for (int q = 0; q < kParts; ++q) h[q][2] = h[q][3] = 0u;
-      }
-#pragma unroll
-      for (int t = 0; t < 8; t += 2) {
-        const int r = (t + (lane >> 4)) * 8 + (lane & 7);
-        uint32_t b[4];
-        ldsm_x4(bst + (k >> 6) * 8192 + r * 128 + (((((k & 63) >> 3) + (lane >> 3 & 1)) ^ (r & 7)) << 4), b);
-        if (k + 16 > rank) {              // past the rank nothing counts, not even a NaN
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int kk = k + (e & 1) * 8 + 2 * c;
-            if (kk >= rank) b[e] = 0u;
-            else if (kk + 1 >= rank) b[e] &= 0xffffu;
-          }
+        for (int k = 0; k < rp; k += 16) {
+          const int hc = at.slice * rp + k;
+          const uint64_t hd = sw128_kmajor_desc(hs_u + q * hpart + (hc >> 6) * (TML * 128)) + ((hc & 63) >> 3);
+          const uint64_t bd = sw128_kmajor_desc(bst + (k >> 6) * (kBN * 128)) + ((k & 63) >> 3);
+          umma_f16_ss(tmem + acc_col, hd, bd, idesc, on);
+          on = 1;
         }
-#pragma unroll
-        for (int q = 0; q < kParts; ++q) {
-          mma_bf16(acc[t], h[q][0], h[q][1], h[q][2], h[q][3], b[0], b[1]);
-          mma_bf16(acc[t + 1], h[q][0], h[q][1], h[q][2], h[q][3], b[2], b[3]);
-        }
-      }
+      umma_commit(&done[it & 1]);
     }
+    __syncwarp();
+    mbar_wait(&done[it & 1], (it >> 1) & 1, 42);
+    __syncwarp();
+    tc_fence_after();
+    uint32_t acc[32];
+    tmem_ld_16x256b_x8(tmem_row + acc_col + half * 64, acc);
+    tmem_wait_ld();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int col = c0 + h * 32 + 8 * c;
-      if (col >= end) continue;
+      if (at.c0 + half * 64 + h * 32 + 8 * c >= at.end) continue;
+      const int64_t off = (int64_t)(at.c0 + h * 32) * es;
+      float d[8];
+      if (row0 >= 0) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int row = u ? row1 : row0;
-        if (row < 0) continue;
-        float d[8];
+        for (int t = 0; t < 4; ++t)
+          d[2 * t] = rp ? __uint_as_float(acc[(h * 4 + t) * 4]) : 0.f, d[2 * t + 1] = rp ? __uint_as_float(acc[(h * 4 + t) * 4 + 1]) : 0.f;
+        bs[h][0].store(out0 + off, d, tl.scale);
+      }
+      if (row1 >= 0) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) d[2 * t] = acc[h * 4 + t][2 * u], d[2 * t + 1] = acc[h * 4 + t][2 * u + 1];
-        bs[h][u].store((u ? out1 : out0) + (int64_t)(c0 + h * 32) * es, d, tl.scale);
+        for (int t = 0; t < 4; ++t)
+          d[2 * t] = rp ? __uint_as_float(acc[(h * 4 + t) * 4 + 2]) : 0.f, d[2 * t + 1] = rp ? __uint_as_float(acc[(h * 4 + t) * 4 + 3]) : 0.f;
+        bs[h][1].store(out1 + off, d, tl.scale);
       }
     }
-    bar_sync(1 + cg, RG * 32);            // the stage is free for the block after the next
+    at = next;
+    block += CL;
   }
   cp_async_wait<0>();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, kTmemCols);
 }
 
 void raise_smem(const void* k, size_t smem) {
   if (smem <= 48 * 1024) return;
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) launch_failed(e);
+}
+
+void set_blocks(LoraArgs& a) {
+  a.block32[0] = a.block128[0] = 0;
+  for (int i = 0; i < kMaxSlices; ++i) {
+    const int width = i < a.S ? a.col_begin[i + 1] - a.col_begin[i] : 0;
+    a.block32[i + 1] = a.block32[i] + (width + 31) / 32;
+    a.block128[i + 1] = a.block128[i] + (width + 127) / 128;
+  }
 }
 
 int cta_slots() {   // two CTAs per SM
@@ -858,35 +890,29 @@ void small(const LoraArgs& a, cudaStream_t s) {
   }
 }
 
-template <bool F32, int TM, int NTW, int CL>
-void launch_large_cl(const LoraArgs& a, int tiles, cudaStream_t s) {
-  const int cols = (a.S * a.R + 15) / 16 * 16;
-  const LargeSmem sm = large_smem<TM>(cols, a.R, F32 ? 3 : 2);
-  auto k = lora_large_kernel<F32, TM, NTW, CL>;
+template <bool F32, int CL>
+void launch_large(const LoraArgs& a, int tiles, cudaStream_t s) {
+  const int cols = a.S * ((a.R + 15) / 16 * 16);
+  const LargeSmem sm = large_smem(cols, a.R, F32 ? 3 : 2);
+  auto k = lora_large_kernel<F32, CL>;
   raise_smem(reinterpret_cast<const void*>(k), sm.total);
   launch_k(k, dim3((unsigned)tiles * CL), dim3(kThreads), sm.total, s, (unsigned)CL, a, cols, (int)sm.hs);
 }
 
-template <bool F32, int TM, int NTW>
-void launch_large(const LoraArgs& a, cudaStream_t s) {
-  const int tiles = a.L / TM + std::min(a.L, a.pool);
-  if ((int64_t)tiles * kCluster <= cta_slots()) launch_large_cl<F32, TM, NTW, kCluster>(a, tiles, s);
-  else launch_large_cl<F32, TM, NTW, 4>(a, tiles, s);
-}
-
-// Four fp32 slices of rank 128 leave no room for a large tile's parts of h.
-bool large_fits(const LoraArgs& a) {
-  const int cols = (a.S * a.R + 15) / 16 * 16;
-  return cols <= 256 || large_smem<32>(cols, a.R, a.f32 ? 3 : 2).total <= 226 * 1024;
-}
-
+// As many slices per launch as an accumulator holds: all of them up to 256 columns.
 template <bool F32>
-void large(const LoraArgs& a, cudaStream_t s) {
-  const int cols = a.S * a.R;
-  if (cols <= 64) launch_large<F32, 64, 2>(a, s);
-  else if (cols <= 192) launch_large<F32, 64, 6>(a, s);
-  else if (cols <= 256) launch_large<F32, 64, 8>(a, s);
-  else launch_large<F32, 32, 8>(a, s);
+void large(const LoraArgs& all, cudaStream_t s) {
+  const int step = kLargeCols / ((all.R + 15) / 16 * 16);
+  const int tiles = all.L / TML + std::min(all.L, all.pool);
+  for (int s0 = 0; s0 < all.S; s0 += step) {
+    LoraArgs a = all;
+    a.s0 = s0;
+    a.S = std::min(step, all.S - s0);
+    for (int i = 0; i <= kMaxSlices; ++i) a.col_begin[i] = all.col_begin[std::min(s0 + std::min(i, a.S), all.S)];
+    set_blocks(a);
+    if ((int64_t)tiles * kCluster <= cta_slots()) launch_large<F32, kCluster>(a, tiles, s);
+    else launch_large<F32, 4>(a, tiles, s);
+  }
 }
 
 }  // namespace
@@ -894,15 +920,11 @@ void large(const LoraArgs& a, cudaStream_t s) {
 void lora_add(const LoraArgs& args, cudaStream_t s) {
   if (args.L <= 0 || args.N <= 0 || args.pool <= 0) return;
   LoraArgs a = args;
-  a.block32[0] = a.block64[0] = 0;
-  for (int i = 0; i < kMaxSlices; ++i) {
-    const int width = i < a.S ? a.col_begin[i + 1] - a.col_begin[i] : 0;
-    a.block32[i + 1] = a.block32[i] + (width + 31) / 32;
-    a.block64[i + 1] = a.block64[i] + (width + 63) / 64;
-  }
-  const bool big = a.L >= kLargeRows && large_fits(a);
-  if (a.f32) big ? large<true>(a, s) : small<true>(a, s);
-  else big ? large<false>(a, s) : small<false>(a, s);
+  a.s0 = 0;
+  a.S_all = a.S;
+  set_blocks(a);
+  if (a.L >= kLargeRows) a.f32 ? large<true>(a, s) : large<false>(a, s);
+  else a.f32 ? small<true>(a, s) : small<false>(a, s);
 }
 
 }  // namespace lora

@@ -23,8 +23,11 @@ struct LoraArgs {
   int64_t ldo;
   int T, K, N, R, pool, L, S;
   int col_begin[kMaxSlices + 1];   // first column of every slice, then N
-  int block32[kMaxSlices + 1];     // blocks of 32 / 64 columns before every slice (set at the launch)
-  int block64[kMaxSlices + 1];
+  // set at the launch: first slice and slices of lora_a (a launch may take some of
+  // them), blocks of 32 / 128 columns before every slice
+  int s0, S_all;
+  int block32[kMaxSlices + 1];
+  int block128[kMaxSlices + 1];
   bool f32;                   // base and out are fp32
 };
 
