@@ -707,22 +707,34 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
       part_at[q] = cluster_addr(part + cta * kOwn * pld, q);
       hs_at[q] = cluster_addr(hs, q);
     }
-    const int quads = cols / 4;
-    for (int i = tid; i < kOwn * quads; i += kThreads) {
-      const int row = i / quads, j = (i - row * quads) * 4;
-      float4 v[CL];
+    const int quads = cols / 4, items = kOwn * quads;
+    constexpr int kIn = 16 / CL;          // items whose remote loads are under way together
+    for (int i0 = tid; i0 < items; i0 += kIn * kThreads) {
+      float4 v[kIn][CL];
+      int row[kIn], j[kIn];
 #pragma unroll
-      for (int q = 0; q < CL; ++q) v[q] = ld_cluster4(part_at[q] + (row * pld + j) * 4);
+      for (int u = 0; u < kIn; ++u) {
+        const int i = min(i0 + u * kThreads, items - 1);
+        row[u] = i / quads;
+        j[u] = (i - row[u] * quads) * 4;
 #pragma unroll
-      for (int q = 1; q < CL; ++q) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
-      uint2 p[kParts];
-      split4<kParts>(v[0], p);
-      const int hr = cta * kOwn + row;
-      const uint32_t off = (j >> 6) * (TML * 128) + hr * 128 + (((j & 63) >> 3 ^ (hr & 7)) << 4) + (j & 7) * 2;
+        for (int q = 0; q < CL; ++q) v[u][q] = ld_cluster4(part_at[q] + (row[u] * pld + j[u]) * 4);
+      }
 #pragma unroll
-      for (int q = 0; q < CL; ++q)
+      for (int u = 0; u < kIn; ++u) {
+        if (i0 + u * kThreads >= items) break;
 #pragma unroll
-        for (int s = 0; s < kParts; ++s) st_cluster2(hs_at[q] + s * hpart + off, p[s]);
+        for (int q = 1; q < CL; ++q)
+          v[u][0].x += v[u][q].x, v[u][0].y += v[u][q].y, v[u][0].z += v[u][q].z, v[u][0].w += v[u][q].w;
+        uint2 p[kParts];
+        split4<kParts>(v[u][0], p);
+        const int hr = cta * kOwn + row[u];
+        const uint32_t off = (j[u] >> 6) * (TML * 128) + hr * 128 + (((j[u] & 63) >> 3 ^ (hr & 7)) << 4) + (j[u] & 7) * 2;
+#pragma unroll
+        for (int q = 0; q < CL; ++q)
+#pragma unroll
+          for (int s = 0; s < kParts; ++s) st_cluster2(hs_at[q] + s * hpart + off, p[s]);
+      }
     }
   }
   asm volatile("fence.proxy.async;" ::: "memory");   // the tensor cores will read what was just stored
@@ -771,13 +783,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
   char* out1 = reinterpret_cast<char*>(a.out) + ((int64_t)row1 * a.ldo + half * 64 + 8 * c) * es;
   const uint32_t idesc = idesc_bf16_f32(TML, kBN);
   const uint32_t hs_u = smem_u32(hs);
-  int block = cta;
-  Block at = column_block<kBN>(a, block);
-  load_b(at, 0);
-  for (int it = 0; at.slice >= 0; ++it) {
-    const Block next = column_block<kBN>(a, block + CL);
-    load_b(next, (it + 1) & 1);           // that stage's product was waited for
-    BaseCols<F32> bs[2][2];
+  auto load_base = [&](const Block& at, BaseCols<F32> (&bs)[2][2]) {
+    if (at.slice < 0) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (at.c0 + half * 64 + h * 32 + 8 * c < at.end) {
@@ -785,12 +792,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
         if (row1 >= 0) bs[h][1].load(base1 + (int64_t)(at.c0 + h * 32) * es);
       }
     }
-    cp_async_wait<1>();
+  };
+  // block `it` has been copied by every thread: its product into accumulator it % 2
+  auto multiply = [&](const Block& at, int it) {
     trim_b(it & 1);
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
-    const uint32_t acc_col = (it & 1) * kBN;
     if (warp == 0 && elect_one()) {
       tc_fence_after();
       const uint32_t bst = raw_u + (it & 1) * bstage;
@@ -800,17 +808,39 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
           const int hc = at.slice * rp + k;
           const uint64_t hd = sw128_kmajor_desc(hs_u + q * hpart + (hc >> 6) * (TML * 128)) + ((hc & 63) >> 3);
           const uint64_t bd = sw128_kmajor_desc(bst + (k >> 6) * (kBN * 128)) + ((k & 63) >> 3);
-          umma_f16_ss(tmem + acc_col, hd, bd, idesc, on);
+          umma_f16_ss(tmem + (it & 1) * kBN, hd, bd, idesc, on);
           on = 1;
         }
       umma_commit(&done[it & 1]);
     }
     __syncwarp();
+  };
+  // While block `it` is added to base and written, the product of the next one runs
+  // and the copy of the one after it is under way.
+  int block = cta;
+  Block at = column_block<kBN>(a, block), next = column_block<kBN>(a, block + CL);
+  BaseCols<F32> bs[2][2], bs_next[2][2];
+  load_b(at, 0);
+  load_b(next, 1);
+  load_base(at, bs);
+  if (at.slice >= 0) {
+    cp_async_wait<1>();
+    multiply(at, 0);
+  }
+  for (int it = 0; at.slice >= 0; ++it) {
+    load_base(next, bs_next);
+    if (next.slice >= 0) {
+      cp_async_wait<0>();
+      multiply(next, it + 1);             // its accumulator was read before this barrier
+    }
     mbar_wait(&done[it & 1], (it >> 1) & 1, 42);
     __syncwarp();
     tc_fence_after();
+    block += CL;
+    const Block after = column_block<kBN>(a, block + CL);
+    load_b(after, it & 1);                // block `it` has been multiplied: its stage is free
     uint32_t acc[32];
-    tmem_ld_16x256b_x8(tmem_row + acc_col + half * 64, acc);
+    tmem_ld_16x256b_x8(tmem_row + (it & 1) * kBN + half * 64, acc);
     tmem_wait_ld();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -831,7 +861,9 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
       }
     }
     at = next;
-    block += CL;
+    next = after;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) bs[h][0] = bs_next[h][0], bs[h][1] = bs_next[h][1];
   }
   cp_async_wait<0>();
   tc_fence_before();
