@@ -943,7 +943,8 @@ void large(const LoraArgs& all, cudaStream_t s) {
     for (int i = 0; i <= kMaxSlices; ++i) a.col_begin[i] = all.col_begin[std::min(s0 + std::min(i, a.S), all.S)];
     set_blocks(a);
     if ((int64_t)tiles * kCluster <= cta_slots()) launch_large<F32, kCluster>(a, tiles, s);
-    else launch_large<F32, 4>(a, tiles, s);
+    else if ((int64_t)tiles * 4 <= cta_slots()) launch_large<F32, 4>(a, tiles, s);
+    else launch_large<F32, 2>(a, tiles, s);
   }
 }
 
