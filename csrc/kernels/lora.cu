@@ -80,6 +80,11 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
   return addr;
 }
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
@@ -237,8 +242,171 @@ constexpr int small_items() {   // items under way
 
 // WIDE: R is a multiple of 32, a lane reads 8 consecutive k of a column (two
 // k-steps); else 4 (one k-step).
+// Streaming 16-byte load (no line kept in L1).
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// Tiles of one row, the usual ones where every request has its own adapter:
+// products of the weights with a vector, on the fp32 units.  A warp reads 512
+// consecutive bytes of one A row at a time (eight rows under way) against x in
+// shared memory, so its sums need no other warp; R / 8 lanes read one column of B.
+// R is a power of two.  The loops are kept short: a CTA runs each once or a few
+// times, and longer ones would wait for their instructions.
+__device__ __forceinline__ float dot8(const uint4& v, const float4& x0, const float4& x1, float acc) {
+  acc += __uint_as_float(v.x << 16) * x0.x;
+  acc += __uint_as_float(v.x & 0xffff0000u) * x0.y;
+  acc += __uint_as_float(v.y << 16) * x0.z;
+  acc += __uint_as_float(v.y & 0xffff0000u) * x0.w;
+  acc += __uint_as_float(v.z << 16) * x1.x;
+  acc += __uint_as_float(v.z & 0xffff0000u) * x1.y;
+  acc += __uint_as_float(v.w << 16) * x1.z;
+  acc += __uint_as_float(v.w & 0xffff0000u) * x1.w;
+  return acc;
+}
+
+template <bool F32>
+__device__ __forceinline__ void one_row(const LoraArgs& a, const Tile& tl, int row, int cl, int cta, uint8_t* raw) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = tl.rank, rp = (rank + 7) / 8 * 8, cols = a.S * rp;
+  const int kblocks = (a.K + 31) / 32, per_cta = (kblocks + cl - 1) / cl;
+  const int kbeg = cta * per_cta * 32, kend = min(a.K, kbeg + per_cta * 32);
+  const int span = (per_cta * 32 + 255) / 256 * 256;             // whole steps of a warp
+  float* xs = reinterpret_cast<float*>(raw);                     // [span]
+  float* part = xs + span;                                       // [cols], this CTA's share of K
+  float* h = part + cols;                                        // [cols]
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+
+  for (int i = tid * 8; i < span; i += kThreads * 8) {
+    const uint4 v = kbeg + i < kend && row >= 0
+                        ? *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.x) + (int64_t)row * a.ldx + kbeg + i)
+                        : zero;
+    float4* d = reinterpret_cast<float4*>(xs + i);
+    d[0] = make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+    d[1] = make_float4(__uint_as_float(v.z << 16), __uint_as_float(v.z & 0xffff0000u), __uint_as_float(v.w << 16), __uint_as_float(v.w & 0xffff0000u));
+  }
+  __syncthreads();
+
+  // h: warp w takes compact columns w, w + 8, ...
+  const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) + (int64_t)tl.adapter * a.S * a.R * a.K + kbeg + lane * 8;
+#pragma unroll 1
+  for (int jg = warp; jg < cols; jg += 8 * kWarps) {
+    const __nv_bfloat16* ap[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int j = jg + u * kWarps, s = j / rp, i = j - s * rp;
+      ap[u] = j < cols && i < rank ? A + (int64_t)(s * a.R + i) * a.K : nullptr;
+    }
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int c = 0; c < span; c += 256) {
+      const bool in = kbeg + c + lane * 8 < kend;
+      uint4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = in && ap[u] != nullptr ? ld_stream(ap[u] + c) : zero;
+      const float4 x0 = *reinterpret_cast<const float4*>(xs + c + lane * 8), x1 = *reinterpret_cast<const float4*>(xs + c + lane * 8 + 4);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) acc[u] = dot8(v[u], x0, x1, acc[u]);
+    }
+    // eight sums over the warp: the lanes halve the set of sums they hold three times
+#pragma unroll
+    for (int o = 16, n = 4; o >= 4; o >>= 1, n >>= 1) {
+      const bool up = lane & o;
+#pragma unroll
+      for (int u = 0; u < n; ++u) {
+        const float keep = up ? acc[u + n] : acc[u], give = up ? acc[u] : acc[u + n];
+        acc[u] = keep + __shfl_xor_sync(kFull, give, o);
+      }
+    }
+    acc[0] += __shfl_xor_sync(kFull, acc[0], 2);
+    acc[0] += __shfl_xor_sync(kFull, acc[0], 1);
+    const int j = jg + ((lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1)) * kWarps;
+    if ((lane & 3) == 0 && j < cols) part[j] = acc[0];
+  }
+
+  // B and base of this warp's next four steps
+  constexpr int NB = 4;
+  const int per_col = a.R / 8, piece = lane & (per_col - 1), k = piece * 8;   // lanes of a column
+  const int cstep = 32 / per_col;         // columns of a step
+  const int share = ((a.N + cl - 1) / cl + 31) / 32 * 32;
+  const int c_lo = cta * share, c_hi = min(a.N, c_lo + share);
+  const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b) + (int64_t)tl.adapter * a.N * a.R + k;
+  const int64_t base_row = (int64_t)(row >= 0 ? row : 0) * a.ldb, out_row = (int64_t)(row >= 0 ? row : 0) * a.ldo;
+  uint4 bv[NB];
+  float bs[NB];
+  auto fetch = [&](int col0) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int col = col0 + i * (kWarps * cstep);
+      bv[i] = col < c_hi && k < rank ? ld_stream(B + (int64_t)col * a.R) : zero;
+      bs[i] = 0.f;
+      if (col < c_hi && piece == 0)
+        bs[i] = F32 ? reinterpret_cast<const float*>(a.base)[base_row + col]
+                    : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.base)[base_row + col]);
+    }
+  };
+  int col0 = c_lo + warp * cstep + lane / per_col;
+  fetch(col0);
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  for (int i = tid; i < cols; i += kThreads) {
+    float v[kCluster], sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < kCluster; ++q) v[q] = q < cl ? ld_cluster(cluster_addr(part + i, q)) : 0.f;
+#pragma unroll
+    for (int q = 0; q < kCluster; ++q) sum += v[q];
+    h[i] = sum;
+  }
+  cluster_arrive();                       // this CTA has read the others' partials
+  __syncthreads();
+#pragma unroll 1
+  for (; col0 - lane / per_col < c_hi; col0 += NB * kWarps * cstep) {
+    float d[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int col = col0 + i * (kWarps * cstep);
+      const int s = (a.S > 1 && col >= a.col_begin[1]) + (a.S > 2 && col >= a.col_begin[2]) + (a.S > 3 && col >= a.col_begin[3]);
+      d[i] = 0.f;
+      if (k < rank && col < c_hi) {
+        uint4 v = bv[i];
+        if (k + 8 > rank) {               // past the rank nothing counts, not even a NaN
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (k + 2 * e >= rank) w[e] = 0u;
+            else if (k + 2 * e + 1 >= rank) w[e] &= 0xffffu;
+          }
+          v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        const float4* hr = reinterpret_cast<const float4*>(h + s * rp + k);
+        d[i] = dot8(v, hr[0], hr[1], 0.f);
+      }
+    }
+    for (int o = per_col >> 1; o > 0; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) d[i] += __shfl_xor_sync(kFull, d[i], o);
+    }
+    if (piece == 0 && row >= 0) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int col = col0 + i * (kWarps * cstep);
+        if (col >= c_hi) continue;
+        if (F32) reinterpret_cast<float*>(a.out)[out_row + col] = bs[i] + tl.scale * d[i];
+        else reinterpret_cast<__nv_bfloat16*>(a.out)[out_row + col] = __float2bfloat16(bs[i] + tl.scale * d[i]);
+      }
+    }
+    fetch(col0 + NB * kWarps * cstep);
+  }
+  cluster_wait();                         // no CTA leaves while another reads its partial h
+}
+
 template <bool F32, int MT, bool WIDE>
-__global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs a, int cols_max, int cl) {
+__global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs a, int cols_max, int cl, bool vector) {
   constexpr int TM = kSmallRows;
   constexpr int kParts = F32 ? 3 : 2;
   constexpr int ST = small_stages<MT>();
@@ -254,6 +422,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
   const Tile tl = find_tile<TM>(a, blockIdx.x / cl);
   if (tl.adapter < 0) return;             // the whole cluster
   const int my_row = lane < TM ? tile_row(a, tl, lane) : -1;
+  if (vector && tl.valid == 1) {
+    one_row<F32>(a, tl, __shfl_sync(kFull, my_row, 0), cl, cta, raw);
+    return;
+  }
   const int rank = tl.rank;
   const int rb = (rank + 7) / 8;          // 8-row blocks of A per slice
   const int rp = rb * 8;
@@ -906,7 +1078,10 @@ void launch_small(const LoraArgs& a, cudaStream_t s) {
   const int64_t bytes = 2 * (int64_t)a.R * ((int64_t)a.S * a.K + a.N);
   int cl = kCluster;
   while (cl > 1 && (int64_t)tiles * cl > cta_slots() && bytes / cl < 128 * 1024) cl /= 2;
-  launch_k(k, dim3((unsigned)(tiles * cl)), dim3(kThreads), smem, s, (unsigned)cl, a, cols, cl);
+  // one_row() keeps its share of x and h in the same shared memory
+  const int64_t span = (((a.K + 31) / 32 + cl - 1) / cl * 32 + 255) / 256 * 256;
+  const bool vector = (a.R & (a.R - 1)) == 0 && (span + 2 * cols) * 4 <= (int64_t)smem;
+  launch_k(k, dim3((unsigned)(tiles * cl)), dim3(kThreads), smem, s, (unsigned)cl, a, cols, cl, vector);
 }
 
 template <bool F32>
