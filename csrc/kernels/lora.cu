@@ -328,8 +328,8 @@ __device__ __forceinline__ void one_row(const LoraArgs& a, const Tile& tl, int r
     if ((lane & 3) == 0 && j < cols) part[j] = acc[0];
   }
 
-  // B and base of this warp's next four steps
-  constexpr int NB = 4;
+  // B and base of this warp's next six steps
+  constexpr int NB = 6;
   const int per_col = a.R / 8, piece = lane & (per_col - 1), k = piece * 8;   // lanes of a column
   const int cstep = 32 / per_col;         // columns of a step
   const int share = ((a.N + cl - 1) / cl + 31) / 32 * 32;
