@@ -42,6 +42,9 @@ class EngineOptions:
     overlap_steps: bool = False            # plan and launch step n+1 before step n's tokens reach the host
     tp_sample_candidates: bool = False     # TP stochastic sampling from per-shard top-k candidates (top_k <= 64)
     moe_all_to_all: bool = False           # with sequence parallelism: experts by dispatch / combine all-to-all
+    sparse_pages: int = 0                  # decode attends to at most this many pages per KV head (0: all of them)
+    sparse_first: int = 1                  # of these, the row's first pages ...
+    sparse_last: int = 2                   # ... and its last ones are always taken, the others by score
 
 
 @dataclasses.dataclass
@@ -91,7 +94,9 @@ class LLMEngine:
                                   sched.max_rows_per_step, opts.max_context, P, opts.graph_sizes, comm=comm,
                                   check_errors_every=opts.check_errors_every,
                                   sequence_parallel=opts.sequence_parallel, overlap=opts.overlap_steps,
-                                  sample_candidates=opts.tp_sample_candidates, moe_all_to_all=opts.moe_all_to_all)
+                                  sample_candidates=opts.tp_sample_candidates, moe_all_to_all=opts.moe_all_to_all,
+                                  sparse_pages=opts.sparse_pages, sparse_first=opts.sparse_first,
+                                  sparse_last=opts.sparse_last)
         if opts.overlap_steps:
             self.scheduler.max_inflight = 2
         self._launched: List[tuple] = []       # (plan, runner handle, t0), oldest first
@@ -104,6 +109,8 @@ class LLMEngine:
     def _pages_from_memory(self, weights, cache, sched, opts) -> int:
         per_page = kv_bytes_per_page(self.spec, weights.shard.kv_heads, cache.tokens_per_page,
                                      weights.embed.element_size())
+        if opts.sparse_pages:
+            per_page += per_page // cache.tokens_per_page     # two bounds per page, for two per token
         want = sched.max_active_requests * -(-opts.max_context // cache.tokens_per_page) + 64
         if self.device.type != "cuda":
             return want

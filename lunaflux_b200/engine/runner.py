@@ -62,7 +62,8 @@ class ModelRunner:
     def __init__(self, weights: ModelWeights, ops, device, num_pages: int, max_tokens: int, max_rows: int,
                  max_context: int, page: int = 16, graph_sizes: Sequence[int] = (), comm=None,
                  check_errors_every: int = 16, sequence_parallel: bool = False, overlap: bool = False,
-                 sample_candidates: bool = False, moe_all_to_all: bool = False):
+                 sample_candidates: bool = False, moe_all_to_all: bool = False, sparse_pages: int = 0,
+                 sparse_first: int = 1, sparse_last: int = 2):
         self.w = weights
         self.spec: LlamaSpec = weights.spec
         self.shard = weights.shard
@@ -88,6 +89,19 @@ class ModelRunner:
         self.kv = torch.zeros(s.layers, 2, self.num_pages, self.Hkv, page, self.D, dtype=dt, device=dev)
         self.cos_sin = rope_table(s.max_position, s.head_dim, s.rope_theta, dev, s.rope_scaling)
         T, R = max_tokens, max_rows
+        # Decode attention over selected pages: key bounds of every page beside
+        # the KV arena, kept in step with it (they move with the page: a shared
+        # prefix page carries its own), the selection of a step and its scores.
+        self.sparse = (int(sparse_pages), int(sparse_first), int(sparse_last)) if sparse_pages else None
+        if self.sparse:
+            if not hasattr(ops, "attn_select"):
+                raise ValueError("this operator set has no attention over selected pages")
+            if min(self.sparse) < 0 or sparse_first + sparse_last > sparse_pages or page != 16:
+                raise ValueError("sparse_pages must hold the first and the last pages, of 16 tokens")
+            self.bounds = torch.zeros(s.layers, self.num_pages, self.Hkv, 2, self.D, dtype=dt, device=dev)
+            self.sel = torch.full((R, self.Hkv, sparse_pages), -1, dtype=torch.int32, device=dev)
+            self.sel_ws = torch.empty(ops.select_workspace(R, self.Hkv, self.W), dtype=torch.float32, device=dev)
+            self.new_from = torch.zeros(2 * R, dtype=torch.int32, device=dev)   # first new token of prefill, decode rows
         self.resid = torch.empty(T, H, dtype=dt, device=dev)
         self.h = torch.empty(T, H, dtype=dt, device=dev)
         self.delta = torch.empty(T, H, dtype=dt, device=dev)
@@ -195,6 +209,12 @@ class ModelRunner:
         # decode rows whose input token was sampled by the previous step (not
         # yet on the host) take it from that step's output inside the embedding
         self._embed_fwd = (v["d_fwd"][:Rd], Tp, self.prev_tok) if self.overlap and Rd else None
+        if self.sparse:
+            if Rp:
+                qs = v["p_qstart"]
+                torch.sub(v["p_seqlen"][:Rp], qs[1:Rp + 1] - qs[:Rp], out=self.new_from[:Rp])
+            if Rd:
+                torch.sub(v["d_seqlen"][:Rd], 1, out=self.new_from[self.max_rows:self.max_rows + Rd])
         if self.sp:
             out = self.forward_sp(v, T, Tp, Rp, Rd, Rs, max_q_len, splits, stochastic, host_meta, gather)
         else:
@@ -288,10 +308,21 @@ class ModelRunner:
         if not fused:
             self._proj(h, lw, "wqkv", qkv, 0)
             ops.rope_kv_write(qkv, v["positions"], v["slots"], self.cos_sin, kc, vc, Hq, Hkv, self.P)
+        if self.sparse:
+            bounds, dec = self.bounds[l], self.new_from[self.max_rows:]
+            if Rp:
+                ops.page_bounds(kc, bounds, v["p_bt"], self.new_from[:Rp], v["p_seqlen"], max_q_len)
+            if Rd:
+                ops.page_bounds(kc, bounds, v["d_bt"], dec[:Rd], v["d_seqlen"], 1)
         if Rp:
             ops.attn_prefill(qkv[:Tp], attn[:Tp], v["p_qstart"], v["p_seqlen"], v["p_bt"], kc, vc, Hq, Hkv,
                              max_q_len, host={"q_start": hm.get("q_start"), "seq_lens": hm.get("seq_lens")})
-        if Rd:
+        if Rd and self.sparse:
+            sel = self.sel[:Rd]
+            ops.attn_select(qkv, v["d_tok"], v["d_seqlen"], v["d_bt"], bounds, sel, self.sparse[1], self.sparse[2],
+                            Hq, Hkv, self.sel_ws)
+            ops.attn_decode_sparse(qkv, attn, v["d_tok"], v["d_seqlen"], v["d_bt"], sel, kc, vc, Hq, Hkv)
+        elif Rd:
             ops.attn_decode(qkv, attn, v["d_tok"], v["d_seqlen"], v["d_bt"], kc, vc, Hq, Hkv, splits,
                             self.part_o, self.part_lse,
                             host={"seq_lens": hm.get("d_seq_lens"), "tok": hm.get("d_tok")})

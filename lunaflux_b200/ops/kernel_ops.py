@@ -131,7 +131,8 @@ class KernelOps:
         ``ranks[a]`` is not used); scales fp32 and ranks int32 [pool].  ``rows``
         (int32) groups token rows by adapter, ``starts[a] .. starts[a + 1]``
         being adapter a's; a row appears at most once, rows without an adapter
-        are not listed and left as they are.  base and out are [T, N], both bf16
+        are not listed and left as they are, entries behind ``starts[pool]``
+        are not read (a captured step gives the list its bucket's length).  base and out are [T, N], both bf16
         or both fp32; out may be base.  ``slices`` are the column widths of a
         stacked projection (e.g. Q, K, V), each with its own R rows of lora_a."""
         if rows.numel() == 0:
