@@ -754,7 +754,8 @@ void qk_norm_rope_kv_write(const at::Tensor& qkv, const at::Tensor& q_weight, co
   lf::ew::qk_norm_rope_kv_write(a, stream());
 }
 
-void lora_add(const at::Tensor& x, const at::Tensor& lora_a, const at::Tensor& lora_b, const at::Tensor& scales,
+// Returns the number of kernels launched.
+int64_t lora_add(const at::Tensor& x, const at::Tensor& lora_a, const at::Tensor& lora_b, const at::Tensor& scales,
               const at::Tensor& ranks, const at::Tensor& rows, const at::Tensor& starts, const at::Tensor& base,
               at::Tensor& out, const std::vector<int64_t>& slices) {
   check_op(x, x, "x", at::kBFloat16, 2);
@@ -786,7 +787,7 @@ void lora_add(const at::Tensor& x, const at::Tensor& lora_a, const at::Tensor& l
   check_ints(starts, x, "starts", pool + 1);
   LF_CHECK(starts.numel() == pool + 1, "lora_add: starts must hold pool + 1 offsets");
   LF_CHECK(rows.numel() <= T, "lora_add: a row is listed at most once");
-  LF_CHECK(T < (1ll << 31) && pool < (1ll << 24) && K < (1ll << 31) && N < (1ll << 31), "lora_add: sizes");
+  LF_CHECK(T < (1ll << 31) && pool < (1ll << 24) && K <= (1ll << 30) && N <= (1ll << 30), "lora_add: sizes");
   c10::cuda::CUDAGuard g(x.device());
   lf::lora::LoraArgs a{};
   a.x = x.data_ptr();
@@ -817,7 +818,7 @@ void lora_add(const at::Tensor& x, const at::Tensor& lora_a, const at::Tensor& l
     a.col_begin[i + 1] = (int)end;
   }
   LF_CHECK(end == N, "lora_add: slices must add up to N");
-  lf::lora::lora_add(a, stream());
+  return lf::lora::lora_add(a, stream());
 }
 
 // Common checks of the sparse attention operators: rows, table, lengths.
@@ -864,7 +865,8 @@ void page_bounds(const at::Tensor& kcache, at::Tensor& bounds, const at::Tensor&
   lf::attn::page_bounds(a, stream());
 }
 
-void attn_select(const at::Tensor& q, const at::Tensor& tok_index, const at::Tensor& seq_lens,
+// Returns the number of kernels launched.
+int64_t attn_select(const at::Tensor& q, const at::Tensor& tok_index, const at::Tensor& seq_lens,
                  const at::Tensor& block_table, const at::Tensor& bounds, at::Tensor& sel, int64_t first, int64_t last,
                  int64_t Hq, int64_t Hkv, at::Tensor& ws) {
   check_op(q, q, "q", at::kBFloat16, 2);
@@ -905,7 +907,7 @@ void attn_select(const at::Tensor& q, const at::Tensor& tok_index, const at::Ten
   a.budget = (int)budget;
   a.first = (int)first;
   a.last = (int)last;
-  lf::attn::select_pages(a, stream());
+  return lf::attn::select_pages(a, stream());
 }
 
 void attn_decode_sparse(const at::Tensor& q, at::Tensor& out, const at::Tensor& tok_index, const at::Tensor& seq_lens,

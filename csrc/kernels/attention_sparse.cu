@@ -1000,6 +1000,7 @@ void page_bounds(const BoundsArgs& a, cudaStream_t s) {
   b.max_pages = (a.max_new + PAGE - 2) / PAGE + 1;   // from any offset in a page
   if (b.max_pages > a.width) b.max_pages = a.width;
   const int64_t units = (int64_t)a.rows * a.Hkv * b.max_pages;
+  if (units / 4 >= INT32_MAX) throw std::runtime_error("lunaflux page_bounds: too many pages for one call");
   launch_k(page_bounds_kernel, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, s, 1, b);
 }
 
@@ -1017,8 +1018,8 @@ void launch_select(const SelectArgs& a, cudaStream_t s) {
 }
 }  // namespace
 
-void select_pages(const SelectArgs& a, cudaStream_t s) {
-  if (a.rows <= 0) return;
+int select_pages(const SelectArgs& a, cudaStream_t s) {
+  if (a.rows <= 0) return 0;
   if (a.width > a.budget) {
     // two passes of 64 pages per CTA where that fills the GPU (64 rows of 2048 pages: 191 us a
     // step, 198 with one, 192 with eight; a ragged batch of 17: 38, 40, 43)
@@ -1033,6 +1034,7 @@ void select_pages(const SelectArgs& a, cudaStream_t s) {
   else if (a.width <= 2048) launch_select<256, 8>(a, s);
   else if (a.width <= 8192) launch_select<1024, 8>(a, s);
   else launch_select<1024, 0>(a, s);
+  return a.width > a.budget ? 2 : 1;
 }
 
 namespace {

@@ -50,7 +50,7 @@ struct SparseArgs {
 };
 
 void page_bounds(const BoundsArgs& a, cudaStream_t s);
-void select_pages(const SelectArgs& a, cudaStream_t s);
+int select_pages(const SelectArgs& a, cudaStream_t s);   // kernels launched
 void decode_sparse(const SparseArgs& a, cudaStream_t s);
 
 }  // namespace attn

@@ -414,7 +414,6 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
   constexpr int kUnit = kThreads * 16;    // a ring unit of all lanes
   constexpr int IU = item_units<F32, WIDE>(), NI = small_items<F32, MT, WIDE>();
   extern __shared__ __align__(128) uint8_t raw[];
-  pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -619,6 +618,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
     }
   }
   cluster_arrive();                       // this CTA has read the others' partials
+  pdl_trigger();
   __syncthreads();
 
   const int es = F32 ? 4 : 2;
@@ -1108,7 +1108,8 @@ void launch_large(const LoraArgs& a, int tiles, cudaStream_t s) {
 
 // As many slices per launch as an accumulator holds: all of them up to 256 columns.
 template <bool F32>
-void large(const LoraArgs& all, cudaStream_t s) {
+int large(const LoraArgs& all, cudaStream_t s) {
+  int launches = 0;
   const int step = kLargeCols / ((all.R + 15) / 16 * 16);
   const int tiles = all.L / TML + std::min(all.L, all.pool);
   for (int s0 = 0; s0 < all.S; s0 += step) {
@@ -1120,19 +1121,22 @@ void large(const LoraArgs& all, cudaStream_t s) {
     if ((int64_t)tiles * kCluster <= cta_slots()) launch_large<F32, kCluster>(a, tiles, s);
     else if ((int64_t)tiles * 4 <= cta_slots()) launch_large<F32, 4>(a, tiles, s);
     else launch_large<F32, 2>(a, tiles, s);
+    ++launches;
   }
+  return launches;
 }
 
 }  // namespace
 
-void lora_add(const LoraArgs& args, cudaStream_t s) {
-  if (args.L <= 0 || args.N <= 0 || args.pool <= 0) return;
+int lora_add(const LoraArgs& args, cudaStream_t s) {
+  if (args.L <= 0 || args.N <= 0 || args.pool <= 0) return 0;
   LoraArgs a = args;
   a.s0 = 0;
   a.S_all = a.S;
   set_blocks(a);
-  if (a.L >= kLargeRows) a.f32 ? large<true>(a, s) : large<false>(a, s);
-  else a.f32 ? small<true>(a, s) : small<false>(a, s);
+  if (a.L >= kLargeRows) return a.f32 ? large<true>(a, s) : large<false>(a, s);
+  a.f32 ? small<true>(a, s) : small<false>(a, s);
+  return 1;
 }
 
 }  // namespace lora

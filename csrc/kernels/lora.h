@@ -31,7 +31,7 @@ struct LoraArgs {
   bool f32;                   // base and out are fp32
 };
 
-void lora_add(const LoraArgs& a, cudaStream_t s);
+int lora_add(const LoraArgs& a, cudaStream_t s);   // kernels launched
 
 }  // namespace lora
 }  // namespace lf

@@ -51,7 +51,6 @@ __global__ void __launch_bounds__(NT) qk_norm_rope_kernel(const QkNormRopeArgs a
   constexpr int kLanes = D / 16;         // lanes of one head
   constexpr int kHalf = D / 16;          // 16-byte pieces of half a head
   constexpr int kGroups = NT / kLanes;   // heads a CTA works on at a time
-  pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x;
   const int group = threadIdx.x / kLanes, l = threadIdx.x % kLanes;

@@ -137,15 +137,15 @@ class KernelOps:
         stacked projection (e.g. Q, K, V), each with its own R rows of lora_a."""
         if rows.numel() == 0:
             return
-        self.launches += 1
-        self.C.lora_add(x, lora_a, lora_b, scales, ranks, rows, starts, base, out,
-                        [lora_b.shape[1]] if slices is None else list(slices))
+        self.launches += self.C.lora_add(x, lora_a, lora_b, scales, ranks, rows, starts, base, out,
+                                         [lora_b.shape[1]] if slices is None else list(slices))
 
     def page_bounds(self, kc, bounds, bt, start, seq_lens, max_new):
         """Smallest and largest key per dimension ([pages, Hkv, 2, D]) of the pages
         that hold tokens start[r] .. seq_lens[r] of every row, over the row's
         valid tokens.  ``max_new`` bounds seq_lens - start; call it after each
-        KV write, so that the bounds follow the cache."""
+        KV write, so that the bounds follow the cache.  Rows that share a page
+        have to hold the same tokens of it."""
         if seq_lens.numel() == 0 or max_new == 0:
             return
         self.launches += 1
@@ -165,8 +165,7 @@ class KernelOps:
         ``select_workspace`` fp32 elements, used until the call's kernels end."""
         if seq_lens.numel() == 0:
             return
-        self.launches += 2 if bt.shape[1] > sel.shape[2] else 1
-        self.C.attn_select(q, tok, seq_lens, bt, bounds, sel, first, last, Hq, Hkv, ws)
+        self.launches += self.C.attn_select(q, tok, seq_lens, bt, bounds, sel, first, last, Hq, Hkv, ws)
 
     def attn_decode_sparse(self, q, out, tok, seq_lens, bt, sel, kc, vc, Hq, Hkv):
         """Decode attention over the pages of ``sel``: the first
