@@ -985,13 +985,6 @@ __global__ void __launch_bounds__(W * 32, (NH == 1 ? 16 : 8) / W) decode_sparse_
   }
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n;
-}
-
 }  // namespace
 
 void page_bounds(const BoundsArgs& a, cudaStream_t s) {
@@ -1005,12 +998,6 @@ void page_bounds(const BoundsArgs& a, cudaStream_t s) {
 }
 
 namespace {
-void raise_smem(const void* k, size_t smem) {
-  if (smem <= 48 * 1024) return;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) launch_failed(e);
-}
-
 template <int NT, int ITEMS>
 void launch_select(const SelectArgs& a, cudaStream_t s) {
   const size_t smem = (size_t)((a.width + 31) / 32) * 2 * sizeof(uint32_t);   // the general routine's masks, at most 16 KB
@@ -1047,7 +1034,8 @@ void launch_decode(const SparseArgs& a, cudaStream_t s) {
   int cl = 1;
   while (cl < kMaxCluster && units * cl * 2 <= slots && a.budget > W * cl) cl *= 2;
   auto k = decode_sparse_kernel<NH, W>;
-  raise_smem(reinterpret_cast<const void*>(k), sizeof(SparseSmem<NH, W>));
+  static std::atomic<unsigned long long> allowed{0};
+  allow_smem(reinterpret_cast<const void*>(k), allowed);
   // Clusters that start while the previous kernel still holds some SMs crowd onto
   // the others; where they would fill the GPU they wait for its end (4 rows x 8
   // heads x 256 pages after a selection: 72 instead of 82 us for the whole step).

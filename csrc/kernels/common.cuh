@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 namespace lf {
@@ -374,6 +375,34 @@ __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
+}
+
+// Multiprocessors of the current device.
+inline int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Lets a kernel take all the dynamic shared memory of an SM of the current device
+// (an attribute per kernel and device; `done` is the kernel's own, a bit per device).
+inline void allow_smem(const void* kernel, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  cudaFuncAttributes fa;
+  int most = 0;
+  cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)fa.sharedSizeBytes);
+  if (e != cudaSuccess) launch_failed(e);
+  done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 // launch_k: host launch of a step kernel: cudaLaunchKernelEx with the programmatic

@@ -1043,12 +1043,6 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
   if (warp == 0) tmem_dealloc(tmem, kTmemCols);
 }
 
-void raise_smem(const void* k, size_t smem) {
-  if (smem <= 48 * 1024) return;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) launch_failed(e);
-}
-
 void set_blocks(LoraArgs& a) {
   a.block32[0] = a.block128[0] = 0;
   for (int i = 0; i < kMaxSlices; ++i) {
@@ -1058,12 +1052,7 @@ void set_blocks(LoraArgs& a) {
   }
 }
 
-int cta_slots() {   // two CTAs per SM
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return 2 * n;
-}
+int cta_slots() { return 2 * sm_count(); }
 
 template <bool F32, int MT, bool WIDE>
 void launch_small(const LoraArgs& a, cudaStream_t s) {
@@ -1071,7 +1060,8 @@ void launch_small(const LoraArgs& a, cudaStream_t s) {
   const int parts = F32 ? 3 : 2;
   const size_t smem = (size_t)small_units<F32, MT, WIDE>() * kThreads * 16 + sizeof(float) * kSmallRows * cols + (size_t)2 * parts * kSmallRows * (cols + 40);
   auto k = lora_small_kernel<F32, MT, WIDE>;
-  raise_smem(reinterpret_cast<const void*>(k), smem);
+  static std::atomic<unsigned long long> allowed{0};
+  allow_smem(reinterpret_cast<const void*>(k), allowed);
   const int tiles = a.L / kSmallRows + std::min(a.L, a.pool);   // at least the sum of ceil(rows / 16) over the adapters
   // Fewer CTAs per tile where they would not all run at once, as long as a CTA's
   // share of the weights stays small.
@@ -1102,7 +1092,8 @@ void launch_large(const LoraArgs& a, int tiles, cudaStream_t s) {
   const int cols = a.S * ((a.R + 15) / 16 * 16);
   const LargeSmem sm = large_smem(cols, a.R, F32 ? 3 : 2);
   auto k = lora_large_kernel<F32, CL>;
-  raise_smem(reinterpret_cast<const void*>(k), sm.total);
+  static std::atomic<unsigned long long> allowed{0};
+  allow_smem(reinterpret_cast<const void*>(k), allowed);
   launch_k(k, dim3((unsigned)tiles * CL), dim3(kThreads), sm.total, s, (unsigned)CL, a, cols, (int)sm.hs);
 }
 

@@ -153,10 +153,7 @@ __global__ void __launch_bounds__(NT) qk_norm_rope_kernel(const QkNormRopeArgs a
 // stores interleave best (8192 rows: 37.2 us, 41.2 with 128, 69 with 256).
 template <int D>
 void launch_d(const QkNormRopeArgs& a, cudaStream_t s) {
-  int dev = 0, sms = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (a.T <= 2 * sms) launch_k(qk_norm_rope_kernel<D, 256>, dim3(a.T), dim3(256), 0, s, 1, a);
+  if (a.T <= 2 * sm_count()) launch_k(qk_norm_rope_kernel<D, 256>, dim3(a.T), dim3(256), 0, s, 1, a);
   else launch_k(qk_norm_rope_kernel<D, 64>, dim3(a.T), dim3(64), 0, s, 1, a);
 }
 
