@@ -723,8 +723,9 @@ __global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
 // the tokens; the sum of the weights is kept in fp32 from the same rounded
 // values, so the rounding does not scale the output.
 //
-// The next page's K is fetched into the same registers as soon as S is known,
-// its V after O is updated: 16 warps per SM with a page each under way.
+// 16 warps per SM have a page each under way; 64 rows x 8 heads x 128 pages read
+// 1.07 GB in 175 us, 6.1 TB/s.  A page ahead in registers halves the warps, and per-lane
+// cp.async delivers less than plain loads: both were slower.
 // ===========================================================================
 constexpr int kMaxCluster = 8;
 
@@ -1017,6 +1018,9 @@ int select_pages(const SelectArgs& a, cudaStream_t s) {
     auto k = a.Hq / a.Hkv <= 8 ? page_score_kernel<1> : page_score_kernel<2>;
     launch_k(k, grid, dim3(kThreads), 0, s, 1, a, passes);
   }
+  // As few threads and pages per thread as hold the block table: 8191 tokens 14.1 us
+  // a step, 16.2 with <256, 8>, 20.4 with <1024, 8>; 64 rows of 32768 tokens 188 us, 212
+  // with <1024, 8>, 303 with the general routine.
   if (a.width <= 512) launch_select<256, 2>(a, s);
   else if (a.width <= 2048) launch_select<256, 8>(a, s);
   else if (a.width <= 8192) launch_select<1024, 8>(a, s);
@@ -1046,9 +1050,14 @@ void launch_decode(const SparseArgs& a, cudaStream_t s) {
 
 void decode_sparse(const SparseArgs& a, cudaStream_t s) {
   if (a.rows <= 0) return;
-  // eight warps per CTA where clusters of eight CTAs still leave SMs without work
-  const bool few = (int64_t)a.rows * a.Hkv * kMaxCluster <= sm_count();
-  if (a.Hq / a.Hkv <= 8) few ? launch_decode<1, 8>(a, s) : launch_decode<1, 4>(a, s);
+  // Eight warps per CTA where clusters of eight CTAs still leave SMs without work (1
+  // row x 8 heads x 64 pages: a step takes 14.1 us, 16.0 with four) or, with four
+  // warps, half of the warps that fit, and each of the eight still gets two pages (4 x 8
+  // x 256 pages 54.9 us, 58.1; 4 x 8 x 128 28.2, 29.2; 4 x 8 x 64 would lose, 19.6, 18.9).
+  const int64_t ctas = (int64_t)a.rows * a.Hkv * kMaxCluster;
+  const bool narrow = a.Hq / a.Hkv <= 8;   // wider groups fit eight warps per SM
+  const bool few = ctas <= sm_count() || (narrow && ctas <= 2 * sm_count() && a.budget >= 2 * 8 * kMaxCluster);
+  if (narrow) few ? launch_decode<1, 8>(a, s) : launch_decode<1, 4>(a, s);
   else few ? launch_decode<2, 8>(a, s) : launch_decode<2, 4>(a, s);
 }
 

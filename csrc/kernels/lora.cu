@@ -9,16 +9,18 @@
 // on as two bf16 parts (three for fp32 outputs), an error of at most 2^-16
 // (2^-24) of h, and the output is rounded once.
 //
-// A cluster of eight CTAs owns a tile of up to TM rows of one adapter: every
-// CTA multiplies an eighth of K, the partial h are added through distributed
-// shared memory in rank order, and every CTA expands an eighth of the columns.
-// So the whole operator is one launch without a workspace, x and the weights
-// are read by one CTA each, and a result does not depend on the order of arrival.  Only the adapter's rank is read, of A and
-// of B: inside a tile, h has S * rank columns, the rank rounded up to 8 (16 in the large kernel) ("compact" below).
+// A cluster of up to eight CTAs owns a tile of up to TM rows of one adapter:
+// every CTA multiplies a share of K, the partial h are added through distributed
+// shared memory in rank order, and every CTA expands a share of the columns.  So
+// the whole operator is one launch without a workspace, x and the weights are
+// read by one CTA each, and a result does not depend on the order of arrival.
+// Only the adapter's rank is read, of A and of B: inside a tile, h has S * rank
+// columns, the rank rounded up to 8 (16 in the large kernel) ("compact" below).
 //
 // Two kernels.  The small one (TM = 16, mma.sync) is for decode, where reading the
 // weights bounds the call; the large one (TM = 64, tcgen05) is for prefill, where
-// x, base and out do, and the weights come from L2 once per tile.
+// x, base and out do, and the weights come from L2 once per tile.  use_large()
+// has the rule and both sides' times.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -712,13 +714,20 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
 //
 // The same tiles on mma.sync took 131 us for 8192 rows of ranks up to 64 beside a
 // QKV projection: fragment loads, copies and products filled one another's time.
-// A CTA holds 256 columns of tensor memory and at least 80 KB of shared memory,
-// so that two, and never more, share an SM.
+//
+// A CTA holds 256 of the SM's 512 columns of tensor memory.  At least 80 KB of shared
+// memory keep it at two per SM, so that none waits for a third one's columns; the
+// other kernels with tensor memory take more than half of the shared memory, so
+// that beside one of them at most one of these runs.
+//
+// 8192 rows beside the QKV projection: 94 us where the bytes that x, base, out and the
+// weights must move once take 40.  What bounds it is copies into shared memory:
+// every tile reads its adapter's weights from L2, and a warp's 16-byte asynchronous
+// copies deliver 19 to 32 bytes per clock and SM.
 // ===========================================================================
 constexpr int TML = 64;                  // rows of a large tile
 constexpr int kStages = 3;
 constexpr int kLargeCols = 256;          // most compact columns (one accumulator)
-constexpr int kLargeRows = 768;          // listed rows from which the large tiles are used
 constexpr int kTmemCols = 256;
 constexpr int kBN = 128;                 // columns of a block of the expansion
 
@@ -1052,6 +1061,22 @@ void set_blocks(LoraArgs& a) {
   }
 }
 
+// The small kernel's time grows with the products of its tiles on mma.sync, the
+// large one's with the CTAs' trips over K and with the weights that its tiles
+// read, whatever the rank.  Tiles are estimated from the number of listed rows and
+// of adapters, which is all the host knows.  Over 430 random calls (up to 4096 rows,
+// K 512 to 14336, N 768 to 10240, ranks 8 to 128, 1 to 128 adapters) the choice
+// costs 1.8 % over the better one in the mean, 40 % at most; large tiles from a
+// fixed number of rows cost 8 % and up to 3.3 times.  Small / large, bf16, eight
+// adapters, K = 4096, three slices of together 6144 columns: rank 64, 128 rows 19.6 /
+// 24.1 us, 384 rows 29.9 / 25.7, 2048 rows 111 / 41; rank 16, 2048 rows 30.6 / 35.5.
+bool use_large(const LoraArgs& a) {
+  const double adapters = std::min(a.L, a.pool);
+  const double small_tiles = a.L / kSmallRows + adapters / 2, large_tiles = a.L / TML + adapters;
+  const double work = small_tiles * a.R * ((double)a.S * a.K + (a.f32 ? 3.0 : 2.0) * a.N);
+  return work >= 105.0 * (32.0 * a.K + large_tiles * ((double)a.K + a.N));
+}
+
 int cta_slots() { return 2 * sm_count(); }
 
 template <bool F32, int MT, bool WIDE>
@@ -1064,7 +1089,8 @@ void launch_small(const LoraArgs& a, cudaStream_t s) {
   allow_smem(reinterpret_cast<const void*>(k), allowed);
   const int tiles = a.L / kSmallRows + std::min(a.L, a.pool);   // at least the sum of ceil(rows / 16) over the adapters
   // Fewer CTAs per tile where they would not all run at once, as long as a CTA's
-  // share of the weights stays small.
+  // share of the weights stays small (64 adapters with a row each, rank 16: clusters
+  // of 8 18.7 us, 4 14.9, 2 19.1; 32 adapters of rank 64 with 2.3 MB each, 8 24.4, 4 26.6).
   const int64_t bytes = 2 * (int64_t)a.R * ((int64_t)a.S * a.K + a.N);
   int cl = kCluster;
   while (cl > 1 && (int64_t)tiles * cl > cta_slots() && bytes / cl < 128 * 1024) cl /= 2;
@@ -1074,6 +1100,10 @@ void launch_small(const LoraArgs& a, cudaStream_t s) {
   launch_k(k, dim3((unsigned)(tiles * cl)), dim3(kThreads), smem, s, (unsigned)cl, a, cols, cl, vector);
 }
 
+// MT: 16-column tiles of h a warp accumulates at a time, no more than there are
+// (256 rows, rank 16 and one slice: 7.5 us, 8.8 with four).  WIDE: steps of 32 along
+// the rank, half as many trips over the same bytes (256 rows of rank 64: 23.7 us, 26.2
+// with steps of 16), which the rank has to be a multiple of.
 template <bool F32>
 void small(const LoraArgs& a, cudaStream_t s) {
   const int cols = a.S * a.R;
@@ -1098,6 +1128,8 @@ void launch_large(const LoraArgs& a, int tiles, cudaStream_t s) {
 }
 
 // As many slices per launch as an accumulator holds: all of them up to 256 columns.
+// The largest clusters whose CTAs all run at once: 768 rows of ranks up to 64, 8 25.6
+// us, 4 39.4, 2 67.4; 2048 rows 52.4, 48.9, 67.6; 8192 rows 129, 103, 95.3.
 template <bool F32>
 int large(const LoraArgs& all, cudaStream_t s) {
   int launches = 0;
@@ -1125,7 +1157,7 @@ int lora_add(const LoraArgs& args, cudaStream_t s) {
   a.s0 = 0;
   a.S_all = a.S;
   set_blocks(a);
-  if (a.L >= kLargeRows) return a.f32 ? large<true>(a, s) : large<false>(a, s);
+  if (use_large(a)) return a.f32 ? large<true>(a, s) : large<false>(a, s);
   a.f32 ? small<true>(a, s) : small<false>(a, s);
   return 1;
 }
