@@ -1079,6 +1079,51 @@ bool use_large(const LoraArgs& a) {
 
 int cta_slots() { return 2 * sm_count(); }
 
+// Clusters of `cl` CTAs of a small kernel that run at once.  GPCs hold different
+// numbers of SMs, so the device is asked, once per kernel, size and CTAs per SM.
+template <typename Kernel>
+int clusters_at_once(Kernel kernel, int cl, size_t smem, std::atomic<int> (&known)[64][2][kCluster + 1]) {
+  const int pair = 2 * (smem + 2048) <= 228 * 1024 ? 1 : 0;       // two CTAs share an SM
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  if (cl == 1) return (1 + pair) * sm_count();
+  if (dev < 64 && (n = known[dev][pair][cl].load(std::memory_order_relaxed)) > 0) return n;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cl;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cl);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  if (e != cudaSuccess) launch_failed(e);
+  n = std::max(n, 1);
+  if (dev < 64) known[dev][pair][cl].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// CTAs per tile of the small kernel: as many as possible while the tiles still run in
+// the fewest waves, a wave costing about 6 us and, per CTA, 24 KB of weights a
+// microsecond.  The tiles are those of evenly used adapters.  64 adapters with a row
+// each, rank 16: clusters of 8 18.9 us, 6 22.9, 5 24.0, 4 14.7, 2 19.0; 512 rows of 20
+// adapters (40 tiles): 8 12.6, 6 7.7, 4 8.9, 2 10.1; one tile: 8 8.0, 4 10.0, 2 14.0.
+template <typename AtOnce>
+int cluster_size(const LoraArgs& a, AtOnce at_once) {
+  const int64_t adapters = std::min(a.L, a.pool);
+  const int64_t tiles = adapters * ((a.L + kSmallRows * adapters - 1) / (kSmallRows * adapters));
+  const int64_t bytes = 2 * (int64_t)a.R * ((int64_t)a.S * a.K + a.N);
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int cl = kCluster; cl >= 1; --cl) {
+    const int64_t n = at_once(cl), cost = (tiles + n - 1) / n * (144 * 1024 + bytes / cl);
+    if (cost < least) least = cost, best = cl;
+  }
+  return best;
+}
+
 template <bool F32, int MT, bool WIDE>
 void launch_small(const LoraArgs& a, cudaStream_t s) {
   const int cols = (a.S * a.R + 15) / 16 * 16;
@@ -1088,12 +1133,8 @@ void launch_small(const LoraArgs& a, cudaStream_t s) {
   static std::atomic<unsigned long long> allowed{0};
   allow_smem(reinterpret_cast<const void*>(k), allowed);
   const int tiles = a.L / kSmallRows + std::min(a.L, a.pool);   // at least the sum of ceil(rows / 16) over the adapters
-  // Fewer CTAs per tile where they would not all run at once, as long as a CTA's
-  // share of the weights stays small (64 adapters with a row each, rank 16: clusters
-  // of 8 18.7 us, 4 14.9, 2 19.1; 32 adapters of rank 64 with 2.3 MB each, 8 24.4, 4 26.6).
-  const int64_t bytes = 2 * (int64_t)a.R * ((int64_t)a.S * a.K + a.N);
-  int cl = kCluster;
-  while (cl > 1 && (int64_t)tiles * cl > cta_slots() && bytes / cl < 128 * 1024) cl /= 2;
+  static std::atomic<int> at_once[64][2][kCluster + 1];
+  const int cl = cluster_size(a, [&](int c) { return clusters_at_once(k, c, smem, at_once); });
   // one_row() keeps its share of x and h in the same shared memory
   const int64_t span = (((a.K + 31) / 32 + cl - 1) / cl * 32 + 255) / 256 * 256;
   const bool vector = (a.R & (a.R - 1)) == 0 && (span + 2 * cols) * 4 <= (int64_t)smem;
