@@ -29,6 +29,7 @@
 #include <stdexcept>
 
 #include "common.cuh"
+#include "gemm_bf16.h"
 #include "lora.h"
 
 namespace lf {
@@ -729,6 +730,7 @@ constexpr int TML = 64;                  // rows of a large tile
 constexpr int kStages = 3;
 constexpr int kLargeCols = 256;          // most compact columns (one accumulator)
 constexpr int kTmemCols = 256;
+constexpr int kBoxRows = 16;             // rows of A per box
 constexpr int kBN = 128;                 // columns of a block of the expansion
 
 // 16 lanes x 8 groups of 8 columns: r[4 x + 0 / 1] = row g, columns 8 x + 2 c, + 1;
@@ -760,17 +762,18 @@ __host__ __device__ inline LargeSmem large_smem(int cols_max, int R, int parts) 
 }
 
 template <bool F32, int CL>
-__global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs a, int cols_max, int smem_hs) {
+__global__ void __launch_bounds__(kThreads, 2)
+    lora_large_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap map_a, int cols_max, int smem_hs) {
   constexpr int kParts = F32 ? 3 : 2;
   extern __shared__ __align__(128) uint8_t raw_unaligned[];
   __shared__ int tile_rows[TML];
-  __shared__ const __nv_bfloat16* row_src[TML + kLargeCols];   // first element of every staged row, null for a zero row
-  __shared__ __align__(8) uint64_t empty[kStages], done[2];
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done[2];
   __shared__ uint32_t tmem_base;
   uint8_t* raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int cta = (int)cluster_rank();
+  if (tid == 0) tma_prefetch_desc(&map_a);
   pdl_wait();
   const Tile tl = find_tile<TML>(a, blockIdx.x / CL);
   if (tl.adapter < 0) return;             // the whole cluster
@@ -787,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
     tmem_relinquish();
   }
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&empty[i], 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     mbar_init(&done[0], 1);
     mbar_init(&done[1], 1);
     fence_barrier_init();
@@ -795,22 +798,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
 
   // ---- shrink
   const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x);
-  {
-    const __nv_bfloat16* A =
-        reinterpret_cast<const __nv_bfloat16*>(a.a) + ((int64_t)tl.adapter * a.S_all + a.s0) * a.R * a.K;
-    for (int r = tid; r < TML + cols; r += kThreads) {
-      const __nv_bfloat16* src = nullptr;
-      if (r < TML) {
-        const int row = tile_row(a, tl, r);
-        tile_rows[r] = row;
-        if (row >= 0) src = x + (int64_t)row * a.ldx;
-      } else {
-        const int j = r - TML, s = j / rp, q = j - s * rp;
-        if (q < rank) src = A + (int64_t)(s * a.R + q) * a.K;
-      }
-      row_src[r] = src;
-    }
-  }
+  if (tid < TML) tile_rows[tid] = tile_row(a, tl, tid);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -822,19 +810,30 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
     const int per_cta = (chunks + CL - 1) / CL;
     const int ch0 = cta * per_cta, n = cols > 0 ? max(0, min(chunks, ch0 + per_cta) - ch0) : 0;
     const int stage_bytes = 128 * (TML + cols);
-    // thread t copies piece t % 8 of rows t / 8, t / 8 + 32, ...
+    // thread t copies piece t % 8 of token rows t / 8 and t / 8 + 32, the first one issues A's boxes
     const int piece = tid & 7, rfirst = tid >> 3;
     const uint32_t dst0 = raw_u + rfirst * 128 + ((piece ^ (rfirst & 7)) << 4);
+    const int row_a = tile_rows[rfirst], row_b = tile_rows[rfirst + 32];
+    const __nv_bfloat16* xa = row_a >= 0 ? x + (int64_t)row_a * a.ldx : nullptr;
+    const __nv_bfloat16* xb = row_b >= 0 ? x + (int64_t)row_b * a.ldx : nullptr;
+    const int first_row = (tl.adapter * a.S_all + a.s0) * a.R;       // of lora_a
+    auto box_row = [&](int b) {            // first row of A of box b
+      const int j = b * kBoxRows, s = rp > 0 ? j / rp : 0;
+      return j < cols ? first_row + s * a.R + j - s * rp : -1;
+    };
+    const int box0 = box_row(warp), box1 = box_row(warp + kWarps);
     auto load_stage = [&](int i) {
       if (i < n) {
-        const uint32_t dst = dst0 + (i % kStages) * stage_bytes;
-        const int k = (ch0 + i) * 64 + piece * 8;
+        const int st = i % kStages;
+        const int k0 = (ch0 + i) * 64, k = k0 + piece * 8;
+        if (tid == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)cols * 128);
+        if (lane == 0 && box0 >= 0) tma_load_2d(raw + st * stage_bytes + (TML + warp * kBoxRows) * 128, &map_a, &full[st], k0, box0);
+        if (lane == 0 && box1 >= 0)
+          tma_load_2d(raw + st * stage_bytes + (TML + (warp + kWarps) * kBoxRows) * 128, &map_a, &full[st], k0, box1);
         const bool in = k < a.K;
-        for (int r = rfirst, o = 0; r < TML + cols; r += 32, o += 32 * 128) {
-          const __nv_bfloat16* src = row_src[r];
-          const bool on = in && src != nullptr;
-          cp_async16(dst + o, on ? src + k : x, on);
-        }
+        const bool on_a = in && xa != nullptr, on_b = in && xb != nullptr;
+        cp_async16(dst0 + st * stage_bytes, on_a ? xa + k : x, on_a);
+        cp_async16(dst0 + st * stage_bytes + 32 * 128, on_b ? xb + k : x, on_b);
       }
       cp_async_commit();
     };
@@ -845,6 +844,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
       fence_proxy_async_smem();
       __syncthreads();
       if (warp == 0 && elect_one()) {
+        mbar_wait(&full[i % kStages], (i / kStages) & 1, 43);
+        tc_fence_after();
         const uint32_t st = raw_u + (i % kStages) * stage_bytes;
         const uint64_t xd = sw128_kmajor_desc(st), ad = sw128_kmajor_desc(st + TML * 128);
 #pragma unroll
@@ -869,11 +870,12 @@ __global__ void __launch_bounds__(kThreads, 2) lora_large_kernel(const LoraArgs 
         const int col = c0 + xg * 8 + 2 * c;
         if (col >= cols) continue;
         float* p = part + (sub * 16 + g) * pld + col;
-        const bool live = n > 0;          // a CTA without a share of K adds zero
+        // Past the rank h is zero, whatever the boxes brought; a CTA without a share of K adds zero.
+        const int left = n > 0 ? rank - col % rp : 0;
         *reinterpret_cast<float2*>(p) =
-            live ? make_float2(__uint_as_float(r[4 * xg]), __uint_as_float(r[4 * xg + 1])) : make_float2(0.f, 0.f);
+            make_float2(left > 0 ? __uint_as_float(r[4 * xg]) : 0.f, left > 1 ? __uint_as_float(r[4 * xg + 1]) : 0.f);
         *reinterpret_cast<float2*>(p + 8 * pld) =
-            live ? make_float2(__uint_as_float(r[4 * xg + 2]), __uint_as_float(r[4 * xg + 3])) : make_float2(0.f, 0.f);
+            make_float2(left > 0 ? __uint_as_float(r[4 * xg + 2]) : 0.f, left > 1 ? __uint_as_float(r[4 * xg + 3]) : 0.f);
       }
     }
     tc_fence_before();
@@ -1071,6 +1073,7 @@ void set_blocks(LoraArgs& a) {
 // adapters, K = 4096, three slices of together 6144 columns: rank 64, 128 rows 19.6 /
 // 24.1 us, 384 rows 29.9 / 25.7, 2048 rows 111 / 41; rank 16, 2048 rows 30.6 / 35.5.
 bool use_large(const LoraArgs& a) {
+  if ((int64_t)a.pool * a.S * a.R > INT32_MAX) return false;   // rows of A are 32-bit coordinates
   const double adapters = std::min(a.L, a.pool);
   const double small_tiles = a.L / kSmallRows + adapters / 2, large_tiles = a.L / TML + adapters;
   const double work = small_tiles * a.R * ((double)a.S * a.K + (a.f32 ? 3.0 : 2.0) * a.N);
@@ -1165,7 +1168,9 @@ void launch_large(const LoraArgs& a, int tiles, cudaStream_t s) {
   auto k = lora_large_kernel<F32, CL>;
   static std::atomic<unsigned long long> allowed{0};
   allow_smem(reinterpret_cast<const void*>(k), allowed);
-  launch_k(k, dim3((unsigned)tiles * CL), dim3(kThreads), sm.total, s, (unsigned)CL, a, cols, (int)sm.hs);
+  const CUtensorMap map_a = gemm::make_tmap_2d(a.a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.pool * a.S_all * a.R, a.K,
+                                               a.K, kBoxRows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+  launch_k(k, dim3((unsigned)tiles * CL), dim3(kThreads), sm.total, s, (unsigned)CL, a, map_a, cols, (int)sm.hs);
 }
 
 // As many slices per launch as an accumulator holds: all of them up to 256 columns.
