@@ -18,7 +18,7 @@
 // columns, the rank rounded up to 8 (16 in the large kernel) ("compact" below).
 //
 // Two kernels.  The small one (TM = 16, mma.sync) is for decode, where reading the
-// weights bounds the call; the large one (TM = 64, tcgen05) is for prefill, where
+// weights bounds the call; the large one (TM = 64 or 128, tcgen05) is for prefill, where
 // x, base and out do, and the weights come from L2 once per tile.  use_large()
 // has the rule and both sides' times.
 #include <cuda_bf16.h>
@@ -169,13 +169,22 @@ __device__ __forceinline__ int tile_row(const LoraArgs& a, const Tile& t, int i)
   return -1;
 }
 
+// Streaming 16-byte load (no line kept in L1).
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
 // Eight consecutive output columns of one row: base + scale * d, rounded once.
 template <bool F32>
 struct BaseCols {
   uint4 v[F32 ? 2 : 1];
   __device__ __forceinline__ void load(const void* at) {
 #pragma unroll
-    for (int i = 0; i < (F32 ? 2 : 1); ++i) v[i] = reinterpret_cast<const uint4*>(at)[i];
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) v[i] = ld_stream(reinterpret_cast<const uint4*>(at) + i);
   }
   __device__ __forceinline__ void store(void* at, const float (&d)[8], float scale) const {
     if (F32) {
@@ -227,7 +236,7 @@ __device__ __forceinline__ Block column_block(const LoraArgs& a, int idx) {
 constexpr int kSmallRows = 16;
 
 template <int MT>
-constexpr int small_stages() { return MT >= 4 ? 2 : MT == 3 ? 3 : 4; }
+constexpr int small_stages() { return MT >= 3 ? 2 : 4; }   // more leave too little L1 for one_row()'s loads: 64 adapters 14.0 us, 14.7 with three
 // The ring in units of 16 bytes per lane.  The warps' sums take its first 2 MT
 // units between the two phases; the expansion's items use the others.
 template <bool F32, bool WIDE>
@@ -245,14 +254,6 @@ constexpr int small_items() {   // items under way
 
 // WIDE: R is a multiple of 32, a lane reads 8 consecutive k of a column (two
 // k-steps); else 4 (one k-step).
-// Streaming 16-byte load (no line kept in L1).
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 
 // Tiles of one row, the usual ones where every request has its own adapter:
 // products of the weights with a vector, on the fp32 units.  A warp reads 512
@@ -260,6 +261,9 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
 // shared memory, so its sums need no other warp; R / 8 lanes read one column of B.
 // R is a power of two.  The loops are kept short: a CTA runs each once or a few
 // times, and longer ones would wait for their instructions.
+// One request of rank 16 beside the QKV projection takes 6.6 us, 7.8 as a tile of
+// 16 rows; 64 requests 14.0 and 16.2, of rank 64 43 and 61; one of rank 64 and K = 14336 loses
+// a microsecond, 12.8 and 11.6.
 __device__ __forceinline__ float dot8(const uint4& v, const float4& x0, const float4& x1, float acc) {
   acc += __uint_as_float(v.x << 16) * x0.x;
   acc += __uint_as_float(v.x & 0xffff0000u) * x0.y;
@@ -700,34 +704,34 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
 }
 
 // ===========================================================================
-// Large tiles: 64 rows, both products on the fifth-generation tensor cores.
+// Large tiles: 64 or 128 rows, both products on the fifth-generation tensor cores.
 //
-// Shrink: h = x A^T accumulates in tensor memory over chunks of 64 k, x rows and
-// the adapter's A rows in a three-stage cp.async ring with the 128-byte swizzle
-// the instruction reads.  Each CTA of the cluster has a share of K; the partial h
-// go to shared memory and are reduced in slices: CTA q of CL adds rows
-// [q 64 / CL, ...) of all CTAs, splits them into bf16 parts and stores those into
-// every CTA's shared memory, a fraction of the traffic of every CTA reading
-// everything.  Expand: blocks of 128 columns of B (two stages) against the parts
-// of h into one of two accumulators, read back in the 16 x 256-bit shape, in which
-// a lane holds two adjacent columns of rows g and g + 8; B's columns are stored in
-// an order that makes them eight consecutive columns over four tiles.
+// Shrink: h = x A^T accumulates in tensor memory over chunks of 64 k, x rows (gathered,
+// cp.async) and the adapter's A rows (TMA, boxes of 16) in a ring of three to six
+// stages with the 128-byte swizzle the instruction reads.  Each CTA of the cluster
+// has a share of K; the partial h go to shared memory and are reduced in slices: CTA
+// q of CL adds rows [q TML / CL, ...) of all CTAs, splits them into bf16 parts and,
+// once all partials have been read, stores those in their place into every CTA's
+// shared memory, a fraction of the traffic of every CTA reading everything.  Expand:
+// blocks of 128 columns of B (two stages) against the parts of h into one of two
+// accumulators, read back in the 16 x 256-bit shape, in which a lane holds two
+// adjacent columns of rows g and g + 8; B's columns are stored in an order that makes
+// them eight consecutive columns over four tiles.
 //
-// The same tiles on mma.sync took 131 us for 8192 rows of ranks up to 64 beside a
-// QKV projection: fragment loads, copies and products filled one another's time.
+// A CTA holds 256 of the SM's 512 columns of tensor memory.  Registers (128 rows) or at
+// least 81 KB of shared memory (64 rows) keep it at one or two per SM, so that none
+// waits for another one's columns; the other kernels with tensor memory take more
+// than half of the shared memory, so that beside one of them at most one of these
+// runs.
 //
-// A CTA holds 256 of the SM's 512 columns of tensor memory.  At least 80 KB of shared
-// memory keep it at two per SM, so that none waits for a third one's columns; the
-// other kernels with tensor memory take more than half of the shared memory, so
-// that beside one of them at most one of these runs.
-//
-// 8192 rows beside the QKV projection: 94 us where the bytes that x, base, out and the
-// weights must move once take 40.  What bounds it is copies into shared memory:
-// every tile reads its adapter's weights from L2, and a warp's 16-byte asynchronous
-// copies deliver 19 to 32 bytes per clock and SM.
+// 8192 rows beside the QKV projection: 76 us, where the bytes that x, base, out and
+// the weights must move once take 40.  64-row tiles take 93: the 64-row instruction
+// runs at half rate and every tile reads its adapter's weights from L2 again.  Not
+// more shared memory than needed, because the loads of base that are under way live
+// in what is left of it as L1: with 226 KB instead of 162 the call takes 88 us.
+// The same 64-row tiles on mma.sync took 131.
 // ===========================================================================
-constexpr int TML = 64;                  // rows of a large tile
-constexpr int kStages = 3;
+constexpr int kMinStages = 3, kMaxStages = 6;
 constexpr int kLargeCols = 256;          // most compact columns (one accumulator)
 constexpr int kTmemCols = 256;
 constexpr int kBoxRows = 16;             // rows of A per box
@@ -747,27 +751,33 @@ __device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t (&r)
       : "r"(taddr));
 }
 
+// Ring, then partial h, then [parts of h | B stages], one after the other in the same memory.
+// What the ring has beyond three stages it uses.
+constexpr size_t kLargeSmem = 226 * 1024;
 struct LargeSmem {
-  size_t hs, total;     // [ring | partial h | B stages] below hs; the ring may reach over it
+  size_t b, total;      // offset of the B stages
 };
-__host__ __device__ inline LargeSmem large_smem(int cols_max, int R, int parts) {
-  const size_t ring = (size_t)kStages * 128 * (TML + cols_max);
-  const size_t part = (size_t)TML * (cols_max + 4) * 4;
+__host__ __device__ inline LargeSmem large_smem(int tm, int cols_max, int R, int parts) {
+  const size_t ring = (size_t)kMinStages * 128 * (tm + cols_max);
+  const size_t part = (size_t)tm * (cols_max + 4) * 4;
+  const size_t hs = (size_t)parts * ((cols_max + 63) / 64) * (tm * 128);
   const size_t b = (size_t)2 * kBN * ((R + 63) / 64 * 128);
-  const size_t low = ((part > b ? part : b) + 1023) / 1024 * 1024;
-  const size_t hs = (size_t)parts * ((cols_max + 63) / 64) * (TML * 128);
-  size_t total = low + hs > ring ? low + hs : ring;
-  if (total < 80 * 1024) total = 80 * 1024;
-  return {low, total + 1024};   // and the alignment to 1024
+  size_t need = hs + b;
+  if (need < ring) need = ring;
+  if (need < part) need = part;
+  need += 1024;                // and the alignment to 1024
+  const size_t least = tm == 64 ? 81 * 1024 : 162 * 1024;   // tall tiles: four stages (76 us), three take 80
+  return {hs, need > least ? need : least};
 }
 
-template <bool F32, int CL>
-__global__ void __launch_bounds__(kThreads, 2)
-    lora_large_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap map_a, int cols_max, int smem_hs) {
+template <bool F32, int TML, int CL>
+__global__ void __launch_bounds__(TML * 4, 128 / TML)
+    lora_large_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap map_a, int cols_max, int smem_b, int smem_ring) {
+  constexpr int kThreads = TML * 4, kWarps = kThreads / 32;
   constexpr int kParts = F32 ? 3 : 2;
   extern __shared__ __align__(128) uint8_t raw_unaligned[];
   __shared__ int tile_rows[TML];
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done[2];
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done[2];
   __shared__ uint32_t tmem_base;
   uint8_t* raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -782,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int cols = a.S * rp;
   const int pld = cols_max + 4;
   float* part = reinterpret_cast<float*>(raw);
-  uint8_t* hs = raw + smem_hs;            // [part][64 columns][64 rows][128 bytes]
+  uint8_t* hs = raw;                      // [part][64 columns][row][128 bytes]
   const int hpart = (cols_max + 63) / 64 * (TML * 128);
   const uint32_t raw_u = smem_u32(raw);
   if (warp == 0) {
@@ -790,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     tmem_relinquish();
   }
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < kMaxStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     mbar_init(&done[0], 1);
     mbar_init(&done[1], 1);
     fence_barrier_init();
@@ -803,17 +813,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
-  const int sub = warp & 3, half = warp >> 2;      // this warp's rows (16 sub ...) and columns of an accumulator
-  const uint32_t tmem_row = tmem + ((uint32_t)(sub * 32) << 16);
+  // This warp's 16 rows and 64 of 128 columns of an accumulator.  The 64-row instruction
+  // leaves rows 16 i ... in lanes 32 i ..., the 128-row one a row in every lane.
+  const int wrow = TML == 64 ? (warp & 3) * 16 : (warp & 3) * 32 + (warp >> 2 & 1) * 16;
+  const int half = warp / (kWarps / 2);
+  const uint32_t tmem_row = tmem + ((uint32_t)(TML == 64 ? wrow * 2 : wrow) << 16);
   {
     const int chunks = (a.K + 63) / 64;
     const int per_cta = (chunks + CL - 1) / CL;
     const int ch0 = cta * per_cta, n = cols > 0 ? max(0, min(chunks, ch0 + per_cta) - ch0) : 0;
     const int stage_bytes = 128 * (TML + cols);
-    // thread t copies piece t % 8 of token rows t / 8 and t / 8 + 32, the first one issues A's boxes
+    const int stages = min(kMaxStages, smem_ring / stage_bytes);
+    // thread t copies piece t % 8 of token rows t / 8 and t / 8 + TML / 2; a warp's first lane a box of A or two
     const int piece = tid & 7, rfirst = tid >> 3;
     const uint32_t dst0 = raw_u + rfirst * 128 + ((piece ^ (rfirst & 7)) << 4);
-    const int row_a = tile_rows[rfirst], row_b = tile_rows[rfirst + 32];
+    const int row_a = tile_rows[rfirst], row_b = tile_rows[rfirst + TML / 2];
     const __nv_bfloat16* xa = row_a >= 0 ? x + (int64_t)row_a * a.ldx : nullptr;
     const __nv_bfloat16* xb = row_b >= 0 ? x + (int64_t)row_b * a.ldx : nullptr;
     const int first_row = (tl.adapter * a.S_all + a.s0) * a.R;       // of lora_a
@@ -822,9 +836,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       return j < cols ? first_row + s * a.R + j - s * rp : -1;
     };
     const int box0 = box_row(warp), box1 = box_row(warp + kWarps);
-    auto load_stage = [&](int i) {
+    auto load_stage = [&](int i, int st) {
       if (i < n) {
-        const int st = i % kStages;
         const int k0 = (ch0 + i) * 64, k = k0 + piece * 8;
         if (tid == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)cols * 128);
         if (lane == 0 && box0 >= 0) tma_load_2d(raw + st * stage_bytes + (TML + warp * kBoxRows) * 128, &map_a, &full[st], k0, box0);
@@ -833,31 +846,41 @@ __global__ void __launch_bounds__(kThreads, 2)
         const bool in = k < a.K;
         const bool on_a = in && xa != nullptr, on_b = in && xb != nullptr;
         cp_async16(dst0 + st * stage_bytes, on_a ? xa + k : x, on_a);
-        cp_async16(dst0 + st * stage_bytes + 32 * 128, on_b ? xb + k : x, on_b);
+        cp_async16(dst0 + st * stage_bytes + TML / 2 * 128, on_b ? xb + k : x, on_b);
       }
       cp_async_commit();
     };
-    for (int i = 0; i < kStages - 1; ++i) load_stage(i);
+    auto wait_stage = [&]() {             // all but the youngest stages - 2 copies have arrived
+      if (stages == 3) cp_async_wait<1>();
+      else if (stages == 4) cp_async_wait<2>();
+      else if (stages == 5) cp_async_wait<3>();
+      else cp_async_wait<4>();
+    };
+    for (int i = 0; i < stages - 1; ++i) load_stage(i, i);
     const uint32_t idesc = idesc_bf16_f32(TML, cols);
+    int st = 0, prev = stages - 1;        // slots of chunks i and i - 1, and the parity of their use
+    uint32_t use = 0, prev_use = 1;
     for (int i = 0; i < n; ++i) {
-      cp_async_wait<kStages - 2>();
+      wait_stage();
       fence_proxy_async_smem();
       __syncthreads();
       if (warp == 0 && elect_one()) {
-        mbar_wait(&full[i % kStages], (i / kStages) & 1, 43);
+        mbar_wait(&full[st], use, 43);
         tc_fence_after();
-        const uint32_t st = raw_u + (i % kStages) * stage_bytes;
-        const uint64_t xd = sw128_kmajor_desc(st), ad = sw128_kmajor_desc(st + TML * 128);
+        const uint32_t at = raw_u + st * stage_bytes;
+        const uint64_t xd = sw128_kmajor_desc(at), ad = sw128_kmajor_desc(at + TML * 128);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) umma_f16_ss(tmem, xd + 2 * ks, ad + 2 * ks, idesc, (i | ks) != 0);
-        umma_commit(&empty[i % kStages]);
+        umma_commit(&empty[st]);
       }
       __syncwarp();
-      if (i > 0 && i + kStages - 1 < n) mbar_wait(&empty[(i - 1) % kStages], ((i - 1) / kStages) & 1, 40);
-      load_stage(i + kStages - 1);
+      if (i > 0 && i + stages - 1 < n) mbar_wait(&empty[prev], prev_use, 40);
+      load_stage(i + stages - 1, prev);
+      prev = st, prev_use = use;
+      if (++st == stages) st = 0, use ^= 1;
     }
     // A wait that runs out records an error: the step's results are void, the control flow stays.
-    if (n > 0) mbar_wait(&empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, 41);
+    if (n > 0) mbar_wait(&empty[prev], prev_use, 41);
     cp_async_wait<0>();
     __syncthreads();                      // the ring's memory becomes the partial h
     tc_fence_after();
@@ -869,7 +892,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int xg = 0; xg < 8; ++xg) {
         const int col = c0 + xg * 8 + 2 * c;
         if (col >= cols) continue;
-        float* p = part + (sub * 16 + g) * pld + col;
+        float* p = part + (wrow + g) * pld + col;
         // Past the rank h is zero, whatever the boxes brought; a CTA without a share of K adds zero.
         const int left = n > 0 ? rank - col % rp : 0;
         *reinterpret_cast<float2*>(p) =
@@ -891,51 +914,62 @@ __global__ void __launch_bounds__(kThreads, 2)
       hs_at[q] = cluster_addr(hs, q);
     }
     const int quads = cols / 4, items = kOwn * quads;
-    constexpr int kIn = 16 / CL;          // items whose remote loads are under way together
-    for (int i0 = tid; i0 < items; i0 += kIn * kThreads) {
-      float4 v[kIn][CL];
-      int row[kIn], j[kIn];
+    constexpr int kIn = kOwn * (kLargeCols / 4) / kThreads;   // items of a thread
+    constexpr int kBatch = CL == 2 ? 4 : 2;                   // whose remote loads are under way together
+    uint2 p[kIn][kParts];
 #pragma unroll
-      for (int u = 0; u < kIn; ++u) {
-        const int i = min(i0 + u * kThreads, items - 1);
-        row[u] = i / quads;
-        j[u] = (i - row[u] * quads) * 4;
+    for (int u0 = 0; u0 < kIn; u0 += kBatch) {
+      if (u0 * kThreads >= items) break;
+      float4 v[kBatch][CL];
 #pragma unroll
-        for (int q = 0; q < CL; ++q) v[u][q] = ld_cluster4(part_at[q] + (row[u] * pld + j[u]) * 4);
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = min(tid + (u0 + u) * kThreads, items - 1);
+        const int row = i / quads, j = (i - row * quads) * 4;
+#pragma unroll
+        for (int q = 0; q < CL; ++q) v[u][q] = ld_cluster4(part_at[q] + (row * pld + j) * 4);
       }
 #pragma unroll
-      for (int u = 0; u < kIn; ++u) {
-        if (i0 + u * kThreads >= items) break;
+      for (int u = 0; u < kBatch; ++u) {
 #pragma unroll
         for (int q = 1; q < CL; ++q)
           v[u][0].x += v[u][q].x, v[u][0].y += v[u][q].y, v[u][0].z += v[u][q].z, v[u][0].w += v[u][q].w;
-        uint2 p[kParts];
-        split4<kParts>(v[u][0], p);
-        const int hr = cta * kOwn + row[u];
-        const uint32_t off = (j[u] >> 6) * (TML * 128) + hr * 128 + (((j[u] & 63) >> 3 ^ (hr & 7)) << 4) + (j[u] & 7) * 2;
-#pragma unroll
-        for (int q = 0; q < CL; ++q)
-#pragma unroll
-          for (int s = 0; s < kParts; ++s) st_cluster2(hs_at[q] + s * hpart + off, p[s]);
+        split4<kParts>(v[u][0], p[u0 + u]);
       }
+    }
+    cluster_arrive();                     // all partials have been read: the parts of h take their place
+    cluster_wait();
+#pragma unroll
+    for (int u = 0; u < kIn; ++u) {
+      const int i = tid + u * kThreads;
+      if (i >= items) break;
+      const int row = i / quads, j = (i - row * quads) * 4;
+      const int hr = cta * kOwn + row;
+      const uint32_t off = (j >> 6) * (TML * 128) + hr * 128 + (((j & 63) >> 3 ^ (hr & 7)) << 4) + (j & 7) * 2;
+#pragma unroll
+      for (int q = 0; q < CL; ++q)
+#pragma unroll
+        for (int s = 0; s < kParts; ++s) st_cluster2(hs_at[q] + s * hpart + off, p[u][s]);
     }
   }
   asm volatile("fence.proxy.async;" ::: "memory");   // the tensor cores will read what was just stored
-  cluster_arrive();                       // all parts of h are in place, all partials read
+  cluster_arrive();                       // all parts of h are in place
   cluster_wait();
   asm volatile("fence.proxy.async;" ::: "memory");
 
   // ---- expand
   const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b) + (int64_t)tl.adapter * a.N * a.R;
   const int bstage = kBN * ((a.R + 63) / 64 * 128);
-  const int piece = tid & 7, cfirst = tid >> 3;
+  const uint32_t braw_u = raw_u + smem_b;
+  const int piece = tid & 7, cfirst = tid >> 3 & 31;
+  constexpr int kBi = kWarps / 8;         // groups of 32 columns the threads cover together
+  const int ifirst = kBi == 1 ? 0 : tid >> 8;
   auto load_b = [&](const Block& at, int st) {
     if (at.slice >= 0) {
 #pragma unroll
-      for (int i = 0; i < kBN / 32; ++i) {
+      for (int i = ifirst; i < kBN / 32; i += kBi) {
         // column q * 8 + 2 t + e of 32 is stored as row t * 8 + 2 q + e
         const int lc = cfirst, r = i * 32 + (lc >> 1 & 3) * 8 + (lc >> 3) * 2 + (lc & 1);
-        const uint32_t dst = raw_u + st * bstage + r * 128 + ((piece ^ (r & 7)) << 4);
+        const uint32_t dst = braw_u + st * bstage + r * 128 + ((piece ^ (r & 7)) << 4);
         const int col = at.c0 + i * 32 + lc;
         const __nv_bfloat16* src = B + (int64_t)col * a.R;
         for (int kb = 0; kb < rp; kb += 64) {
@@ -951,13 +985,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto trim_b = [&](int st) {
     if ((rank & 7) == 0 || piece != (rank >> 3 & 7)) return;
 #pragma unroll
-    for (int i = 0; i < kBN / 32; ++i) {
+    for (int i = ifirst; i < kBN / 32; i += kBi) {
       const int lc = cfirst, r = i * 32 + (lc >> 1 & 3) * 8 + (lc >> 3) * 2 + (lc & 1);
-      uint16_t* p = reinterpret_cast<uint16_t*>(raw + st * bstage + (rank >> 6) * (kBN * 128) + r * 128 + ((piece ^ (r & 7)) << 4));
+      uint16_t* p = reinterpret_cast<uint16_t*>(raw + smem_b + st * bstage + (rank >> 6) * (kBN * 128) + r * 128 + ((piece ^ (r & 7)) << 4));
       for (int e = rank & 7; e < 8; ++e) p[e] = 0;
     }
   };
-  const int row0 = tile_rows[sub * 16 + g], row1 = tile_rows[sub * 16 + g + 8];
+  const int row0 = tile_rows[wrow + g], row1 = tile_rows[wrow + g + 8];
   const int es = F32 ? 4 : 2;
   // used where the row exists
   const char* base0 = reinterpret_cast<const char*>(a.base) + ((int64_t)row0 * a.ldb + half * 64 + 8 * c) * es;
@@ -984,7 +1018,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     if (warp == 0 && elect_one()) {
       tc_fence_after();
-      const uint32_t bst = raw_u + (it & 1) * bstage;
+      const uint32_t bst = braw_u + (it & 1) * bstage;
       uint32_t on = 0;
       for (int q = 0; q < kParts; ++q)
         for (int k = 0; k < rp; k += 16) {
@@ -1066,27 +1100,24 @@ void set_blocks(LoraArgs& a) {
 // The small kernel's time grows with the products of its tiles on mma.sync, the
 // large one's with the CTAs' trips over K and with the weights that its tiles
 // read, whatever the rank.  Tiles are estimated from the number of listed rows and
-// of adapters, which is all the host knows.  Over 430 random calls (up to 4096 rows,
+// of adapters, which is all the host knows.  Over 390 random calls (up to 4096 rows,
 // K 512 to 14336, N 768 to 10240, ranks 8 to 128, 1 to 128 adapters) the choice
-// costs 1.8 % over the better one in the mean, 40 % at most; large tiles from a
-// fixed number of rows cost 8 % and up to 3.3 times.  Small / large, bf16, eight
-// adapters, K = 4096, three slices of together 6144 columns: rank 64, 128 rows 19.6 /
-// 24.1 us, 384 rows 29.9 / 25.7, 2048 rows 111 / 41; rank 16, 2048 rows 30.6 / 35.5.
+// costs 1.1 % over the better one in the mean, 50 % at most; large tiles from 768
+// rows cost 7.9 % and up to six times.  Small / large, bf16, eight adapters, K = 4096,
+// three slices of together 6144 columns: rank 64, 128 rows 19.3 / 24.8 us, 384 rows
+// 30.1 / 27.1, 2048 rows 56.5 / 45.3; rank 16, 2048 rows 24.1 / 38.4.
 bool use_large(const LoraArgs& a) {
   if ((int64_t)a.pool * a.S * a.R > INT32_MAX) return false;   // rows of A are 32-bit coordinates
-  const double adapters = std::min(a.L, a.pool);
-  const double small_tiles = a.L / kSmallRows + adapters / 2, large_tiles = a.L / TML + adapters;
+  const double small_tiles = (a.L + kSmallRows - 1) / kSmallRows, large_tiles = a.L / 64 + std::min(a.L, a.pool);
   const double work = small_tiles * a.R * ((double)a.S * a.K + (a.f32 ? 3.0 : 2.0) * a.N);
-  return work >= 105.0 * (32.0 * a.K + large_tiles * ((double)a.K + a.N));
+  return work >= 155.0 * (32.0 * a.K + large_tiles * ((double)a.K + a.N));
 }
 
-int cta_slots() { return 2 * sm_count(); }
-
-// Clusters of `cl` CTAs of a small kernel that run at once.  GPCs hold different
+// Clusters of `cl` CTAs of a kernel that run at once.  GPCs hold different
 // numbers of SMs, so the device is asked, once per kernel, size and CTAs per SM.
 template <typename Kernel>
-int clusters_at_once(Kernel kernel, int cl, size_t smem, std::atomic<int> (&known)[64][2][kCluster + 1]) {
-  const int pair = 2 * (smem + 2048) <= 228 * 1024 ? 1 : 0;       // two CTAs share an SM
+int clusters_at_once(Kernel kernel, int threads, int cl, size_t smem, std::atomic<int> (&known)[64][2][kCluster + 1]) {
+  const int pair = threads == kThreads && 2 * (smem + 2048) <= 228 * 1024 ? 1 : 0;   // two CTAs share an SM
   int dev = 0, n = 0;
   cudaGetDevice(&dev);
   if (cl == 1) return (1 + pair) * sm_count();
@@ -1097,7 +1128,7 @@ int clusters_at_once(Kernel kernel, int cl, size_t smem, std::atomic<int> (&know
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cl);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -1137,7 +1168,7 @@ void launch_small(const LoraArgs& a, cudaStream_t s) {
   allow_smem(reinterpret_cast<const void*>(k), allowed);
   const int tiles = a.L / kSmallRows + std::min(a.L, a.pool);   // at least the sum of ceil(rows / 16) over the adapters
   static std::atomic<int> at_once[64][2][kCluster + 1];
-  const int cl = cluster_size(a, [&](int c) { return clusters_at_once(k, c, smem, at_once); });
+  const int cl = cluster_size(a, [&](int c) { return clusters_at_once(k, kThreads, c, smem, at_once); });
   // one_row() keeps its share of x and h in the same shared memory
   const int64_t span = (((a.K + 31) / 32 + cl - 1) / cl * 32 + 255) / 256 * 256;
   const bool vector = (a.R & (a.R - 1)) == 0 && (span + 2 * cols) * 4 <= (int64_t)smem;
@@ -1161,35 +1192,67 @@ void small(const LoraArgs& a, cudaStream_t s) {
   }
 }
 
-template <bool F32, int CL>
-void launch_large(const LoraArgs& a, int tiles, cudaStream_t s) {
-  const int cols = a.S * ((a.R + 15) / 16 * 16);
-  const LargeSmem sm = large_smem(cols, a.R, F32 ? 3 : 2);
-  auto k = lora_large_kernel<F32, CL>;
-  static std::atomic<unsigned long long> allowed{0};
-  allow_smem(reinterpret_cast<const void*>(k), allowed);
-  const CUtensorMap map_a = gemm::make_tmap_2d(a.a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.pool * a.S_all * a.R, a.K,
-                                               a.K, kBoxRows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
-  launch_k(k, dim3((unsigned)tiles * CL), dim3(kThreads), sm.total, s, (unsigned)CL, a, map_a, cols, (int)sm.hs);
+template <bool F32, int TML, int CL>
+struct Large {
+  LargeSmem sm;
+  int tiles, likely, cols;   // at most and as a rule
+  explicit Large(const LoraArgs& a)
+      : sm(large_smem(TML, a.S * ((a.R + 15) / 16 * 16), a.R, F32 ? 3 : 2)),
+        tiles(a.L / TML + std::min(a.L, a.pool)), likely(a.L / TML + (std::min(a.L, a.pool) + 1) / 2), cols(a.S * ((a.R + 15) / 16 * 16)) {
+    static std::atomic<unsigned long long> allowed{0}, allowed_twin{0};
+    allow_smem(reinterpret_cast<const void*>(lora_large_kernel<F32, TML, CL>), allowed);
+    if (TML == 64) allow_smem(reinterpret_cast<const void*>(kTwin), allowed_twin);
+  }
+  // The device counts one CTA of a kernel with tensor memory per SM, although two of 64
+  // rows do share one: it is asked about a kernel that is alike but for that.
+  static constexpr auto kTwin = lora_small_kernel<F32, 4, true>;
+  int waves() const {
+    static std::atomic<int> at_once[64][2][kCluster + 1];
+    const int n = TML == 64 ? clusters_at_once(kTwin, kThreads, CL, sm.total, at_once)
+                            : clusters_at_once(lora_large_kernel<F32, TML, CL>, TML * 4, CL, sm.total, at_once);
+    return (likely + n - 1) / n;
+  }
+  void launch(const LoraArgs& a, cudaStream_t s) const {
+    const CUtensorMap map_a = gemm::make_tmap_2d(a.a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.pool * a.S_all * a.R, a.K,
+                                                 a.K, kBoxRows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    launch_k(lora_large_kernel<F32, TML, CL>, dim3((unsigned)tiles * CL), dim3(TML * 4), sm.total, s, (unsigned)CL, a, map_a, cols,
+             (int)sm.b, (int)sm.total - 1024);
+  }
+};
+
+// Tile and cluster by the number of waves and what one takes (us, ranks up to 64 beside
+// the QKV projection): 64 rows in clusters of 8 26, 4 45, 2 92; 128 rows in clusters of 4
+// 43, 2 76.
+template <bool F32>
+void launch_large(const LoraArgs& a, cudaStream_t s) {
+  const Large<F32, 64, 8> a8(a);
+  const Large<F32, 64, 4> a4(a);
+  const Large<F32, 64, 2> a2(a);
+  const Large<F32, 128, 4> b4(a);
+  const Large<F32, 128, 2> b2(a);
+  const int64_t us[5] = {26LL * a8.waves(), 45LL * a4.waves(), 92LL * a2.waves(), 43LL * b4.waves(), 76LL * b2.waves()};
+  const int best = (int)(std::min_element(us, us + 5) - us);
+  if (best == 0) a8.launch(a, s);
+  else if (best == 1) a4.launch(a, s);
+  else if (best == 2) a2.launch(a, s);
+  else if (best == 3) b4.launch(a, s);
+  else b2.launch(a, s);
 }
 
-// As many slices per launch as an accumulator holds: all of them up to 256 columns.
-// The largest clusters whose CTAs all run at once: 768 rows of ranks up to 64, 8 25.6
-// us, 4 39.4, 2 67.4; 2048 rows 52.4, 48.9, 67.6; 8192 rows 129, 103, 95.3.
+// As many slices per launch as an accumulator (256 columns) and shared memory hold.
 template <bool F32>
 int large(const LoraArgs& all, cudaStream_t s) {
   int launches = 0;
-  const int step = kLargeCols / ((all.R + 15) / 16 * 16);
-  const int tiles = all.L / TML + std::min(all.L, all.pool);
+  const int rp = (all.R + 15) / 16 * 16;
+  int step = std::min(all.S, kLargeCols / rp);
+  while (step > 1 && large_smem(128, step * rp, all.R, F32 ? 3 : 2).total > kLargeSmem) --step;
   for (int s0 = 0; s0 < all.S; s0 += step) {
     LoraArgs a = all;
     a.s0 = s0;
     a.S = std::min(step, all.S - s0);
     for (int i = 0; i <= kMaxSlices; ++i) a.col_begin[i] = all.col_begin[std::min(s0 + std::min(i, a.S), all.S)];
     set_blocks(a);
-    if ((int64_t)tiles * kCluster <= cta_slots()) launch_large<F32, kCluster>(a, tiles, s);
-    else if ((int64_t)tiles * 4 <= cta_slots()) launch_large<F32, 4>(a, tiles, s);
-    else launch_large<F32, 2>(a, tiles, s);
+    launch_large<F32>(a, s);
     ++launches;
   }
   return launches;
