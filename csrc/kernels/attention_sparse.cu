@@ -994,6 +994,7 @@ void page_bounds(const BoundsArgs& a, cudaStream_t s) {
   b.max_pages = (a.max_new + PAGE - 2) / PAGE + 1;   // from any offset in a page
   if (b.max_pages > a.width) b.max_pages = a.width;
   const int64_t units = (int64_t)a.rows * a.Hkv * b.max_pages;
+  if (units == 0) return;                            // a table without pages
   if (units / 4 >= INT32_MAX) throw std::runtime_error("lunaflux page_bounds: too many pages for one call");
   launch_k(page_bounds_kernel, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, s, 1, b);
 }

@@ -307,6 +307,31 @@ def test_lora_without_rows(ops):
     assert torch.equal(out, d["base"])
 
 
+@pytest.mark.parametrize("T,K,R,counts", [(40, 264, 16, [17, 1, 20]), (1300, 264, 64, [700, 1, 590])])
+def test_lora_row_that_is_not_finite(ops, T, K, R, counts):
+    """An infinity or a NaN in x stays in its row."""
+    slices = (48, 24)
+    v = _lora_inputs(T, K, slices, R, counts, 23, ranks=[R, R - 3, R - 9], integer=False)
+    d = {k: t.to(ops.dev) for k, t in v.items()}
+
+    def run(x):
+        out = d["base"].clone()
+        ops.lora_add(x, d["a"], d["b"], d["scales"], d["ranks"], d["rows"], d["starts"], out, out, slices)
+        return out
+
+    want = run(d["x"])
+    bad = [int(v["rows"][3]), int(v["rows"][counts[0]]), int(v["rows"][-1])]
+    x = d["x"].clone()
+    for r, value in zip(bad, (float("inf"), float("nan"), float("-inf"))):
+        x[r, 5] = value
+    got = run(x)
+    for r in bad:
+        assert not bool(torch.isfinite(got[r]).any())
+    others = torch.ones(T, dtype=torch.bool, device=ops.dev)
+    others[bad] = False
+    assert torch.equal(got[others], want[others])
+
+
 @gpu
 def test_lora_bad_indices_are_recorded(kernels):
     T, K, R, slices = 40, 64, 8, (64,)
@@ -494,6 +519,34 @@ def test_select_takes_pages_that_are_not_finite(ops):
     ws = torch.zeros(max(1, ops.select_workspace(1, Hkv, v["width"])), device=ops.dev)
     ops.attn_select(d["q"], d["tok"], d["lens"], d["bt"], d["bounds"], sel, 0, 1, Hq, Hkv, ws)
     assert {30, 50, 70, 89} <= set(sel[0, 0].tolist())
+
+
+def test_select_first_and_last_fill_the_budget(ops):
+    Hq, Hkv, lens = 4, 2, [16 * 40 + 1, 16 * 3, 5]
+    v = _paged(lens, Hq, Hkv, 9)
+    d = {k: t.to(ops.dev) if torch.is_tensor(t) else t for k, t in v.items()}
+    for first, last in ((1, 2), (3, 0), (0, 3)):
+        sel = torch.zeros(3, Hkv, 3, dtype=I32, device=ops.dev)
+        ws = torch.zeros(max(1, ops.select_workspace(3, Hkv, v["width"])), device=ops.dev)
+        ops.attn_select(d["q"], d["tok"], d["lens"], d["bt"], d["bounds"], sel, first, last, Hq, Hkv, ws)
+        assert torch.equal(sel.cpu(), _select_reference(v, Hq, Hkv, 3, first, last))
+    _no_error(ops)
+
+
+def test_sparse_step_without_pages(ops):
+    """A block table without columns: every row is empty."""
+    Hq, Hkv = 4, 2
+    z = lambda *s, dtype=BF: torch.zeros(*s, dtype=dtype, device=ops.dev)  # noqa: E731
+    kc, bounds = torch.ones(2, Hkv, 16, 128, dtype=BF, device=ops.dev), z(2, Hkv, 2, 128)
+    bt, lens, tok = z(3, 0, dtype=I32), z(3, dtype=I32), torch.arange(3, dtype=I32, device=ops.dev)
+    ops.page_bounds(kc, bounds, bt, lens, lens, 1)
+    assert not bool(bounds.any())
+    q, out, sel = torch.ones(3, Hq * 128, dtype=BF, device=ops.dev), torch.ones(3, Hq * 128, dtype=BF, device=ops.dev), z(3, Hkv, 2, dtype=I32)
+    ops.attn_select(q, tok, lens, bt, bounds, sel, 0, 1, Hq, Hkv, z(1, dtype=F32))
+    assert bool((sel == -1).all())
+    ops.attn_decode_sparse(q, out, tok, lens, bt, sel, kc, kc, Hq, Hkv)
+    assert not bool(out.any())
+    _no_error(ops)
 
 
 def test_sparse_with_every_page_is_dense(ops):

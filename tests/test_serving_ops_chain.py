@@ -207,3 +207,33 @@ def test_launch_checks_admit_the_layer(monkeypatch):
     sel, ws = _buffers(d, width, ops, 4)
     _run(ops, d, sel, ws, 4)
     assert ops.admitted == 8 and ops.read_error(True)[0] == 0
+
+
+_FIRST_CALL = """
+import torch
+from lunaflux_b200.ops import KernelOps
+from tests.test_serving_ops import _lora_inputs, _lora_reference, BF
+ops = KernelOps()
+for T, K, slices, R, counts in ((3, 256, (64, 32), 16, [1, 2]), (1300, 136, (72,), 64, [600, 700]),
+                                (2600, 136, (40, 32), 64, [65] * 40)):
+    v = _lora_inputs(T, K, slices, R, counts, T)
+    d = {k: t.cuda() for k, t in v.items()}
+    out = torch.zeros_like(d["base"])
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=s):
+        ops.lora_add(d["x"], d["a"], d["b"], d["scales"], d["ranks"], d["rows"], d["starts"], d["base"], out, slices)
+    g.replay()
+    torch.cuda.synchronize()
+    rows = v["rows"].long()
+    assert torch.equal(out.cpu()[rows], _lora_reference(v, slices, R)[0].to(BF)[rows])
+print("captured")
+"""
+
+
+def test_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+    p = subprocess.run([sys.executable, "-c", _FIRST_CALL], cwd=Path(__file__).resolve().parent.parent, timeout=300,
+                       capture_output=True, text=True)
+    assert p.returncode == 0 and "captured" in p.stdout, p.stderr[-2000:]
