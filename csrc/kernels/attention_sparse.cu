@@ -1033,11 +1033,13 @@ namespace {
 template <int NH, int W>
 void launch_decode(const SparseArgs& a, cudaStream_t s) {
   const int64_t units = (int64_t)a.rows * a.Hkv;
-  // CTAs per unit: as many as run at the same time (16 warps per SM, 8 for wide
-  // groups) and get two pages per warp
+  // CTAs per unit: as many as run at the same time (16 warps per SM, 8 for wide groups)
+  // and get two pages per warp; two also where only half of them run at once, because
+  // one CTA with a long row would outlast the others of a ragged batch (64 rows of 1 to 32768
+  // tokens x 8 heads x 128 pages: a step takes 77 us, 96 with one; all of 32768: 194, 189).
   const int64_t slots = (int64_t)sm_count() * ((NH == 1 ? 16 : 8) / W);
   int cl = 1;
-  while (cl < kMaxCluster && units * cl * 2 <= slots && a.budget > W * cl) cl *= 2;
+  while (cl < kMaxCluster && units * cl * 2 <= (cl == 1 ? 2 : 1) * slots && a.budget > W * cl) cl *= 2;
   auto k = decode_sparse_kernel<NH, W>;
   static std::atomic<unsigned long long> allowed{0};
   allow_smem(reinterpret_cast<const void*>(k), allowed);
