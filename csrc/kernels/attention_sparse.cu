@@ -724,7 +724,7 @@ __global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
 // values, so the rounding does not scale the output.
 //
 // 16 warps per SM have a page each under way; 64 rows x 8 heads x 128 pages read
-// 537 MB in 84 us, 6.4 TB/s.  A page ahead in registers halves the warps, and per-lane
+// 537 MB in 89 us, 6.0 TB/s (84 with one CTA per row and head).  A page ahead in registers halves the warps, and per-lane
 // cp.async delivers less than plain loads: both were slower.
 // ===========================================================================
 constexpr int kMaxCluster = 8;
@@ -1021,8 +1021,11 @@ int select_pages(const SelectArgs& a, cudaStream_t s) {
   }
   // As few threads and pages per thread as hold the block table: 8191 tokens 14.1 us
   // a step, 16.2 with <256, 8>, 20.4 with <1024, 8>; 64 rows of 32768 tokens 188 us, 212
-  // with <1024, 8>, 303 with the general routine.
+  // with <1024, 8>, 303 with the general routine.  Where every CTA has an SM for itself
+  // 512 threads for 2048 pages (one row of 32768 tokens 17.4 us, 18.2 with 256; 64 rows
+  // 197, 194).
   if (a.width <= 512) launch_select<256, 2>(a, s);
+  else if (a.width <= 2048 && (int64_t)a.rows * a.Hkv <= sm_count()) launch_select<512, 4>(a, s);
   else if (a.width <= 2048) launch_select<256, 8>(a, s);
   else if (a.width <= 8192) launch_select<1024, 8>(a, s);
   else launch_select<1024, 0>(a, s);

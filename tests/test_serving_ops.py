@@ -444,6 +444,11 @@ SPARSE = [
     ([3000, 17, 2999, 16, 100, 1600], 32, 8, 40, 1, 2),
     ([9000], 2, 2, 129, 1, 1),
     ([40] * 50, 4, 4, 2, 0, 1),
+    # 512 to 2048 pages in few and in many rows x heads; two CTAs per row and head where not all run at once
+    ([16 * 700 + 3, 16 * 1030], 8, 2, 20, 1, 2),
+    ([16 * 1100 - 5] + [1 + 37 * i for i in range(39)], 8, 8, 24, 0, 1),
+    # eight-warp CTAs for more rows: a large budget
+    ([16 * 200 + i for i in range(25)], 4, 1, 130, 1, 1),
 ]
 
 
