@@ -1221,21 +1221,19 @@ struct Large {
 };
 
 // Tile and cluster by the number of waves and what one takes (us, ranks up to 64 beside
-// the QKV projection): 64 rows in clusters of 8 26, 4 45, 2 92; 128 rows in clusters of 4
-// 43, 2 76.
+// the QKV projection): 64 rows in clusters of 8 26, 4 45 (of 2 92, no better than two
+// waves of 4); 128 rows in clusters of 4 43, 2 76.
 template <bool F32>
 void launch_large(const LoraArgs& a, cudaStream_t s) {
   const Large<F32, 64, 8> a8(a);
   const Large<F32, 64, 4> a4(a);
-  const Large<F32, 64, 2> a2(a);
   const Large<F32, 128, 4> b4(a);
   const Large<F32, 128, 2> b2(a);
-  const int64_t us[5] = {26LL * a8.waves(), 45LL * a4.waves(), 92LL * a2.waves(), 43LL * b4.waves(), 76LL * b2.waves()};
-  const int best = (int)(std::min_element(us, us + 5) - us);
+  const int64_t us[4] = {26LL * a8.waves(), 45LL * a4.waves(), 43LL * b4.waves(), 76LL * b2.waves()};
+  const int best = (int)(std::min_element(us, us + 4) - us);
   if (best == 0) a8.launch(a, s);
   else if (best == 1) a4.launch(a, s);
-  else if (best == 2) a2.launch(a, s);
-  else if (best == 3) b4.launch(a, s);
+  else if (best == 2) b4.launch(a, s);
   else b2.launch(a, s);
 }
 

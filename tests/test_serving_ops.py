@@ -225,7 +225,10 @@ LORA_SHAPES = [
     (1000, 264, (128, 64), 128, [500, 500], [128, 100]),
     (800, 328, (64, 8, 72, 64), 128, [31, 33, 736], [128, 50, 121]),
     (770, 8, (8,), 40, [769], [33]),
-    # tiles in clusters of four and of two CTAs
+    # 64-row tiles in clusters of four, 128-row tiles in clusters of four and of two
+    (3000, 136, (72,), 64, [1500, 1, 1499], [64, 40, 7]),
+    (3000, 72, (64, 64), 128, [1400, 1500], [128, 101]),
+    (6000, 136, (40, 32), 64, [3000, 2000, 900], [64, 33, 16]),
     (1300, 136, (72,), 64, [50] * 20 + [0] * 5 + [60] * 5, [64, 1, 33, 0, 17, 48] * 5),
     (2600, 136, (40, 32), 64, [65] * 40, [(7 * i) % 65 for i in range(40)]),
 ]
