@@ -718,10 +718,9 @@ __global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
 // the A operand directly (16 bytes = eight dimensions = two k-steps).  V^T needs
 // two tokens side by side: a lane reads the same eight dimensions of two tokens
 // and interleaves them with byte permutes; row g of tile t is dimension 8g + t.
-// P^T comes from S^T by an 8 x 8 register transpose.  P is rounded to bf16 for
-// the tensor cores, an error of at most 2^-8 of each weight that averages over
-// the tokens; the sum of the weights is kept in fp32 from the same rounded
-// values, so the rounding does not scale the output.
+// P^T comes from S^T by an 8 x 8 register transpose.  The tensor cores take P as
+// two bf16 parts, which hold each weight to 2^-16; with one part (2^-8) the output
+// would be off by up to 2^-8 of sum p |v|, however small the mean itself is.
 //
 // 16 warps per SM have a page each under way; 64 rows x 8 heads x 128 pages read
 // 537 MB in 89 us, 6.0 TB/s (84 with one CTA per row and head).  A page ahead in registers halves the warps, and per-lane
@@ -803,8 +802,7 @@ __global__ void __launch_bounds__(W * 32, (NH == 1 ? 16 : 8) / W) decode_sparse_
 
   // a lane's pieces of a page: K rows g and g + 8, pieces c, c + 4, ...; V rows 2c,
   // 2c + 1, 2c + 8, 2c + 9, piece g of both halves of the dimensions
-  const __nv_bfloat16* kl = a.kcache + (int64_t)kvh * PAGE * D + g * D + c * 8;
-  const __nv_bfloat16* vl = a.vcache + (int64_t)kvh * PAGE * D + 2 * c * D + g * 8;
+  const int kl = g * D + c * 8, vl = 2 * c * D + g * 8;
   const int64_t page_elems = (int64_t)a.Hkv * PAGE * D;
   uint4 k0[4], k1[4], v[2][4];          // v[half of the dimensions][token 2c, 2c + 1, 2c + 8, 2c + 9]
   int t0 = L, t0_next = L;
@@ -812,13 +810,13 @@ __global__ void __launch_bounds__(W * 32, (NH == 1 ? 16 : 8) / W) decode_sparse_
   auto locate = [&](int i) {            // page i of this warp
     if ((i & 31) == 0) open_window(i);
     t0_next = __shfl_sync(kFull, win_tok, i & 31);
-    at = __shfl_sync(kFull, win_phys, i & 31) * page_elems;
+    at = __shfl_sync(kFull, win_phys, i & 31) * page_elems + kvh * (PAGE * D);
   };
   auto load_k = [&]() {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      k0[j] = ld_stream(kl + at + j * 32);
-      k1[j] = ld_stream(kl + at + 8 * D + j * 32);
+      k0[j] = ld_stream(a.kcache + (at + kl) + j * 32);
+      k1[j] = ld_stream(a.kcache + (at + kl) + 8 * D + j * 32);
     }
   };
   auto load_v = [&]() {
@@ -826,8 +824,8 @@ __global__ void __launch_bounds__(W * 32, (NH == 1 ? 16 : 8) / W) decode_sparse_
     for (int x = 0; x < 4; ++x) {
       const int t = (x & 1) + (x >> 1) * 8;
       const bool on = t0_next + 2 * c + t < L;      // zeros past the sequence's end
-      v[0][x] = on ? ld_stream(vl + at + t * D) : make_uint4(0u, 0u, 0u, 0u);
-      v[1][x] = on ? ld_stream(vl + at + t * D + 64) : make_uint4(0u, 0u, 0u, 0u);
+      v[0][x] = on ? ld_stream(a.vcache + (at + vl) + t * D) : make_uint4(0u, 0u, 0u, 0u);
+      v[1][x] = on ? ld_stream(a.vcache + (at + vl) + t * D + 64) : make_uint4(0u, 0u, 0u, 0u);
     }
   };
   uint4 q[NH][4];
@@ -864,7 +862,7 @@ __global__ void __launch_bounds__(W * 32, (NH == 1 ? 16 : 8) / W) decode_sparse_
         mma_bf16(s[t][1], k0[j].z, k1[j].z, k0[j].w, k1[j].w, q[t][j].z, q[t][j].w);
       }
     }
-    uint32_t p[NH][2];
+    uint32_t p[NH][2][2];               // [part][tokens 0 to 7, 8 to 15]
 #pragma unroll
     for (int t = 0; t < NH; ++t) {
       // x[0], x[1]: token g, heads 2c, 2c + 1; x[2], x[3]: token g + 8
@@ -889,12 +887,14 @@ __global__ void __launch_bounds__(W * 32, (NH == 1 ? 16 : 8) / W) decode_sparse_
 #pragma unroll
         for (int i8 = 0; i8 < 8; ++i8) o[t][i8][e] *= al, o[t][i8][e + 2] *= al;
       }
-      const uint32_t plo = pack_bf16x2(pr[0], pr[1]), phi = pack_bf16x2(pr[2], pr[3]);
-      const float2 f0 = __bfloat1622float2(as_bf2(plo)), f1 = __bfloat1622float2(as_bf2(phi));
-      l[t][0] += f0.x + f1.x;
-      l[t][1] += f0.y + f1.y;
-      p[t][0] = movmatrix_trans(plo);
-      p[t][1] = movmatrix_trans(phi);
+      l[t][0] += pr[0] + pr[2];
+      l[t][1] += pr[1] + pr[3];
+      const uint32_t b0 = pack_bf16x2(pr[0], pr[1]), b1 = pack_bf16x2(pr[2], pr[3]);
+      const float2 f0 = __bfloat1622float2(as_bf2(b0)), f1 = __bfloat1622float2(as_bf2(b1));
+      p[t][0][0] = movmatrix_trans(b0);
+      p[t][0][1] = movmatrix_trans(b1);
+      p[t][1][0] = movmatrix_trans(pack_bf16x2(pr[0] - f0.x, pr[1] - f0.y));
+      p[t][1][1] = movmatrix_trans(pack_bf16x2(pr[2] - f1.x, pr[3] - f1.y));
     }
     const uint32_t* vw = reinterpret_cast<const uint32_t*>(v);   // [half][token][word]
 #pragma unroll
@@ -906,7 +906,10 @@ __global__ void __launch_bounds__(W * 32, (NH == 1 ? 16 : 8) / W) decode_sparse_
       const uint32_t a2 = __byte_perm(vw[2 * 4 + wd], vw[3 * 4 + wd], sel2);
       const uint32_t a3 = __byte_perm(vw[16 + 2 * 4 + wd], vw[16 + 3 * 4 + wd], sel2);
 #pragma unroll
-      for (int t = 0; t < NH; ++t) mma_bf16(o[t][i8], a0, a1, a2, a3, p[t][0], p[t][1]);
+      for (int t = 0; t < NH; ++t) {
+        mma_bf16(o[t][i8], a0, a1, a2, a3, p[t][1][0], p[t][1][1]);
+        mma_bf16(o[t][i8], a0, a1, a2, a3, p[t][0][0], p[t][0][1]);
+      }
     }
   }
 

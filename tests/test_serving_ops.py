@@ -575,6 +575,32 @@ def test_sparse_with_every_page_is_dense(ops):
     _attend_check(dense, v, sel.cpu(), Hq, Hkv)
 
 
+@pytest.mark.parametrize("lens,Hq,Hkv,budget", [([2, 3, 16, 17, 40], 8, 1, 3), ([33, 2, 100], 12, 1, 7),
+                                                ([90, 48, 7], 16, 4, 4), ([30, 31], 32, 2, 2)])
+def test_sparse_weights_are_not_rounded(ops, lens, Hq, Hkv, budget):
+    """Values of both signs, whose weighted mean is far smaller than its terms: weights
+    rounded to 8 bits move it by up to 2^-8, which the output's own rounding does not hide."""
+    v = _paged(lens, Hq, Hkv, 31 + Hq)
+    g = _gen(32)
+    # one dimension carries the logits: the products are exact in fp32, |log2 weight| <= 8 * 4 / 11.3 * 1.45 < 5
+    v["q"][:] = 0
+    v["q"][:, :Hq * 128:128] = torch.randint(1, 9, (v["q"].shape[0], Hq), generator=g).to(BF)
+    v["kc"][:] = 0
+    v["kc"][..., 0] = (torch.randint(0, 129, v["kc"].shape[:3], generator=g) / 32).to(BF)
+    v["vc"] = torch.where(torch.rand(v["vc"].shape, generator=g) < 0.5, -1.0, 1.0).to(BF)
+    d = {k: t.to(ops.dev) if torch.is_tensor(t) else t for k, t in v.items()}
+    sel = torch.full((len(lens), Hkv, budget), -1, dtype=I32)
+    for r, n in enumerate(lens):
+        count = min(-(-n // 16), budget)
+        sel[r, :, :count] = torch.arange(-(-n // 16) - count, -(-n // 16), dtype=I32)
+    out = torch.zeros(d["q"].shape[0], Hq * 128, dtype=BF, device=ops.dev)
+    ops.attn_decode_sparse(d["q"], out, d["tok"], d["lens"], d["bt"], sel.to(ops.dev), d["kc"], d["vc"], Hq, Hkv)
+    ref, mag = _attend_reference(v, sel, Hq, Hkv)
+    # a weight: its logit 5 * 2^-23, the exponential 2^-22, two bf16 parts 2^-16; a weighted sum over at most 7 steps
+    # of 16 tokens in two parts, 17 * 2^-23 each; the sum of weights less: under 2^-14 of sum p |v| + |out| in all
+    _within(out[v["tok"].long().to(out.device)], ref, 2.0 ** -8 * ref.abs() + 2.0 ** -14 * (mag + ref.abs()), "attention")
+
+
 @pytest.mark.parametrize("lens", [[16 * 20000 + 3], [16 * 9000, 16 * 3]])
 @gpu
 def test_select_long_rows(kernels, lens):
