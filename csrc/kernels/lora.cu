@@ -739,6 +739,32 @@ constexpr int kTmemCols = 256;
 constexpr int kBoxRows = 16;             // rows of A per box
 constexpr int kBN = 128;                 // columns of a block of the expansion
 
+// Waits of the large kernel.  Unlike mbar_wait() they are not cut short by an error that is
+// already recorded: a bad row or rank of one tile must not void the copies and products of
+// the others.  A thread whose wait runs out (kErrMbarTimeout) loads nothing more, hardly waits
+// again (`gave_up`) and goes on through the barriers; what it has not loaded is not multiplied,
+// what is not multiplied is not loaded over, so the CTA comes to rest.  Behind the loops
+// it waits for what is under way (drained(): a second at least, whatever the limit is
+// set to) before the memory is used again or freed.  Its shares of h become NaN, its
+// columns are not written.
+__device__ __forceinline__ bool arrived(uint64_t* bar, uint32_t parity, uint32_t where, bool gave_up = false) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((++spins & 255u) == 0 && (gave_up || globaltimer_ns() - t0 > wait_limit_ns())) {
+      set_error(kErrMbarTimeout, (unsigned long long)where);
+      return false;
+    }
+  }
+}
+__device__ __noinline__ void drained(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns(), limit = max(wait_limit_ns(), (uint64_t)1000000000);
+  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 <= limit) {
+  }
+}
+
 // 16 lanes x 8 groups of 8 columns: r[4 x + 0 / 1] = row g, columns 8 x + 2 c, + 1;
 // r[4 x + 2 / 3] = row g + 8.
 __device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t (&r)[32]) {
@@ -779,8 +805,9 @@ __global__ void __launch_bounds__(TML * 4, 128 / TML)
   constexpr int kParts = F32 ? 3 : 2;
   extern __shared__ __align__(128) uint8_t raw_unaligned[];
   __shared__ int tile_rows[TML];
-  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done[2];
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done[2], rest;
   __shared__ uint32_t tmem_base;
+  __shared__ int loaded_most, multiplied_to;
   uint8_t* raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -802,10 +829,14 @@ __global__ void __launch_bounds__(TML * 4, 128 / TML)
     tmem_relinquish();
   }
   if (tid == 0) {
-    for (int i = 0; i < kMaxStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    // a stage of A is complete when every warp's boxes of it are
+    const int box_warps = max(1, min(kWarps, cols / kBoxRows));
+    for (int i = 0; i < kMaxStages; ++i) mbar_init(&full[i], box_warps), mbar_init(&empty[i], 1);
     mbar_init(&done[0], 1);
     mbar_init(&done[1], 1);
+    mbar_init(&rest, 1);
     fence_barrier_init();
+    loaded_most = 0;
   }
 
   // ---- shrink
@@ -820,6 +851,7 @@ __global__ void __launch_bounds__(TML * 4, 128 / TML)
   const int wrow = TML == 64 ? (warp & 3) * 16 : (warp & 3) * 32 + (warp >> 2 & 1) * 16;
   const int half = warp / (kWarps / 2);
   const uint32_t tmem_row = tmem + ((uint32_t)(TML == 64 ? wrow * 2 : wrow) << 16);
+  bool ok;                                // no wait of this CTA's has run out, later of this thread's
   {
     const int chunks = (a.K + 63) / 64;
     const int per_cta = (chunks + CL - 1) / CL;
@@ -838,10 +870,11 @@ __global__ void __launch_bounds__(TML * 4, 128 / TML)
       return j < cols ? first_row + s * a.R + j - s * rp : -1;
     };
     const int box0 = box_row(warp), box1 = box_row(warp + kWarps);
+    int loads = n, products = n;          // chunks this thread loads and, the one that does, multiplies without a gap
     auto load_stage = [&](int i, int st) {
-      if (i < n) {
+      if (i < loads) {
         const int k0 = (ch0 + i) * 64, k = k0 + piece * 8;
-        if (tid == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)cols * 128);
+        if (lane == 0 && box0 >= 0) mbar_arrive_expect_tx(&full[st], (box1 >= 0 ? 2 : 1) * kBoxRows * 128);
         if (lane == 0 && box0 >= 0) tma_load_2d(raw + st * stage_bytes + (TML + warp * kBoxRows) * 128, &map_a, &full[st], k0, box0);
         if (lane == 0 && box1 >= 0)
           tma_load_2d(raw + st * stage_bytes + (TML + (warp + kWarps) * kBoxRows) * 128, &map_a, &full[st], k0, box1);
@@ -866,30 +899,53 @@ __global__ void __launch_bounds__(TML * 4, 128 / TML)
       wait_stage();
       fence_proxy_async_smem();
       __syncthreads();
-      if (warp == 0 && elect_one()) {
-        mbar_wait(&full[st], use, 43);
-        tc_fence_after();
-        const uint32_t at = raw_u + st * stage_bytes;
-        const uint64_t xd = sw128_kmajor_desc(at), ad = sw128_kmajor_desc(at + TML * 128);
+      if (warp == 0 && elect_one()) {     // (a further condition here costs 4 us)
+        if (arrived(&full[st], use, 43, products < n)) {
+          tc_fence_after();
+          const uint32_t at = raw_u + st * stage_bytes;
+          const uint64_t xd = sw128_kmajor_desc(at), ad = sw128_kmajor_desc(at + TML * 128);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) umma_f16_ss(tmem, xd + 2 * ks, ad + 2 * ks, idesc, (i | ks) != 0);
-        umma_commit(&empty[st]);
+          for (int ks = 0; ks < 4; ++ks) umma_f16_ss(tmem, xd + 2 * ks, ad + 2 * ks, idesc, (i | ks) != 0);
+          umma_commit(&empty[st]);
+        } else {
+          products = min(products, i);
+          loads = min(loads, i + stages - 1);
+        }
       }
       __syncwarp();
-      if (i > 0 && i + stages - 1 < n) mbar_wait(&empty[prev], prev_use, 40);
+      if (i > 0 && i + stages - 1 < loads && !arrived(&empty[prev], prev_use, 40)) loads = i + stages - 1;
       load_stage(i + stages - 1, prev);
       prev = st, prev_use = use;
       if (++st == stages) st = 0, use ^= 1;
     }
-    // A wait that runs out records an error: the step's results are void, the control flow stays.
-    if (n > 0) mbar_wait(&empty[prev], prev_use, 41);
+    ok = n == 0 || (loads == n && products == n && arrived(&empty[prev], prev_use, 41));
     cp_async_wait<0>();
-    __syncthreads();                      // the ring's memory becomes the partial h
+    ok = __syncthreads_and(ok);           // the ring's memory becomes the partial h
+    if (!ok) {
+      // Warps that gave up later than others have loaded up to a ring's length more: those stages are
+      // completed by plain arrivals.  Then every stage not multiplied, and the products.
+      const bool boxes = lane == 0 && box0 >= 0;
+      if (boxes) atomicMax(&loaded_most, loads);
+      if (warp == 0 && elect_one()) {
+        multiplied_to = products;
+        umma_commit(&rest);
+      }
+      __syncthreads();
+      if (boxes)
+        for (int c = loads; c < loaded_most; ++c) mbar_arrive(&full[c % stages]);
+      for (int c = multiplied_to; c < loaded_most; ++c) drained(&full[c % stages], c / stages & 1);
+      drained(&rest, 0);
+      __syncthreads();
+    }
     tc_fence_after();
     for (int c0 = half * 64; c0 < cols; c0 += 128) {
       uint32_t r[32];
       tmem_ld_16x256b_x8(tmem_row + c0, r);
       tmem_wait_ld();
+      if (!ok) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) r[e] = 0x7fffffffu;
+      }
 #pragma unroll
       for (int xg = 0; xg < 8; ++xg) {
         const int col = c0 + xg * 8 + 2 * c;
@@ -993,7 +1049,7 @@ __global__ void __launch_bounds__(TML * 4, 128 / TML)
       for (int e = rank & 7; e < 8; ++e) p[e] = 0;
     }
   };
-  const int row0 = tile_rows[wrow + g], row1 = tile_rows[wrow + g + 8];
+  int row0 = tile_rows[wrow + g], row1 = tile_rows[wrow + g + 8];
   const int es = F32 ? 4 : 2;
   // used where the row exists
   const char* base0 = reinterpret_cast<const char*>(a.base) + ((int64_t)row0 * a.ldb + half * 64 + 8 * c) * es;
@@ -1036,7 +1092,8 @@ __global__ void __launch_bounds__(TML * 4, 128 / TML)
   };
   // While block `it` is added to base and written, the product of the next one runs
   // and the copy of the one after it is under way.
-  int block = cta;
+  const bool shrunk = ok;
+  int block = ok ? cta : a.block128[kMaxSlices];
   Block at = column_block<kBN>(a, block), next = column_block<kBN>(a, block + CL);
   BaseCols<F32> bs[2][2], bs_next[2][2];
   load_b(at, 0);
@@ -1052,7 +1109,10 @@ __global__ void __launch_bounds__(TML * 4, 128 / TML)
       cp_async_wait<0>();
       multiply(next, it + 1);             // its accumulator was read before this barrier
     }
-    mbar_wait(&done[it & 1], (it >> 1) & 1, 42);
+    if (!arrived(&done[it & 1], (it >> 1) & 1, 42, !ok)) {
+      ok = false;                         // what follows is void and is not written
+      row0 = row1 = -1;
+    }
     __syncwarp();
     tc_fence_after();
     block += CL;
@@ -1086,7 +1146,11 @@ __global__ void __launch_bounds__(TML * 4, 128 / TML)
   }
   cp_async_wait<0>();
   tc_fence_before();
-  __syncthreads();
+  if (!__syncthreads_and(ok)) {
+    if (warp == 0 && elect_one()) umma_commit(&rest);
+    drained(&rest, shrunk ? 0 : 1);
+    __syncthreads();
+  }
   if (warp == 0) tmem_dealloc(tmem, kTmemCols);
 }
 

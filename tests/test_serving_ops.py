@@ -354,6 +354,47 @@ def test_lora_bad_indices_are_recorded(kernels):
         assert kernels.read_error(True)[0] == 3, what
 
 
+@gpu
+@pytest.mark.parametrize("T,K,slices,R,counts,ranks", [
+    (1300, 264, (72, 64), 64, [700, 590], [64, 41]),                      # 64-row tiles
+    (3000, 520, (72,), 64, [1500, 1, 1400], [64, 40, 7]),                 # clusters of four
+    (6000, 136, (40, 32), 64, [3000, 2000, 900], [64, 33, 16])])          # 128-row tiles
+@pytest.mark.parametrize("f32", [False, True])
+def test_lora_large_tiles_with_a_recorded_error(kernels, T, K, slices, R, counts, ranks, f32):
+    """A bad row, offset or rank leaves the other rows' values as they are, in the call that
+    records it and in the calls after it until the host has read the error."""
+    for what in ("row", "negative", "starts", "rank"):
+        v = _lora_inputs(T, K, slices, R, counts, 29, ranks, f32)
+        ref, _ = _lora_reference(v, slices, R)
+        good = {k: t.cuda() for k, t in v.items()}
+        spoilt = torch.zeros(T, dtype=torch.bool)
+        last = v["rows"][int(v["starts"][-2]):].long()
+        if what == "row":
+            spoilt[int(v["rows"][5])] = True
+            v["rows"][5] = T
+        elif what == "negative":
+            spoilt[int(v["rows"][counts[0] - 1])] = True
+            v["rows"][counts[0] - 1] = -1
+        elif what == "starts":
+            spoilt[last] = True
+            v["starts"][-1] = sum(counts) + 1
+        else:
+            spoilt[last] = True
+            v["ranks"][-1] = R + 1
+        d = {k: t.cuda() for k, t in v.items()}
+
+        def run(d):
+            out = d["base"].clone()
+            kernels.lora_add(d["x"], d["a"], d["b"], d["scales"], d["ranks"], d["rows"], d["starts"], out, out, slices)
+            return out.cpu()
+
+        bad, after = run(d), run(good)
+        assert torch.equal(bad[~spoilt], ref.to(bad.dtype)[~spoilt]), what
+        assert torch.equal(bad[spoilt], v["base"][spoilt]), what
+        assert torch.equal(after, ref.to(after.dtype)), what
+        assert kernels.read_error(True)[0] == 3, what
+
+
 # ---------------------------------------------------------------------------
 # attention over selected pages
 # ---------------------------------------------------------------------------
