@@ -371,6 +371,7 @@ __device__ __noinline__ void select_general(const SelectArgs& a, const SelectUni
   float sk = INFINITY, lower = INFINITY, upper = -INFINITY;
   __syncthreads();
   if (tid < 4) sm.cnt[tid] = 0, sm.totals[tid] = 0;
+  __syncthreads();                      // no place to give out (k = 0): nothing below waits before the counts
   if (u.k > 0) {
     uint32_t kmin = 0xffffffffu, kmax = 0u, lo, hi;
     for (int p = u.first + tid; p < u.mid1; p += NT) {

@@ -662,6 +662,25 @@ def test_select_long_rows(kernels, lens):
     _no_error(kernels)
 
 
+@pytest.mark.parametrize("first,last", [(5, 7), (12, 0), (0, 12)])
+@gpu
+def test_select_long_rows_without_a_free_place(kernels, first, last):
+    """More pages than the selection holds in registers, and the first and last ones fill the budget."""
+    Hq, Hkv, budget, lens = 8, 2, 12, [16 * 8300 + 1, 16 * 12000, 16 * 11, 16 * 13, 16 * 9000 - 3]
+    v = _paged(lens, Hq, Hkv, 40)
+    d = {k: t.cuda() if torch.is_tensor(t) else t for k, t in v.items()}
+    R = len(lens)
+    kernels.page_bounds(d["kc"], d["bounds"], d["bt"], torch.zeros(R, dtype=I32, device="cuda"), d["lens"], max(lens))
+    v["bounds"] = d["bounds"].cpu()
+    ws = torch.zeros(kernels.select_workspace(R, Hkv, v["width"]), device="cuda")
+    want = _select_reference(v, Hq, Hkv, budget, first, last)
+    for _ in range(3):
+        sel = torch.full((R, Hkv, budget), 99, dtype=I32, device="cuda")
+        kernels.attn_select(d["q"], d["tok"], d["lens"], d["bt"], d["bounds"], sel, first, last, Hq, Hkv, ws)
+        assert torch.equal(sel.cpu(), want)
+    _no_error(kernels)
+
+
 @gpu
 def test_sparse_bad_indices_are_recorded(kernels):
     """Bad pages, list entries, tokens and lengths: an error code, other rows unharmed."""
