@@ -19,9 +19,10 @@
 // The order of the scores is that of the exact sums.  bf16 products are exact
 // in fp32; their fp32 sums carry an error bound e = kScoreErr * sum|terms|, and
 // where the bounds of two pages around the cut overlap, both are summed again
-// in fp64.  A score that is not finite (a page or query that holds an infinity
-// or a NaN) counts as +infinity, so such a page is taken and shows up in the
-// output as it would without the selection.
+// in fp64.  Where a page or query holds an infinity or a NaN the score counts as
+// +infinity, so such a page is taken and shows up in the output as it would without the
+// selection; where only the fp32 sums overflow, the error bound is infinite and the
+// page compared in fp64.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -220,6 +221,7 @@ __global__ void __launch_bounds__(kThreads, NH == 1 ? 4 : 2) page_score_kernel(c
       q[t][j] = t * 8 + g < G ? *reinterpret_cast<const uint4*>(qh + 8 * (c + 4 * j)) : make_uint4(0u, 0u, 0u, 0u);
   }
   float2* ws = a.ws + ((int64_t)r * a.Hkv + kvh) * a.width;
+  float odd = 0.f;                        // infinite where a score was not finite
   auto score = [&](int it, const Tile& tile) {
     const int p0 = begin + it * kScoreTile;
     float best_a = -INFINITY, best_b = -INFINITY, err_a = 0.f, err_b = 0.f;
@@ -251,8 +253,8 @@ __global__ void __launch_bounds__(kThreads, NH == 1 ? 4 : 2) page_score_kernel(c
           const bool fin = isfinite(v) && isfinite(m[i]);
           float& b = i < 2 ? best_a : best_b;
           float& e = i < 2 ? err_a : err_b;
-          b = fmaxf(b, fin ? v : INFINITY);
-          e = fmaxf(e, fin ? m[i] * kScoreErr : 0.f);
+          b = fmaxf(b, fin ? v : 0.f);
+          e = fmaxf(e, fin ? m[i] * kScoreErr : INFINITY);
         }
       }
     }
@@ -263,14 +265,37 @@ __global__ void __launch_bounds__(kThreads, NH == 1 ? 4 : 2) page_score_kernel(c
       err_a = fmaxf(err_a, __shfl_xor_sync(kFull, err_a, o));
       err_b = fmaxf(err_b, __shfl_xor_sync(kFull, err_b, o));
     }
+    odd = fmaxf(odd, fmaxf(err_a, err_b));
     if (c == 0) {
-      if (p0 + g < end) ws[p0 + g] = make_float2(best_a, isinf(best_a) ? 0.f : err_a);
-      if (p0 + g + 8 < end) ws[p0 + g + 8] = make_float2(best_b, isinf(best_b) ? 0.f : err_b);
+      if (p0 + g < end) ws[p0 + g] = make_float2(best_a, err_a);
+      if (p0 + g + 8 < end) ws[p0 + g + 8] = make_float2(best_b, err_b);
     }
   };
   for (int it = 0; it < mine; ++it) {
     if (it > 0) load(it, t0);
     score(it, t0);
+  }
+  if (__any_sync(kFull, isinf(odd))) {    // rare: which ones hold an infinity or a NaN, and which only overflow
+    auto bad = [](const uint4& x) {
+      auto two = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
+      return two(x.x) || two(x.y) || two(x.z) || two(x.w);
+    };
+    bool bad_q = false;
+#pragma unroll
+    for (int t = 0; t < NH; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bad_q |= bad(q[t][j]);
+    bad_q = __any_sync(kFull, bad_q);
+#pragma unroll 1
+    for (int i = 0; i < mine * 16; i += 8) {   // pages g and g + 8 of every pass
+      const uint4* page = bounds + __shfl_sync(kFull, table, i + g) * page_pieces;
+      bool bad_p = bad_q;
+#pragma unroll 1
+      for (int j = 0; j < 8; ++j) bad_p |= bad(page[4 * j]);
+      bad_p = __ballot_sync(kFull, bad_p) >> (lane & 28) & 0xfu;
+      const int p = begin + (i >> 4) * kScoreTile + (i & 15) + g;
+      if (c == 0 && bad_p && p < end) ws[p] = make_float2(INFINITY, 0.f);
+    }
   }
   pdl_trigger();
 }

@@ -570,6 +570,27 @@ def test_select_takes_pages_that_are_not_finite(ops):
     assert {30, 50, 70, 89} <= set(sel[0, 0].tolist())
 
 
+@pytest.mark.parametrize("Hq,Hkv", [(8, 1), (24, 2)])
+@pytest.mark.parametrize("n", [60, 1300])
+@pytest.mark.parametrize("q,k", [(2.0 ** 70, 2.0 ** 70), (2.0 ** 64, 2.0 ** 60), (2.0 ** 60, 2.0 ** 60)])
+def test_select_scores_beyond_fp32(ops, Hq, Hkv, n, q, k):
+    """Finite keys and queries whose scores, or parts of them, lie beyond fp32: they are compared like others."""
+    budget = 9
+    v = _paged([16 * n, 16 * 20], Hq, Hkv, 51)
+    v["q"] = (v["q"].float() * q).to(BF)
+    v["kc"] = (v["kc"].float() * k).to(BF)
+    v["kc"][v["bt"][0, 5:40:3].long()] *= 2.0 ** -20
+    v["kc"][int(v["bt"][0, 17]), 0, 2, 9] = float("nan")
+    assert bool(torch.isfinite(v["q"]).all())
+    d = {k_: t.to(ops.dev) if torch.is_tensor(t) else t for k_, t in v.items()}
+    ops.page_bounds(d["kc"], d["bounds"], d["bt"], torch.zeros(2, dtype=I32, device=ops.dev), d["lens"], 16 * n)
+    v["bounds"] = d["bounds"].cpu()
+    sel = torch.zeros(2, Hkv, budget, dtype=I32, device=ops.dev)
+    ws = torch.zeros(max(1, ops.select_workspace(2, Hkv, v["width"])), device=ops.dev)
+    ops.attn_select(d["q"], d["tok"], d["lens"], d["bt"], d["bounds"], sel, 1, 2, Hq, Hkv, ws)
+    assert torch.equal(sel.cpu(), _select_reference(v, Hq, Hkv, budget, 1, 2))
+
+
 def test_select_first_and_last_fill_the_budget(ops):
     Hq, Hkv, lens = 4, 2, [16 * 40 + 1, 16 * 3, 5]
     v = _paged(lens, Hq, Hkv, 9)
