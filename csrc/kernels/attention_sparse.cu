@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(128) page_bounds_kernel(const BoundsArgs a) {
 // same instruction on the operands without their signs.
 // ===========================================================================
 constexpr float kScoreErr = 1.f / 32768.f;   // 2^-15, four times what is derived above
+constexpr float kScoreTiny = 0x1p-118f;      // and what 256 products and their sums may lose below 2^-126
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kScoreTile = 16 * kWarps;      // pages of one pass of a CTA
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, NH == 1 ? 4 : 2) page_score_kernel(c
           float& b = i < 2 ? best_a : best_b;
           float& e = i < 2 ? err_a : err_b;
           b = fmaxf(b, fin ? v : 0.f);
-          e = fmaxf(e, fin ? m[i] * kScoreErr : INFINITY);
+          e = fmaxf(e, fin ? fmaf(m[i], kScoreErr, kScoreTiny) : INFINITY);
         }
       }
     }

@@ -591,6 +591,24 @@ def test_select_scores_beyond_fp32(ops, Hq, Hkv, n, q, k):
     assert torch.equal(sel.cpu(), _select_reference(v, Hq, Hkv, budget, 1, 2))
 
 
+@pytest.mark.parametrize("q,k", [(2.0 ** -64, 2.0 ** -64), (2.0 ** -70, 2.0 ** -70), (2.0 ** -73, 2.0 ** -70),
+                                 (2.0 ** -76, 2.0 ** -74), (2.0 ** -78, 2.0 ** -76), (2.0 ** 20, 2.0 ** -130),
+                                 (2.0 ** -14, 2.0 ** -130)])
+def test_select_scores_below_fp32(ops, q, k):
+    """Products at and below fp32's smallest numbers: pages that their fp32 sums order wrongly."""
+    Hq, Hkv, n, budget = 16, 4, 1300, 24
+    v = _paged([16 * n, 16 * (n - 100) - 5], Hq, Hkv, 52)
+    v["q"] = (v["q"].float() * q).to(BF)
+    v["kc"] = (v["kc"].float() * k).to(BF)
+    d = {k_: t.to(ops.dev) if torch.is_tensor(t) else t for k_, t in v.items()}
+    ops.page_bounds(d["kc"], d["bounds"], d["bt"], torch.zeros(2, dtype=I32, device=ops.dev), d["lens"], 16 * n)
+    v["bounds"] = d["bounds"].cpu()
+    sel = torch.zeros(2, Hkv, budget, dtype=I32, device=ops.dev)
+    ws = torch.zeros(max(1, ops.select_workspace(2, Hkv, v["width"])), device=ops.dev)
+    ops.attn_select(d["q"], d["tok"], d["lens"], d["bt"], d["bounds"], sel, 1, 2, Hq, Hkv, ws)
+    assert torch.equal(sel.cpu(), _select_reference(v, Hq, Hkv, budget, 1, 2))
+
+
 def test_select_first_and_last_fill_the_budget(ops):
     Hq, Hkv, lens = 4, 2, [16 * 40 + 1, 16 * 3, 5]
     v = _paged(lens, Hq, Hkv, 9)
