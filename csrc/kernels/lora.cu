@@ -100,13 +100,20 @@ __device__ __forceinline__ void st_cluster2(uint32_t addr, uint2 v) {
   asm volatile("st.shared::cluster.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
 }
 
-// The four values as PARTS bf16 values each that add up to them.
+// The four values as PARTS bf16 values each that add up to them.  Parts before the last
+// one stay finite: a value beyond the largest bf16 is still held, an infinity is the
+// last part alone (as the first it would leave inf - inf for the next).
 template <int PARTS>
 __device__ __forceinline__ void split4(float4 v, uint2 (&p)[PARTS]) {
+  constexpr float kMost = 0x1.fep127f;
 #pragma unroll
   for (int i = 0; i < PARTS; ++i) {
-    p[i].x = pack_bf16x2(v.x, v.y);
-    p[i].y = pack_bf16x2(v.z, v.w);
+    float4 w = v;
+    if (i + 1 < PARTS)
+      w = make_float4(fminf(fmaxf(v.x, -kMost), kMost), fminf(fmaxf(v.y, -kMost), kMost), fminf(fmaxf(v.z, -kMost), kMost),
+                      fminf(fmaxf(v.w, -kMost), kMost));
+    p[i].x = pack_bf16x2(w.x, w.y);
+    p[i].y = pack_bf16x2(w.z, w.w);
     const float2 a = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&p[i].x));
     const float2 b = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&p[i].y));
     v.x -= a.x, v.y -= a.y, v.z -= b.x, v.w -= b.y;

@@ -335,6 +335,33 @@ def test_lora_row_that_is_not_finite(ops, T, K, R, counts):
     assert torch.equal(got[others], want[others])
 
 
+# one row, 16-row tiles, large tiles
+LORA_KERNELS = [(3, 72, 8, [1, 2], [5, 8]), (3, 328, 32, [0, 1, 1], [32, 32, 25]), (40, 264, 24, [17, 1, 20], [13, 24, 24]),
+                (40, 264, 64, [17, 1, 20], [64, 51, 64]), (1300, 264, 64, [700, 1, 590], [64, 64, 41])]
+
+
+@pytest.mark.parametrize("T,K,R,counts,ranks", LORA_KERNELS)
+@pytest.mark.parametrize("f32", [False, True])
+def test_lora_h_beyond_bf16(ops, T, K, R, counts, ranks, f32):
+    """h between the largest bf16 and the largest fp32 value, +-(2 - 2^-9) 2^127: outputs stay finite."""
+    slices = (48, 24)
+    v = _lora_inputs(T, K, slices, R, counts, 62, ranks, f32)
+    v["x"][:] = 0
+    v["x"][:, 3:13] = torch.where(torch.arange(T) % 2 == 0, 2.0 ** 64, -2.0 ** 64)[:, None].to(BF)
+    v["a"][..., 3:13] = torch.where(v["a"][..., 3:13].isnan(), v["a"][..., 3:13], (2.0 ** (63 - torch.arange(10.0))).to(BF))
+    v["b"] = torch.where(v["b"].isnan(), v["b"], torch.zeros_like(v["b"]))
+    v["b"][..., 0] = 2.0 ** -110
+    v["base"][:] = 0
+    ref, _ = _lora_reference(v, slices, R)
+    assert bool((ref[v["rows"].long()].abs() > 1e4).all())
+    d = {k: t.to(ops.dev) for k, t in v.items()}
+    out = d["base"].clone()
+    ops.lora_add(d["x"], d["a"], d["b"], d["scales"], d["ranks"], d["rows"], d["starts"], out, out, slices)
+    # every product, the sum and the two bf16 parts of h (10 bits) are exact: only the output is rounded
+    assert torch.equal(out.cpu(), ref.to(out.dtype))
+    _no_error(ops)
+
+
 @gpu
 def test_lora_bad_indices_are_recorded(kernels):
     T, K, R, slices = 40, 64, 8, (64,)
