@@ -376,7 +376,7 @@ __device__ __forceinline__ void one_row(const LoraArgs& a, const Tile& tl, int r
     for (int q = 0; q < kCluster; ++q) v[q] = q < cl ? ld_cluster(cluster_addr(part + i, q)) : 0.f;
 #pragma unroll
     for (int q = 0; q < kCluster; ++q) sum += v[q];
-    h[i] = sum;
+    h[i] = i % rp < rank ? sum : 0.f;     // past the rank: zero rows of A, times an infinity in x
   }
   cluster_arrive();                       // this CTA has read the others' partials
   __syncthreads();
@@ -624,8 +624,9 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
     for (int q = 1; q < kCluster; ++q)
       if (q < cl) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
     uint2 p[kParts];
-    split4<kParts>(v[0], p);
     const int j = i / (TM / 4), row = i % (TM / 4) * 4;
+    if (rank < rp && j % rp >= rank) v[0] = make_float4(0.f, 0.f, 0.f, 0.f);   // zero rows of A, times an infinity in x
+    split4<kParts>(v[0], p);
 #pragma unroll
     for (int q = 0; q < kParts; ++q) {
       const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&p[q]);

@@ -342,6 +342,25 @@ LORA_KERNELS = [(3, 72, 8, [1, 2], [5, 8]), (3, 328, 32, [0, 1, 1], [32, 32, 25]
 
 @pytest.mark.parametrize("T,K,R,counts,ranks", LORA_KERNELS)
 @pytest.mark.parametrize("f32", [False, True])
+def test_lora_infinities_as_in_64_bits(ops, T, K, R, counts, ranks, f32):
+    """An infinite h times weights of one sign is an infinity, not a NaN, whatever lies past the rank."""
+    slices = (48, 24)
+    v = _lora_inputs(T, K, slices, R, counts, 61, ranks, f32)
+    for name in ("a", "b"):
+        v[name] = torch.where(v[name].isnan(), v[name], v[name].abs() + 1)
+    v["x"][int(v["rows"][0]), 5] = float("inf")
+    v["x"][int(v["rows"][-1]), 7] = -float("inf")
+    ref, _ = _lora_reference(v, slices, R)
+    assert bool(ref[int(v["rows"][0])].isinf().all()) and bool(ref[int(v["rows"][-1])].isinf().all())
+    d = {k: t.to(ops.dev) for k, t in v.items()}
+    out = d["base"].clone()
+    ops.lora_add(d["x"], d["a"], d["b"], d["scales"], d["ranks"], d["rows"], d["starts"], out, out, slices)
+    assert torch.equal(out.cpu(), ref.to(out.dtype))
+    _no_error(ops)
+
+
+@pytest.mark.parametrize("T,K,R,counts,ranks", LORA_KERNELS)
+@pytest.mark.parametrize("f32", [False, True])
 def test_lora_h_beyond_bf16(ops, T, K, R, counts, ranks, f32):
     """h between the largest bf16 and the largest fp32 value, +-(2 - 2^-9) 2^127: outputs stay finite."""
     slices = (48, 24)
