@@ -967,7 +967,8 @@ __global__ void __launch_bounds__(W * 32, (NH == 1 ? 16 : 8) / W) decode_sparse_
   if (cl > 1) cluster_wait();
   __nv_bfloat16* out = a.out + (int64_t)(tok_ok ? tok : 0) * a.out_ld + (int64_t)kvh * G * D;
   auto write = [&](int quad, float4 acc, float sum) {
-    const float f = sum > 0.f ? 1.f / sum : 0.f;
+    // no weight at all: nothing to attend to, or logits of -inf alone, whose softmax is NaN
+    const float f = sum > 0.f ? 1.f / sum : count > 0 ? __int_as_float(0x7fffffff) : 0.f;
     if (tok_ok)
       *reinterpret_cast<uint2*>(out + quad * 4) = make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
   };

@@ -727,6 +727,36 @@ def test_sparse_weights_are_not_rounded(ops, lens, Hq, Hkv, budget):
     _within(out[v["tok"].long().to(out.device)], ref, 2.0 ** -8 * ref.abs() + 2.0 ** -14 * (mag + ref.abs()), "attention")
 
 
+@pytest.mark.parametrize("Hq,Hkv,budget", [(8, 1, 4), (8, 1, 40), (24, 2, 4)])
+def test_sparse_logits_that_are_not_finite(ops, Hq, Hkv, budget):
+    """Logits of -inf weigh nothing beside finite ones; where a row has no others, or one of +inf or NaN, it is NaN."""
+    lens = [1, 40, 40, 40, 600, 600, 0]
+    v = _paged(lens, Hq, Hkv, 70)
+    v["q"][:, :Hq * 128:128] = 1.0
+    neg = -float("inf")
+    for r in (0, 1, 4):                              # every key
+        v["kc"][v["bt"][r, :-(-lens[r] // 16)].long(), :, :, 0] = neg
+    v["kc"][v["bt"][2, :3].long(), :, ::2, 0] = neg  # every second key
+    v["kc"][int(v["bt"][2, 2]), :, :, 0] = neg
+    v["kc"][int(v["bt"][3, 1]), :, 3, 0] = float("inf")
+    v["kc"][v["bt"][5, 1:37].long(), :, :, 0] = neg  # all but the first and the last page
+    d = {k: t.to(ops.dev) if torch.is_tensor(t) else t for k, t in v.items()}
+    sel = torch.full((len(lens), Hkv, budget), -1, dtype=I32)
+    for r, n in enumerate(lens):
+        count = min(-(-n // 16), budget)
+        sel[r, :, :count] = torch.tensor(([0] + list(range(-(-n // 16) - count + 1, -(-n // 16))))[:count], dtype=I32)
+    out = torch.full((d["q"].shape[0], Hq * 128), 3.0, dtype=BF, device=ops.dev)
+    ops.attn_decode_sparse(d["q"], out, d["tok"], d["lens"], d["bt"], sel.to(ops.dev), d["kc"], d["vc"], Hq, Hkv)
+    got = out[v["tok"].long().to(out.device)].cpu()
+    for r in (0, 1, 3, 4):
+        assert bool(got[r].isnan().all()), r
+    assert not bool(got[6].any())
+    ref, mag = _attend_reference(v, sel, Hq, Hkv)
+    for r in (2, 5):
+        assert bool(ref[r].isfinite().all())
+        _within(got[r], ref[r], 2.0 ** -8 * ref[r].abs() + 2.0 ** -11 * (mag[r] + ref[r].abs()), r)
+
+
 @pytest.mark.parametrize("lens", [[16 * 20000 + 3], [16 * 9000, 16 * 3]])
 @gpu
 def test_select_long_rows(kernels, lens):
