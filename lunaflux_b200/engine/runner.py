@@ -98,6 +98,10 @@ class ModelRunner:
                 raise ValueError("this operator set has no attention over selected pages")
             if min(self.sparse) < 0 or sparse_first + sparse_last > sparse_pages or page != 16:
                 raise ValueError("sparse_pages must hold the first and the last pages, of 16 tokens")
+            limits = getattr(ops, "sparse_unsupported", None)     # the plain operators have none
+            why = limits and limits(self.Hq, self.Hkv, self.D, page, dt, max_rows, self.W, int(sparse_pages))
+            if why:
+                raise ValueError(f"attention over selected pages takes {why}")
             self.bounds = torch.zeros(s.layers, self.num_pages, self.Hkv, 2, self.D, dtype=dt, device=dev)
             self.sel = torch.full((R, self.Hkv, sparse_pages), -1, dtype=torch.int32, device=dev)
             self.sel_ws = torch.empty(ops.select_workspace(R, self.Hkv, self.W), dtype=torch.float32, device=dev)

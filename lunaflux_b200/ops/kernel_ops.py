@@ -152,6 +152,17 @@ class KernelOps:
         self.C.page_bounds(kc, bounds, bt, start, seq_lens, max_new)
 
     @staticmethod
+    def sparse_unsupported(Hq, Hkv, D, page, dtype, rows, width, budget) -> Optional[str]:
+        """Why attention over selected pages does not take this model or these sizes; None where it does."""
+        if D != 128 or page != 16 or dtype != torch.bfloat16:
+            return f"pages of 16 bf16 keys with head_dim 128, not {page} of {dtype} with {D}"
+        if Hq % Hkv or Hq // Hkv > 16:
+            return f"at most 16 query heads per KV head, not {Hq} for {Hkv}"
+        if max(width, budget) > 65536 or rows > 65535:
+            return f"at most 65536 pages and 65535 rows, not {max(width, budget)} and {rows}"
+        return None
+
+    @staticmethod
     def select_workspace(rows, Hkv, width):
         """fp32 elements of ``attn_select``'s workspace for block tables of `width` pages."""
         return 2 * rows * Hkv * width

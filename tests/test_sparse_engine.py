@@ -113,6 +113,46 @@ def test_options_are_checked(tiny):
                   EngineOptions(max_context=256, num_pages=64, graph_sizes=(), sparse_pages=4))
 
 
+@pytest.mark.parametrize("change,words", [(dict(head_dim=64), "head_dim 128"), (dict(heads=34, kv_heads=2), "16 query heads"),
+                                          (dict(), None)])
+def test_kernel_limits_are_checked_at_construction(change, words):
+    """A model or a table the kernels do not take is refused before any request is admitted."""
+    from lunaflux_b200.ops import KernelOps
+
+    class Limited(TorchOps):
+        sparse_unsupported = staticmethod(KernelOps.sparse_unsupported)
+
+    spec = LlamaSpec(**{**dict(hidden=64, layers=1, heads=4, kv_heads=2, head_dim=128, ffn=128, vocab=64, rope_theta=10000.0,
+                               max_position=512, dtype="bf16"), **change})
+    ck = random_checkpoint(spec, 0)
+    w = build_runtime(spec, lambda n: ck[n], dtype=torch.bfloat16)
+    sched = SchedulerConfig(step_token_budget=64, max_active_requests=4, prefill_chunk_tokens=64,
+                            emergency_decode_page_reserve=1)
+
+    def engine(**opts):
+        return LLMEngine(w, Limited(), "cpu", sched, CacheConfig(), EngineOptions(**{**dict(
+            max_context=256, num_pages=64, graph_sizes=(), sparse_pages=4), **opts}))
+
+    if words:
+        with pytest.raises(ValueError, match=words):
+            engine()
+    else:
+        engine()
+        with pytest.raises(ValueError, match="65536 pages"):
+            engine(sparse_pages=65537)
+    engine(sparse_pages=0)
+
+
+def test_kernel_limits():
+    from lunaflux_b200.ops import KernelOps
+    at = dict(Hq=32, Hkv=8, D=128, page=16, dtype=torch.bfloat16, rows=256, width=8192, budget=64)
+    assert KernelOps.sparse_unsupported(**at) is None
+    assert KernelOps.sparse_unsupported(**{**at, "Hq": 16, "Hkv": 1, "width": 65536, "rows": 65535}) is None
+    for change in (dict(D=64), dict(page=32), dict(dtype=torch.float16), dict(Hq=34, Hkv=2), dict(Hq=12), dict(width=65537),
+                   dict(budget=65537), dict(rows=65536)):
+        assert KernelOps.sparse_unsupported(**{**at, **change})
+
+
 def _gpu_engine(spec, ck, sparse, graphs):
     from lunaflux_b200.ops import KernelOps
     w = build_runtime(spec, lambda n: ck[n], device="cuda", dtype=torch.bfloat16)
