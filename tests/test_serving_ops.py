@@ -144,6 +144,19 @@ def test_norm_rope_strides_and_zero_rows(ops):
 
 
 @gpu
+@pytest.mark.parametrize("T,Hq,Hkv,D", [(400, 8, 2, 128), (1023, 64, 8, 128), (297, 5, 3, 128), (300, 4, 1, 256), (297, 3, 3, 256)])
+def test_norm_rope_many_tokens(kernels, T, Hq, Hkv, D):
+    """More than two tokens per SM: the narrow CTAs."""
+    x = _norm_rope_inputs(T, Hq, Hkv, D, T + Hq, pad=T // 7)
+    d = {k: v.cuda() if torch.is_tensor(v) else v for k, v in x.items()}
+    q = torch.full((T, Hq * D), 7.0, dtype=BF, device="cuda")
+    kernels.qk_norm_rope_kv_write(d["qkv"], d["wq"], d["wk"], 1e-5, d["pos"], d["slots"], d["cs"], q, d["kc"], d["vc"],
+                                  Hq, Hkv, 16)
+    _norm_rope_check(q, d["kc"], d["vc"], _norm_rope_reference(x, Hq, Hkv, D, 1e-5))
+    _no_error(kernels)
+
+
+@gpu
 def test_norm_rope_bad_position_and_slot_are_recorded(kernels):
     T, Hq, Hkv, D = 4, 2, 1, 128
     for field, value in (("pos", 512), ("pos", -1), ("slots", (T + 2) * 16)):
@@ -439,6 +452,70 @@ def test_lora_large_tiles_with_a_recorded_error(kernels, T, K, slices, R, counts
         assert torch.equal(bad[spoilt], v["base"][spoilt]), what
         assert torch.equal(after, ref.to(after.dtype)), what
         assert kernels.read_error(True)[0] == 3, what
+
+
+@pytest.mark.parametrize("T,K,slices,R,counts,ranks", [
+    (5, 1024, (96,), 32, [1, 2, 1], [32, 31, 7]), (40, 264, (72,), 32, [17, 1, 20], [32, 25, 32]),
+    (64, 520, (1032,), 32, [1] * 60, [32] * 60), (50, 136, (40, 32, 24, 8), 8, [20, 30], [8, 5]),
+    (50, 136, (40, 32, 24), 8, [20, 30], [8, 5])])
+@pytest.mark.parametrize("f32", [False, True])
+def test_lora_more_ranks_and_slices(ops, T, K, slices, R, counts, ranks, f32):
+    """Rank 32 beside one projection, 24 and 32 columns of h: variants that the shapes above pass by."""
+    test_lora_integers_are_exact(ops, T, K, slices, R, counts, ranks, f32)
+    test_lora_against_64_bits(ops, T, K, slices, R, counts, ranks, f32)
+
+
+@pytest.mark.parametrize("T,K,R,counts,ranks", LORA_KERNELS)
+def test_lora_fp32_outputs_hold_h_to_24_bits(ops, T, K, R, counts, ranks):
+    """h of 23 bits, exact in fp32, and one +-1 of B per column: two bf16 parts of h would lose the lowest bits."""
+    slices = (48, 24)
+    v = _lora_inputs(T, K, slices, R, counts, 63, ranks, True)
+    g = _gen(64)
+    v["x"][:] = 0
+    v["x"][:, 3] = torch.randint(64, 128, (T,), generator=g).to(BF)              # h = 2^16 x[3] + x[40] a[40]
+    v["x"][:, 40] = (torch.randint(0, 128, (T,), generator=g) * 2 + 1).to(BF)
+    nan = v["a"][..., 3].isnan()
+    v["a"][..., 3] = torch.where(nan, v["a"][..., 3], torch.full_like(v["a"][..., 3], 2.0 ** 16))
+    odd = (torch.randint(0, 64, nan.shape, generator=g) * 2 + 1).to(BF)
+    v["a"][..., 40] = torch.where(nan, v["a"][..., 40], odd)
+    v["b"] = torch.where(v["b"].isnan(), v["b"], torch.zeros_like(v["b"]))
+    for ad, rank in enumerate(ranks):
+        c = torch.arange(sum(slices))
+        v["b"][ad, c, c % rank] = torch.where(c % 3 == 0, -1.0, 1.0).to(BF)
+    v["base"][:] = 0
+    ref, _ = _lora_reference(v, slices, R)
+    assert bool((ref.float().double() == ref).all()) and bool((ref[v["rows"].long()].abs() >= 2.0 ** 19).all())
+    d = {k: t.to(ops.dev) for k, t in v.items()}
+    out = d["base"].clone()
+    ops.lora_add(d["x"], d["a"], d["b"], d["scales"], d["ranks"], d["rows"], d["starts"], out, out, slices)
+    assert torch.equal(out.cpu().double(), ref)
+    _no_error(ops)
+
+
+@pytest.mark.parametrize("T,K,R,counts,ranks", LORA_KERNELS)
+@pytest.mark.parametrize("f32", [False, True])
+def test_lora_repeats_exactly(ops, T, K, R, counts, ranks, f32):
+    """The same call gives the same bits, a row by itself the same value to the sums' accuracy."""
+    slices = (48, 24)
+    v = _lora_inputs(T, K, slices, R, counts, 65, ranks, f32, integer=False)
+    ref, mag = _lora_reference(v, slices, R)
+    d = {k: t.to(ops.dev) for k, t in v.items()}
+    args = (d["x"], d["a"], d["b"], d["scales"], d["ranks"])
+    want = d["base"].clone()
+    ops.lora_add(*args, d["rows"], d["starts"], want, want, slices)
+    for _ in range(3):
+        out = d["base"].clone()
+        ops.lora_add(*args, d["rows"], d["starts"], out, out, slices)
+        assert torch.equal(out, want)
+    ad = len(counts) - 1                             # the last listed row is the last adapter's
+    t = int(v["rows"][-1])
+    starts = torch.tensor([0] * (ad + 1) + [1], dtype=I32, device=ops.dev)
+    one = d["base"].clone()
+    ops.lora_add(*args, d["rows"][-1:].contiguous(), starts, one, one, slices)
+    steps = K // 16 + 1 + 4 * 3                      # as in test_lora_against_64_bits
+    rel = 17 * 2.0 ** -23 * steps + (2.0 ** -24 if f32 else 2.0 ** -16)
+    for got in (one, want):
+        _within(got[t], ref[t], (2.0 ** -23 if f32 else 2.0 ** -8) * ref[t].abs() + rel * mag[t], "row")
 
 
 # ---------------------------------------------------------------------------
@@ -774,6 +851,33 @@ def test_select_long_rows(kernels, lens):
         ws = torch.zeros(kernels.select_workspace(R, Hkv, v["width"]), device="cuda")
         kernels.attn_select(d["q"], d["tok"], d["lens"], d["bt"], d["bounds"], sel, 1, 2, Hq, Hkv, ws)
         assert torch.equal(sel.cpu(), _select_reference(v, Hq, Hkv, budget, 1, 2))
+    _no_error(kernels)
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv,budget", [
+    ([16 * 5000 + 3, 16 * 2100, 16 * 8000, 700, 16 * 60], 8, 2, 60),     # 2049 to 8192 pages
+    ([16 * 3000 - 7, 16 * 2500], 12, 1, 700),                            # the same, two groups of query heads
+    ([16 * 640, 1, 0, 17] + [16 * 30 + 5 * i for i in range(36)], 24, 2, 24),
+    ([16 * 9 + i for i in range(40)], 32, 2, 4)])                        # many rows of wide groups
+@gpu
+def test_sparse_step_more_rows_pages_and_heads(kernels, lens, Hq, Hkv, budget):
+    """Launch variants that the cases above pass by: with random keys, then with one key for all (ties)."""
+    for tie in (False, True):
+        v = _paged(lens, Hq, Hkv, 43)
+        if tie:
+            v["kc"][:] = v["kc"][5, 0, 0, 0].clone()
+        d = {k: t.cuda() if torch.is_tensor(t) else t for k, t in v.items()}
+        R = len(lens)
+        kernels.page_bounds(d["kc"], d["bounds"], d["bt"], torch.zeros(R, dtype=I32, device="cuda"), d["lens"], max(lens))
+        v["bounds"] = d["bounds"].cpu()
+        sel = torch.full((R, Hkv, budget), 99, dtype=I32, device="cuda")
+        ws = torch.zeros(kernels.select_workspace(R, Hkv, v["width"]), device="cuda")
+        kernels.attn_select(d["q"], d["tok"], d["lens"], d["bt"], d["bounds"], sel, 1, 2, Hq, Hkv, ws)
+        want = _select_reference(v, Hq, Hkv, budget, 1, 2)
+        assert torch.equal(sel.cpu(), want)
+        out = torch.full((d["q"].shape[0], Hq * 128), 4.0, dtype=BF, device="cuda")
+        kernels.attn_decode_sparse(d["q"], out, d["tok"], d["lens"], d["bt"], sel, d["kc"], d["vc"], Hq, Hkv)
+        _attend_check(out, v, want, Hq, Hkv)
     _no_error(kernels)
 
 
