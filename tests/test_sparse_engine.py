@@ -1,6 +1,11 @@
 """The engine's decode over selected pages (``EngineOptions.sparse_pages``)."""
+import os
+import socket
+
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from lunaflux_b200.config import CacheConfig, SchedulerConfig
 from lunaflux_b200.engine.engine import EngineOptions, LLMEngine
@@ -151,6 +156,47 @@ def test_kernel_limits():
     for change in (dict(D=64), dict(page=32), dict(dtype=torch.float16), dict(Hq=34, Hkv=2), dict(Hq=12), dict(width=65537),
                    dict(budget=65537), dict(rows=65536)):
         assert KernelOps.sparse_unsupported(**{**at, **change})
+
+
+def _rank(rank, world, port, q, sp, sparse):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        from lunaflux_b200.parallel.comm import TPComm
+        from lunaflux_b200.parallel.tp import TPShard
+        spec = tiny_llama()
+        ck = random_checkpoint(spec, 0)
+        sched = SchedulerConfig(step_token_budget=64, max_active_requests=4, prefill_chunk_tokens=64,
+                                emergency_decode_page_reserve=1, waiting_age_threshold_steps=8)
+        eng = LLMEngine(build_runtime(spec, lambda n: ck[n], TPShard(rank, world, spec)), TorchOps(), "cpu", sched,
+                        CacheConfig(), EngineOptions(max_context=256, num_pages=96, graph_sizes=(), sequence_parallel=sp,
+                                                     sparse_pages=sparse, sparse_first=1, sparse_last=1), comm=TPComm())
+        assert eng.runner.sp == sp and eng.runner.bounds.shape[2] == max(1, spec.kv_heads // world)
+        q.put((rank, eng.generate(_prompts(256, (150, 90, 30), seed=1), 10)))
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("world,sp,sparse", [(2, False, 4), (2, True, 4), (4, True, 16)])
+def test_tensor_and_sequence_parallel_ranks(tiny, world, sp, sparse):
+    """Ranks with whole KV heads select what one rank selects; with shared ones (world 4 of 2
+    KV heads) a rank selects for its own query heads, so there every page is taken."""
+    spec, ck = tiny
+    want = _cpu_engine(ck, spec, sparse, budget=64).generate(_prompts(256, (150, 90, 30), seed=1), 10)
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_rank, args=(r, world, port, q, sp, sparse)) for r in range(world)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=240) for _ in range(world))
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    for r in range(world):
+        assert got[r] == want, f"rank {r}"
 
 
 def _gpu_engine(spec, ck, sparse, graphs):
