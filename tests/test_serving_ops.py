@@ -799,8 +799,9 @@ def test_sparse_weights_are_not_rounded(ops, lens, Hq, Hkv, budget):
     out = torch.zeros(d["q"].shape[0], Hq * 128, dtype=BF, device=ops.dev)
     ops.attn_decode_sparse(d["q"], out, d["tok"], d["lens"], d["bt"], sel.to(ops.dev), d["kc"], d["vc"], Hq, Hkv)
     ref, mag = _attend_reference(v, sel, Hq, Hkv)
-    # a weight: its logit 5 * 2^-23, the exponential 2^-22, two bf16 parts 2^-16; a weighted sum over at most 7 steps
-    # of 16 tokens in two parts, 17 * 2^-23 each; the sum of weights less: under 2^-14 of sum p |v| + |out| in all
+    # a weight: its logit 5 * 2^-23, the exponential 2^-22, two bf16 parts 2^-15; a weighted sum over at most 2 steps
+    # of 16 tokens per warp in two parts, 17 * 2^-23 each (2^-16.9); the sum of weights less: under 2^-14 of
+    # sum p |v| + |out| in all
     _within(out[v["tok"].long().to(out.device)], ref, 2.0 ** -8 * ref.abs() + 2.0 ** -14 * (mag + ref.abs()), "attention")
 
 
@@ -832,6 +833,29 @@ def test_sparse_logits_that_are_not_finite(ops, Hq, Hkv, budget):
     for r in (2, 5):
         assert bool(ref[r].isfinite().all())
         _within(got[r], ref[r], 2.0 ** -8 * ref[r].abs() + 2.0 ** -11 * (mag[r] + ref[r].abs()), r)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (24, 2)])
+def test_sparse_values_that_are_infinite(ops, Hq, Hkv):
+    """An infinite value of a token that weighs anything makes its dimension infinite, not NaN."""
+    lens, budget = [1, 33, 200, 16], 30
+    v = _paged(lens, Hq, Hkv, 71)
+    v["q"][:] = (v["q"].float() * 0.25).to(BF)
+    inf = float("inf")
+    for r, (p, t) in enumerate(((0, 0), (1, 3), (12, 7), (0, 15))):
+        v["vc"][int(v["bt"][r, p]), :, t, 17] = inf
+        v["vc"][int(v["bt"][r, p]), :, t, 90] = -inf
+    d = {k: t.to(ops.dev) if torch.is_tensor(t) else t for k, t in v.items()}
+    sel = torch.full((len(lens), Hkv, budget), -1, dtype=I32)
+    for r, n in enumerate(lens):
+        sel[r, :, :-(-n // 16)] = torch.arange(-(-n // 16), dtype=I32)
+    out = torch.zeros(d["q"].shape[0], Hq * 128, dtype=BF, device=ops.dev)
+    ops.attn_decode_sparse(d["q"], out, d["tok"], d["lens"], d["bt"], sel.to(ops.dev), d["kc"], d["vc"], Hq, Hkv)
+    got = out[v["tok"].long().to(out.device)].cpu().view(len(lens), Hq, 128)
+    assert bool((got[..., 17] == inf).all()) and bool((got[..., 90] == -inf).all())
+    ref, mag = (x.view(len(lens), Hq, 128) for x in _attend_reference(v, sel, Hq, Hkv))
+    finite = [i for i in range(128) if i not in (17, 90)]
+    _within(got[..., finite], ref[..., finite], 2.0 ** -8 * ref[..., finite].abs() + 2.0 ** -11 * (mag + ref.abs())[..., finite], "out")
 
 
 @pytest.mark.parametrize("lens", [[16 * 20000 + 3], [16 * 9000, 16 * 3]])
