@@ -11,12 +11,14 @@
 //   decode_sparse  softmax attention over the chosen pages' valid tokens
 //
 // max(q lo, q hi) = max(q, 0) hi + min(q, 0) lo because lo <= hi, so a page's
-// score is a dot product of 256 terms: tensor-core work with 16 pages as the
+// score is a dot product of 256 terms (the bound by a page's smallest and largest keys
+// was published by Tang et al., "Query-Aware Sparsity for Efficient Long-Context LLM
+// Inference", 2024): tensor-core work with 16 pages as the
 // rows and the group's query heads as the columns.  What bounds the selection
 // is reading the bounds, 512 bytes per (page, KV head); what bounds the
 // attention is reading 8 KB per chosen (page, KV head).
 //
-// The order of the scores is that of the exact sums.  bf16 products are exact
+// The order of the scores is that of their sums in 64 bits.  bf16 products are exact
 // in fp32; their fp32 sums carry an error bound e = kScoreErr * sum|terms|, and
 // where the bounds of two pages around the cut overlap, both are summed again
 // in fp64.  Where a page or query holds an infinity or a NaN the score counts as
@@ -752,7 +754,7 @@ __global__ void __launch_bounds__(NT) page_select_kernel(const SelectArgs a) {
 // have the weight's sign and neither is zero alone: an infinite value stays one.
 //
 // 16 warps per SM have a page each under way; 64 rows x 8 heads x 128 pages read
-// 537 MB in 89 us, 6.0 TB/s (84 with one CTA per row and head).  A page ahead in registers halves the warps, and per-lane
+// 537 MB in 90 us, 6.0 TB/s (85 with one CTA per row and head).  A page ahead in registers halves the warps, and per-lane
 // cp.async delivers less than plain loads: both were slower.
 // ===========================================================================
 constexpr int kMaxCluster = 8;
@@ -1046,8 +1048,8 @@ void launch_select(const SelectArgs& a, cudaStream_t s) {
 int select_pages(const SelectArgs& a, cudaStream_t s) {
   if (a.rows <= 0) return 0;
   if (a.width > a.budget) {
-    // two passes of 64 pages per CTA where that fills the GPU (64 rows of 2048 pages: 191 us a
-    // step, 198 with one, 192 with eight; a ragged batch of 17: 38, 40, 43)
+    // two passes of 64 pages per CTA where that fills the GPU (64 rows of 2048 pages: 196 us a
+    // step, 201 with one; 64 ragged rows 79 and 86; 4 rows of 8192 pages 55.3 and 56.4)
     const int64_t tiles = (int64_t)a.rows * a.Hkv * ((a.width + kScoreTile - 1) / kScoreTile);
     const int passes = tiles > 4 * sm_count() ? kScorePasses : 1;
     const int chunk = passes * kScoreTile;
@@ -1055,11 +1057,11 @@ int select_pages(const SelectArgs& a, cudaStream_t s) {
     auto k = a.Hq / a.Hkv <= 8 ? page_score_kernel<1> : page_score_kernel<2>;
     launch_k(k, grid, dim3(kThreads), 0, s, 1, a, passes);
   }
-  // As few threads and pages per thread as hold the block table: 8191 tokens 14.1 us
-  // a step, 16.2 with <256, 8>, 20.4 with <1024, 8>; 64 rows of 32768 tokens 188 us, 212
-  // with <1024, 8>, 303 with the general routine.  Where every CTA has an SM for itself
-  // 512 threads for 2048 pages (one row of 32768 tokens 17.4 us, 18.2 with 256; 64 rows
-  // 197, 194).
+  // As few threads and pages per thread as hold the block table: 8191 tokens 14.0 us
+  // a step, 16.0 with <256, 8>, 19.5 with <1024, 8>; 64 rows of 32768 tokens 196 us, 220
+  // with <1024, 8>, 311 with the general routine.  Where every CTA has an SM for itself
+  // 512 threads for 2048 pages (one row of 32768 tokens 17.5 us, 18.5 with 256; 17 ragged
+  // rows 37, 38; 64 rows would take 200, and take 196).
   if (a.width <= 512) launch_select<256, 2>(a, s);
   else if (a.width <= 2048 && (int64_t)a.rows * a.Hkv <= sm_count()) launch_select<512, 4>(a, s);
   else if (a.width <= 2048) launch_select<256, 8>(a, s);
@@ -1075,7 +1077,7 @@ void launch_decode(const SparseArgs& a, cudaStream_t s) {
   // CTAs per unit: as many as run at the same time (16 warps per SM, 8 for wide groups)
   // and get two pages per warp; two also where only half of them run at once, because
   // one CTA with a long row would outlast the others of a ragged batch (64 rows of 1 to 32768
-  // tokens x 8 heads x 128 pages: a step takes 77 us, 96 with one; all of 32768: 194, 189).
+  // tokens x 8 heads x 128 pages: a step takes 79 us, 98 with one; all of 32768: 196, 191).
   const int64_t slots = (int64_t)sm_count() * ((NH == 1 ? 16 : 8) / W);
   int cl = 1;
   while (cl < kMaxCluster && units * cl * 2 <= (cl == 1 ? 2 : 1) * slots && a.budget > W * cl) cl *= 2;
@@ -1084,7 +1086,7 @@ void launch_decode(const SparseArgs& a, cudaStream_t s) {
   allow_smem(reinterpret_cast<const void*>(k), allowed);
   // Clusters that start while the previous kernel still holds some SMs crowd onto
   // the others; where they would fill the GPU they wait for its end (4 rows x 8
-  // heads x 256 pages after a selection: 72 instead of 82 us for the whole step).
+  // heads x 256 pages after a selection: 55 instead of 63 us for the whole step).
   launch_with(cl == 1 || units * cl * W <= sm_count() * 8, k, dim3((unsigned)(units * cl)), dim3(W * 32),
               sizeof(SparseSmem<NH, W>), s, (unsigned)cl, a, cl);
 }
@@ -1093,9 +1095,11 @@ void launch_decode(const SparseArgs& a, cudaStream_t s) {
 void decode_sparse(const SparseArgs& a, cudaStream_t s) {
   if (a.rows <= 0) return;
   // Eight warps per CTA where clusters of eight CTAs still leave SMs without work (1
-  // row x 8 heads x 64 pages: a step takes 14.1 us, 16.0 with four) or, with four
-  // warps, half of the warps that fit, and each of the eight still gets two pages (4 x 8
-  // x 256 pages 54.9 us, 58.1; 4 x 8 x 128 28.2, 29.2; 4 x 8 x 64 would lose, 19.6, 18.9).
+  // row x 8 heads x 64 pages: a step takes 14.0 us, 14.4 with four; 8 x 2 x 256 34.2, 38.5)
+  // or, with four warps, half of the warps that fit, and each of the eight still gets two
+  // pages (4 x 8 x 256 pages 55.3 us, 58.6; 4 x 8 x 128 48.8, 49.8; 4 x 8 x 64 46.2 and 46.0
+  // the other way round).  Not good for groups of more than eight heads in between: 8 rows x
+  // 4 heads x 256 pages take 73.8 us and would take 57.4 with eight.
   const int64_t ctas = (int64_t)a.rows * a.Hkv * kMaxCluster;
   const bool narrow = a.Hq / a.Hkv <= 8;   // wider groups fit eight warps per SM
   const bool few = ctas <= sm_count() || (narrow && ctas <= 2 * sm_count() && a.budget >= 2 * 8 * kMaxCluster);

@@ -13,7 +13,10 @@
 // every CTA multiplies a share of K, the partial h are added through distributed
 // shared memory in rank order, and every CTA expands a share of the columns.  So
 // the whole operator is one launch without a workspace, x and the weights are
-// read by one CTA each, and a result does not depend on the order of arrival.
+// read by one CTA each, and a result does not depend on the order of arrival.  (The
+// large kernel takes one launch per group of slices where slices x rank exceeds an
+// accumulator's 256 columns or shared memory.)  The last bits of a row do depend on the
+// batch it comes in: on the kernel, the tile and the shares of K.
 // Only the adapter's rank is read, of A and of B: inside a tile, h has S * rank
 // columns, the rank rounded up to 8 (16 in the large kernel) ("compact" below).
 //
@@ -270,9 +273,9 @@ constexpr int small_items() {   // items under way
 // shared memory, so its sums need no other warp; R / 8 lanes read one column of B.
 // R is a power of two.  The loops are kept short: a CTA runs each once or a few
 // times, and longer ones would wait for their instructions.
-// One request of rank 16 beside the QKV projection takes 6.6 us, 7.8 as a tile of
-// 16 rows; 64 requests 14.0 and 16.2, of rank 64 43 and 61; one of rank 64 and K = 14336 loses
-// a microsecond, 12.8 and 11.6.
+// One request of rank 16 beside the QKV projection takes 6.7 us, 7.5 as a tile of
+// 16 rows; 64 requests 14.7 and 15.9.  Rank 64 loses: 64 requests 43 and 39, one of K = 14336
+// 12.1 and 11.2.
 __device__ __forceinline__ float dot8(const uint4& v, const float4& x0, const float4& x1, float acc) {
   acc += __uint_as_float(v.x << 16) * x0.x;
   acc += __uint_as_float(v.x & 0xffff0000u) * x0.y;
@@ -734,8 +737,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_small_kernel(const LoraArgs 
 // than half of the shared memory, so that beside one of them at most one of these
 // runs.
 //
-// 8192 rows beside the QKV projection: 76 us, where the bytes that x, base, out and
-// the weights must move once take 40.  64-row tiles take 93: the 64-row instruction
+// 8192 rows beside the QKV projection (K = 4096, N = 6144): 76 us, where the bytes that x,
+// base, out and the weights must move once take 40.  64-row tiles take 93: the 64-row instruction
 // runs at half rate and every tile reads its adapter's weights from L2 again.  Not
 // more shared memory than needed, because the loads of base that are under way live
 // in what is left of it as L1: with 226 KB instead of 162 the call takes 88 us.
@@ -802,7 +805,7 @@ __host__ __device__ inline LargeSmem large_smem(int tm, int cols_max, int R, int
   if (need < ring) need = ring;
   if (need < part) need = part;
   need += 1024;                // and the alignment to 1024
-  const size_t least = tm == 64 ? 81 * 1024 : 162 * 1024;   // tall tiles: four stages (76 us), three take 80
+  const size_t least = tm == 64 ? 81 * 1024 : 162 * 1024;   // tall tiles: four stages (76 us beside the QKV projection), three take 80
   return {hs, need > least ? need : least};
 }
 
@@ -1178,8 +1181,8 @@ void set_blocks(LoraArgs& a) {
 // K 512 to 14336, N 768 to 10240, ranks 8 to 128, 1 to 128 adapters) the choice
 // costs 1.1 % over the better one in the mean, 50 % at most; large tiles from 768
 // rows cost 7.9 % and up to six times.  Small / large, bf16, eight adapters, K = 4096,
-// three slices of together 6144 columns: rank 64, 128 rows 19.3 / 24.8 us, 384 rows
-// 30.1 / 27.1, 2048 rows 56.5 / 45.3; rank 16, 2048 rows 24.1 / 38.4.
+// three slices of together 6144 columns: rank 64, 128 rows 19.5 / 25.7 us, 384 rows
+// 29.9 / 28.0, 2048 rows 56.9 / 45.4; rank 16, 2048 rows 24.2 / 38.7.
 bool use_large(const LoraArgs& a) {
   if ((int64_t)a.pool * a.S * a.R > INT32_MAX) return false;   // rows of A are 32-bit coordinates
   const double small_tiles = (a.L + kSmallRows - 1) / kSmallRows, large_tiles = a.L / 64 + std::min(a.L, a.pool);
@@ -1216,8 +1219,10 @@ int clusters_at_once(Kernel kernel, int threads, int cl, size_t smem, std::atomi
 // CTAs per tile of the small kernel: as many as possible while the tiles still run in
 // the fewest waves, a wave costing about 6 us and, per CTA, 24 KB of weights a
 // microsecond.  The tiles are those of evenly used adapters.  64 adapters with a row
-// each, rank 16: clusters of 8 18.9 us, 6 22.9, 5 24.0, 4 14.7, 2 19.0; 512 rows of 20
-// adapters (40 tiles): 8 12.6, 6 7.7, 4 8.9, 2 10.1; one tile: 8 8.0, 4 10.0, 2 14.0.
+// each, rank 16: clusters of 8 18.5 us, 6 22.6, 5 23.9, 4 14.7, 2 19.8; 512 rows of 20
+// adapters (40 tiles, K = N = 4096): 8 13.8, 6 8.9, 4 10.0, 2 12.3; one tile: 8 8.0, 4 10.0,
+// 2 14.0.  Uneven use misleads it: 256 rows of 32 among 48 adapters (36 tiles, taken for 48,
+// K = 14336) run in clusters of 5, 24.9 us; 6 would take 22.8, 8 24.7, 4 26.5.
 template <typename AtOnce>
 int cluster_size(const LoraArgs& a, AtOnce at_once) {
   const int64_t adapters = std::min(a.L, a.pool);
@@ -1295,8 +1300,9 @@ struct Large {
 };
 
 // Tile and cluster by the number of waves and what one takes (us, ranks up to 64 beside
-// the QKV projection): 64 rows in clusters of 8 26, 4 45 (of 2 92, no better than two
-// waves of 4); 128 rows in clusters of 4 43, 2 76.
+// the QKV projection, K = 4096, N = 6144): 64 rows in clusters of 8 26, 4 45 (of 2 92, no
+// better than two waves of 4); 128 rows in clusters of 4 43, 2 76.  The ratios are taken for
+// every K, N and rank; other shapes were not measured.
 template <bool F32>
 void launch_large(const LoraArgs& a, cudaStream_t s) {
   const Large<F32, 64, 8> a8(a);

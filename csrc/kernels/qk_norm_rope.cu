@@ -148,9 +148,13 @@ __global__ void __launch_bounds__(NT) qk_norm_rope_kernel(const QkNormRopeArgs a
 }
 
 // Few tokens (two per SM at most) are bound by latency: 256 threads each, so that a
-// head group has one or two heads (256 rows of 48 heads of 128: 2.8 us, 3.7 with 64
-// threads).  Many are bound by memory: 64 threads, whose 1 KB rounds of loads and
-// stores interleave best (8192 rows: 37.2 us, 41.2 with 128, 69 with 256).
+// head group has one or two heads.  Many are bound by memory: 64 threads, whose 1 KB
+// rounds of loads and stores interleave best.  In between 128 threads would be better;
+// the rule ignores that.  us, head_dim 128, 64 / 128 / 256 threads:
+//
+//   tokens        256               300               600                1023               2000                8192
+//   32 + 8 heads  3.2 / 2.7 / 2.8   3.5 / 3.1 / 3.7   5.0 / 4.2 / 6.3    7.5 / 8.2 / 11.1   12.4 / 12.5 / 18.7  36.9 / 40.6 / 67.2
+//   64 + 8 heads  5.2 / 4.0 / 3.4   6.2 / 4.4 / 4.8   9.3 / 7.4 / 8.8   11.2 / 11.7 / 13.6  19.3 / 18.2 / 23.0
 template <int D>
 void launch_d(const QkNormRopeArgs& a, cudaStream_t s) {
   if (a.T <= 2 * sm_count()) launch_k(qk_norm_rope_kernel<D, 256>, dim3(a.T), dim3(256), 0, s, 1, a);

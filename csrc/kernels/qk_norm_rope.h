@@ -13,7 +13,7 @@ struct QkNormRopeArgs {
   const void* q_weight;       // [D] bf16
   const void* k_weight;       // [D] bf16
   const int32_t* positions;   // [T]
-  const int32_t* slots;       // [T]; -1: no K / V write
+  const int32_t* slots;       // [T]; negative: no K / V write
   const void* cos_sin;        // [max_pos, D / 2] float2
   void* kcache;               // [pages][Hkv][page][D] bf16
   void* vcache;

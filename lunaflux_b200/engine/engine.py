@@ -42,7 +42,8 @@ class EngineOptions:
     overlap_steps: bool = False            # plan and launch step n+1 before step n's tokens reach the host
     tp_sample_candidates: bool = False     # TP stochastic sampling from per-shard top-k candidates (top_k <= 64)
     moe_all_to_all: bool = False           # with sequence parallelism: experts by dispatch / combine all-to-all
-    sparse_pages: int = 0                  # decode attends to at most this many pages per KV head (0: all of them)
+    sparse_pages: int = 0                  # decode attends to at most this many pages per KV head (0: all of them);
+                                           # ranks that share a KV head select each for its own query heads
     sparse_first: int = 1                  # of these, the row's first pages ...
     sparse_last: int = 2                   # ... and its last ones are always taken, the others by score
 

@@ -112,7 +112,7 @@ class KernelOps:
         """RMS norm of every query and key head (one [D] weight each), split-half
         rotation and the paged K / V write in one pass; head_dim 64, 128 or 256.
         Q goes to ``q_out`` ([T, Hq * D]; ``qkv[:, :Hq * D]`` for in place), K and
-        V to the cache at ``slots`` (-1: no write; a slot appears at most once).
+        V to the cache at ``slots`` (negative: no write; a slot appears at most once).
         A position outside the table or a slot outside the cache is recorded in
         the error word."""
         if qkv.shape[0] == 0:
@@ -134,7 +134,11 @@ class KernelOps:
         are not listed and left as they are, entries behind ``starts[pool]``
         are not read (a captured step gives the list its bucket's length).  base and out are [T, N], both bf16
         or both fp32; out may be base.  ``slices`` are the column widths of a
-        stacked projection (e.g. Q, K, V), each with its own R rows of lora_a."""
+        stacked projection (e.g. Q, K, V), each with its own R rows of lora_a.
+        The same call gives the same bits; the last bits of a row depend on the
+        batch it comes in (its kernel, tiles and shares of K).  A bad row, offset
+        or rank is recorded in the error word; the rows it concerns are left as
+        they are or get base alone, the others their values."""
         if rows.numel() == 0:
             return
         self.launches += self.C.lora_add(x, lora_a, lora_b, scales, ranks, rows, starts, base, out,
@@ -172,7 +176,8 @@ class KernelOps:
         logical pages in ascending order, then -1.  All pages where they fit the
         budget; else the ``first`` first and ``last`` last ones and those of the
         highest upper bound max_h sum_d max(q_hd lo_d, q_hd hi_d) over the
-        group's query heads, compared exactly, ties to the lowest page.  ``ws``:
+        group's query heads, in the order of their sums in 64 bits, ties to the
+        lowest page (a page or query that holds an infinity or a NaN comes first).  ``ws``:
         ``select_workspace`` fp32 elements, used until the call's kernels end."""
         if seq_lens.numel() == 0:
             return
@@ -181,7 +186,7 @@ class KernelOps:
     def attn_decode_sparse(self, q, out, tok, seq_lens, bt, sel, kc, vc, Hq, Hkv):
         """Decode attention over the pages of ``sel``: the first
         min(pages of the row, budget) entries of every (row, KV head), each
-        page at most once.  A row of length 0 gives zeros; an entry outside the
+        page at most once, a token index too.  A row of length 0 gives zeros; an entry outside the
         row's pages is recorded in the error word and skipped."""
         if seq_lens.numel() == 0:
             return
