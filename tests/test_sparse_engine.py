@@ -228,3 +228,26 @@ def test_gpu_engine_over_selected_pages():
     assert graph.generate(prompts, 24) == eager.generate(prompts, 24)
     for e in (graph, eager):
         assert e.runner.ops.read_error(True)[0] == 0
+
+
+@pytest.mark.gpu
+def test_gpu_engine_launches_admitted(monkeypatch):
+    """Every launch of the engine over selected pages meets its contract; the tokens are the same."""
+    spec = LlamaSpec(hidden=1024, layers=2, heads=8, kv_heads=2, head_dim=128, ffn=2816, vocab=4096,
+                     rope_theta=500000.0, max_position=2048, dtype="bf16")
+    ck = {k: v.bfloat16().float() for k, v in random_checkpoint(spec, 1).items()}
+    prompts = _prompts(spec.vocab, (5, 70, 300, 33), seed=2)
+    want = _gpu_engine(spec, ck, 6, True).generate(prompts, 16)
+    monkeypatch.setenv("LUNAFLUX_CHECK_LAUNCHES", "1")
+    for graphs in (True, False):
+        eng = _gpu_engine(spec, ck, 6, graphs)
+        assert eng.generate(prompts, 16) == want
+        assert eng.runner.ops.read_error(True)[0] == 0
+
+
+@pytest.mark.gpu
+def test_gpu_engine_refuses_what_the_kernels_do_not_take():
+    spec = LlamaSpec(hidden=512, layers=1, heads=8, kv_heads=2, head_dim=64, ffn=512, vocab=256, max_position=1024, dtype="bf16")
+    ck = {k: v.bfloat16().float() for k, v in random_checkpoint(spec, 0).items()}
+    with pytest.raises(ValueError, match="head_dim 128"):
+        _gpu_engine(spec, ck, 6, False)
